@@ -112,6 +112,38 @@ class FileTensor(C.Structure):
                 ("shard", C.c_int), ("data", C.c_void_p)]
 
 
+class QkRopeArgs(C.Structure):
+    """cmf_qk_rope_args."""
+    _fields_ = [(n, C.c_void_p) for n in ("qkv", "q_out", "k", "v", "q_norm", "k_norm", "rope", "d_pos0", "d_depth")] + \
+        [("eps", C.c_double), ("head_stride", C.c_longlong), ("row_stride", C.c_longlong)] + \
+        [(n, C.c_int) for n in ("b", "nh", "nkv", "ldq", "ldo", "kv_dtype", "max_pos", "pos0", "slots", "at_pos")] + \
+        [("stream", C.c_void_p)]
+
+
+class AttentionArgs(C.Structure):
+    """cmf_attention_args."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "k", "v", "k_new", "v_new", "d_mask", "d_pos0", "d_depth", "ws")] + \
+        [("ws_bytes", C.c_size_t)] + \
+        [(n, C.c_longlong) for n in ("head_stride", "row_stride", "new_head_stride", "new_row_stride")] + \
+        [(n, C.c_int) for n in ("b", "nh", "nkv", "ldq", "ldo", "kv_dtype", "pos0", "slots", "len_bound", "window",
+                                "sinks")] + [("scale", C.c_float), ("stream", C.c_void_p)]
+
+
+class KvCopyArgs(C.Structure):
+    """cmf_kv_copy_args."""
+    _fields_ = [(n, C.c_void_p) for n in ("d_dst", "d_src", "d_idx", "d_n", "d_pos0")] + \
+        [(n, C.c_longlong) for n in ("dst_head_stride", "dst_row_stride", "src_head_stride", "src_row_stride")] + \
+        [(n, C.c_int) for n in ("nbuf", "nkv", "kv_dtype", "n", "pos0", "dst_slots", "src_slots")] + \
+        [("stream", C.c_void_p)]
+
+
+class LogprobsArgs(C.Structure):
+    """cmf_logprobs_args."""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "target", "logprob", "entropy", "top_ids", "top_lp", "ws")] + \
+        [("ws_bytes", C.c_size_t), ("ld", C.c_longlong)] + [(n, C.c_int) for n in ("rows", "V", "dtype", "top_k")] + \
+        [("stream", C.c_void_p)]
+
+
 # every symbol include/cmf_hip.h declares, with its ctypes signature
 _P, _I, _F, _S, _U64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
 SIGNATURES = {
@@ -177,6 +209,14 @@ SIGNATURES = {
     "cmf_state_get": (_I, [_P, C.POINTER(_I), _P]),
     "cmf_kv_export": (_I, [_P, _I, _I, _P, _P]),
     "cmf_model_set_embed": (_I, [_P, C.POINTER(Tensor)]),
+    # operators of drafted trees over a cache (csrc/cache_ops.hip, cache_attn.hip, logprobs.hip)
+    "cmf_qk_rope_dev": (_I, [C.POINTER(QkRopeArgs)]),
+    "cmf_attention_workspace": (_S, [C.POINTER(AttentionArgs)]),
+    "cmf_attention_dev": (_I, [C.POINTER(AttentionArgs)]),
+    "cmf_tree_masks": (_I, [_P, _I, _I, _I, _I, _P, _P]),
+    "cmf_kv_copy_dev": (_I, [C.POINTER(KvCopyArgs)]),
+    "cmf_logprobs_workspace": (_S, [C.POINTER(LogprobsArgs)]),
+    "cmf_logprobs_dev": (_I, [C.POINTER(LogprobsArgs)]),
     # .cmf container (csrc/container.cpp)
     "cmf_hash64": (_U64, [_P, _S]),
     "cmf_file_open": (_I, [C.c_char_p, C.POINTER(_P)]),

@@ -1,0 +1,443 @@
+// Attention of b rows (a tree of drafted tokens, or a chain) over a cache,
+// whole or through a sliding window with a few first positions that stay
+// visible (cmf_attention_dev).
+//
+// The query rows of one kv head are its queries qi = row * hpk + head (hpk =
+// query heads per kv head).  What a block of queries can see is two runs of
+// positions, [0, sinks) and [lo, hi); keys are numbered through both, and only
+// those are read.
+#include <math.h>
+
+#include <algorithm>
+#include <string>
+
+#include "cache_ops.h"
+#include "runtime.h"
+#include "wave.h"
+
+namespace cmf {
+
+namespace {
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr int HD = CACHE_HD;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float lanes4_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lanes4_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A call as the kernels take it.
+struct AttnCall {
+    cmf_attention_args a;
+    int hpk;         // query heads per kv head
+    int nsplit;      // key splits per query block; 1: the output itself
+    float qscale;    // scale * log2(e)
+    float *pm, *pl;  // [b * nh][nsplit] partial maxima (log2 units) and sums
+    float* po;       // [b * nh][nsplit][128], relative to the maximum
+};
+
+// The keys that the rows [r0, r1] of a block see, numbered [0, nv): positions
+// [0, s), then [lo, lo + nv - s).
+struct Keys {
+    int npos0;  // cached positions
+    int s, lo, nv;
+    int min_p, max_p;  // the rows' lowest and highest position
+    bool tree;
+    __device__ __forceinline__ int pos(int v) const { return v < s ? v : v - s + lo; }
+};
+
+__device__ __forceinline__ int cached_positions(const cmf_attention_args& a) {
+    int n = a.pos0;
+    if (a.d_pos0) n = min(n + *a.d_pos0, a.len_bound);
+    return max(0, min(n, a.slots));
+}
+
+__device__ __forceinline__ Keys keys_of(const cmf_attention_args& a, int r0, int r1) {
+    Keys k;
+    k.npos0 = cached_positions(a);
+    k.tree = a.d_mask != nullptr;
+    // a tree's rows lie at most 63 positions past the root: the bound for the
+    // range alone (d_depth is looked at row by row)
+    k.min_p = k.tree || a.d_depth ? k.npos0 : k.npos0 + r0;
+    k.max_p = k.tree || a.d_depth ? 0x3fffffff : k.npos0 + r1;
+    const int hi = k.npos0 + (k.tree ? a.b : r1 + 1);
+    k.lo = a.window ? max(0, min(k.min_p - a.window + 1, hi)) : 0;
+    if (k.tree) k.lo = min(k.lo, k.npos0);  // (new rows are the mask's alone)
+    k.s = min(a.sinks, k.lo);
+    k.nv = k.s + hi - k.lo;
+    return k;
+}
+
+template <class T>
+__device__ __forceinline__ void key_row(const cmf_attention_args& a, const Keys& k, int pos, int g, const T*& kp,
+                                        const T*& vp) {
+    if (pos < k.npos0 || !a.k_new) {
+        const size_t o = (size_t)g * a.head_stride + (size_t)pos * a.row_stride;
+        kp = (const T*)a.k + o;
+        vp = (const T*)a.v + o;
+    } else {
+        const size_t o = (size_t)g * a.new_head_stride + (size_t)(pos - k.npos0) * a.new_row_stride;
+        kp = (const T*)a.k_new + o;
+        vp = (const T*)a.v_new + o;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few queries per kv head (decode rows, small trees): the scores and values
+// in f32 on the 16x16x4 MFMA, K and V straight from memory into its operands.
+//
+// A wave takes 16 keys at a time for up to 16 QB queries, transposed so that
+// nothing goes through LDS: S^T = K Q^T (rows keys, columns queries), and the
+// weights come out in the lanes and registers that O^T = V^T P^T wants them
+// in (lane (n, kq) = query n, keys 4 kq + e in register e; the MFMA's k order
+// is free, so step e takes key 4 kq + e from lane group kq).  Lane (m, kq)
+// loads 8 consecutive dims 32 j + 8 kq of key m (K) and 16 bytes at a time of
+// keys 4 kq + e (V).  Softmax with a running maximum, one column a lane.
+// Four waves take a workgroup's 16-key tiles in turn and meet in LDS in wave
+// order.  f32 operands: no rounding of the inputs, any range.
+//
+// Bound by the cache's bytes: 16 KiB of f32 K/V per tile against 64 MFMAs of
+// 32 cycles per 16 queries.
+// grid (nsplit ceil(b hpk / 16 QB), nkv), block 256.
+// ---------------------------------------------------------------------------
+template <class T, int QB>
+__global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
+    const cmf_attention_args& a = c.a;
+    constexpr int NW = 4, QN = 16 * QB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, kq = lane >> 4, split = blockIdx.x % c.nsplit, g = blockIdx.y, q0 = blockIdx.x / c.nsplit * QN;
+    const int nq = a.b * c.hpk;
+    const int r0 = q0 / c.hpk, r1 = (min(q0 + QN, nq) - 1) / c.hpk;
+    const Keys ks = keys_of(a, r0, r1);
+
+    // this split's keys, whole rounds of the four waves
+    const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + 16 * NW - 1) / (16 * NW) * (16 * NW);
+    const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
+
+    // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n
+    float qf[QB][32];
+    int row[QB], P[QB];
+    uint64_t mask[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+        const int qi = min(q0 + 16 * qb + n, nq - 1), r = qi / c.hpk, h = g * c.hpk + qi - r * c.hpk;
+        row[qb] = r;
+        P[qb] = ks.npos0 + (a.d_depth ? a.d_depth[r] : r);
+        mask[qb] = ks.tree ? a.d_mask[r] : 0;
+        const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 8 * kq;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float t[8];
+            load8(q + 32 * j, t);
+#pragma unroll
+            for (int i = 0; i < 8; i++) qf[qb][8 * j + i] = t[i];
+        }
+    }
+
+    float4v acc[QB][8];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+        m[qb] = -INFINITY;
+        l[qb] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
+        // K row n, then V rows 4 kq + e (numbers past the end read the last key)
+        float kf[32], vf[4][8];
+        const T *kp, *vp;
+        key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float t[8];
+            load8(kp + 32 * j + 8 * kq, t);
+#pragma unroll
+            for (int i = 0; i < 8; i++) kf[8 * j + i] = t[i];
+        }
+        // dims of component i of lane m: f32 64 (i / 4) + 4 m + i % 4, else 8 m + i
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const T *kp2, *vp2;
+            key_row(a, ks, ks.pos(min(v0 + 4 * kq + e, ks.nv - 1)), g, kp2, vp2);
+            if constexpr (sizeof(T) == 4) {
+                const float4 x = ((const float4*)vp2)[n], y = ((const float4*)vp2)[16 + n];
+                vf[e][0] = x.x, vf[e][1] = x.y, vf[e][2] = x.z, vf[e][3] = x.w;
+                vf[e][4] = y.x, vf[e][5] = y.y, vf[e][6] = y.z, vf[e][7] = y.w;
+            } else {
+                load8(vp2 + 8 * n, vf[e]);
+            }
+        }
+        // infinities and NaN in V (0 * v is NaN then): such a tile's values go
+        // by comparisons, not by products with weights of zero
+        float odd = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) odd = fmaf(vf[e][i], 0.f, odd);
+        const bool finite = __builtin_amdgcn_ballot_w64(odd != odd) == 0;
+
+#pragma unroll
+        for (int qb = 0; qb < QB; qb++) {
+            float4v s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[qb][i], s, 0, 0, 0);
+            float mx = m[qb];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int v = v0 + 4 * kq + e, pos = ks.pos(v);
+                const int j = pos - ks.npos0;
+                const bool near = !a.window || pos > P[qb] - a.window || pos < a.sinks;
+                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask[qb] >> (j & 63) & 1) : (j <= row[qb] && near));
+                s[e] = vis ? s[e] * c.qscale : -INFINITY;
+                mx = fmaxf(mx, s[e]);
+            }
+            mx = lanes4_max(mx);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            const float al = exp2f(m[qb] - ref);
+            m[qb] = mx;
+            float4v p;
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] = exp2f(s[e] - ref);
+            l[qb] = l[qb] * al + (p[0] + p[1] + p[2] + p[3]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[qb][i] *= al;
+            if (finite) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        acc[qb][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][i], p[e], acc[qb][i], 0, 0, 0);
+            } else {
+                // output row 4 kq + e2 of block i is component i of lane 4 kq + e2
+                for (int k = 0; k < 16; k++) {
+                    const int e = k & 3, from = (lane & 15) + 16 * (k >> 2);
+                    const float pe = e == 0 ? p[0] : e == 1 ? p[1] : e == 2 ? p[2] : p[3];
+                    const float se = e == 0 ? s[0] : e == 1 ? s[1] : e == 2 ? s[2] : s[3];
+                    const float pk = __shfl(pe, from), sk = __shfl(se, from);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float ve = e == 0 ? vf[0][i] : e == 1 ? vf[1][i] : e == 2 ? vf[2][i] : vf[3][i];
+#pragma unroll
+                        for (int e2 = 0; e2 < 4; e2++) {
+                            const float vv = __shfl(ve, 16 * (k >> 2) + 4 * kq + e2);
+                            acc[qb][i][e2] += sk == -INFINITY ? 0.f : pk * vv;
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // the four waves' states, in wave order
+    __shared__ float sm[NW][QN], sl[NW][QN];
+    __shared__ __align__(16) float so[NW][QN][HD + 4];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+        const float lt = lanes4_sum(l[qb]);
+        if (kq == 0) {
+            sm[wave][16 * qb + n] = m[qb];
+            sl[wave][16 * qb + n] = lt;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int r = 4 * kq + e;
+                so[wave][16 * qb + n][sizeof(T) == 4 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[qb][i][e];
+            }
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < QN * 32; t += 256) {
+        const int qq = t >> 5, d = (t & 31) * 4, qi = q0 + qq;
+        if (qi >= nq) continue;
+        float M = sm[0][qq];
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, sm[w][qq]);
+        float L = 0.f;
+        float4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = sm[w][qq] == -INFINITY ? 0.f : exp2f(sm[w][qq] - M);
+            L += sl[w][qq] * f;
+            const float4v x = *(const float4v*)&so[w][qq][d];
+            if (sm[w][qq] != -INFINITY) o += x * f;
+        }
+        const int r = qi / c.hpk, h = g * c.hpk + qi - r * c.hpk;
+        if (c.nsplit == 1) {
+            const float inv = L == 0.f ? 0.f : 1.0f / L;
+            *(float4v*)(a.out + (size_t)r * a.ldo + (size_t)h * HD + d) = o * inv;
+        } else {
+            const size_t rh = (size_t)r * a.nh + h;
+            *(float4v*)(c.po + (rh * c.nsplit + split) * HD + d) = o;
+            if (d == 0) {
+                c.pm[rh * c.nsplit + split] = M;
+                c.pl[rh * c.nsplit + split] = L;
+            }
+        }
+    }
+}
+
+// The splits of one (row, head) by one wave: out = sum w_c o_c / sum w_c l_c,
+// w_c = 2^(m_c - M); lane = dim pair.  Bound by latency.  grid (b nh / 4).
+__global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
+    const cmf_attention_args& a = c.a;
+    const int lane = threadIdx.x & 63;
+    const size_t rh = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (rh >= (size_t)a.b * a.nh) return;
+    const int ns = c.nsplit;
+    const float* pm = c.pm + rh * ns;
+    const float* pl = c.pl + rh * ns;
+    const float2* po = (const float2*)(c.po + rh * ns * HD);
+    float M = -INFINITY;
+    for (int j = lane; j < ns; j += 64) M = fmaxf(M, pm[j]);
+    M = wave_max(M);
+    float L = 0.f;
+    float2 o = make_float2(0.f, 0.f);
+    for (int j0 = 0; j0 < ns; j0 += 64) {
+        const int j = j0 + lane;
+        const float mj = j < ns ? pm[j] : -INFINITY, lj = j < ns ? pl[j] : 0.f;
+        const float w = mj == -INFINITY ? 0.f : exp2f(mj - M);
+        L += wave_sum(w * lj);
+        const int je = min(64, ns - j0);
+        for (int t0 = 0; t0 < je; t0 += 8) {
+            float2 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) x[u] = po[(size_t)(j0 + min(t0 + u, je - 1)) * 64 + lane];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float wu = __shfl(w, min(t0 + u, 63));
+                const float mu = __shfl(mj, min(t0 + u, 63));
+                if (t0 + u < je && mu != -INFINITY) {
+                    o.x += wu * x[u].x;
+                    o.y += wu * x[u].y;
+                }
+            }
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const size_t r = rh / a.nh, h = rh - r * a.nh;
+    ((float2*)(a.out + r * a.ldo + h * HD))[lane] = make_float2(o.x * inv, o.y * inv);
+}
+
+// the most keys that a block of rows may have to read
+long long keys_bound(const cmf_attention_args& a, int rows) {
+    const long long cached = a.d_pos0 ? std::min(a.len_bound, a.slots) : a.pos0;
+    long long n = cached + (a.d_mask ? a.b : std::min(a.b, rows));
+    if (!a.d_mask && !a.d_depth && !a.d_pos0) n = cached + a.b;
+    if (a.window) n = std::min(n, (long long)a.sinks + a.window + (a.d_mask || a.d_depth ? a.b : rows));
+    return std::max(1ll, n);
+}
+
+struct Plan {
+    int qb = 1, groups = 1, nsplit = 1;
+    size_t bytes = 0;
+};
+
+Plan plan_of(const cmf_attention_args& a) {
+    Plan p;
+    const long long nq = (long long)a.b * (a.nh / a.nkv);
+    p.qb = nq <= 16 ? 1 : 2;
+    p.groups = (int)((nq + 16 * p.qb - 1) / (16 * p.qb));
+    const int rows = std::min<long long>(a.b, 16 * p.qb / (a.nh / a.nkv) + 2);
+    const long long nv = keys_bound(a, rows);
+    // about two workgroups a CU; a split of at least 64 keys
+    long long ns = 512 / std::max(1ll, (long long)a.nkv * p.groups);
+    ns = std::max(1ll, std::min(ns, (nv + 63) / 64));
+    const size_t per = (size_t)a.b * a.nh * (HD + 2) * sizeof(float);
+    while (ns > 1 && per * ns > OP_WS_MAX) ns--;
+    p.nsplit = (int)ns;
+    p.bytes = ns > 1 ? per * ns : 0;
+    return p;
+}
+
+template <class T>
+void launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
+    const dim3 grid((unsigned)c.nsplit * p.groups, c.a.nkv);
+    if (p.qb == 1) hipLaunchKernelGGL((k_attn_rows<T, 1>), grid, dim3(256), 0, s, c);
+    else hipLaunchKernelGGL((k_attn_rows<T, 2>), grid, dim3(256), 0, s, c);
+}
+
+}  // namespace
+
+size_t cache_attention_ws(const cmf_attention_args& a) { return plan_of(a).bytes; }
+
+int launch_cache_attention(const cmf_attention_args& a, hipStream_t s) {
+    const Plan p = plan_of(a);
+    if (p.bytes > a.ws_bytes || (p.bytes && !a.ws)) return fail("attention: the workspace is too small (cmf_attention_workspace)");
+    AttnCall c{a, a.nh / a.nkv, p.nsplit, (a.scale == 0.f ? 0.08838834764831845f : a.scale) * LOG2E, nullptr, nullptr, nullptr};
+    if (p.nsplit > 1) {
+        const size_t rh = (size_t)a.b * a.nh * p.nsplit;
+        c.po = (float*)a.ws;
+        c.pm = c.po + rh * HD;
+        c.pl = c.pm + rh;
+    }
+    if (a.kv_dtype == CMF_DT_F32) launch_t<float>(c, p, s);
+    else if (a.kv_dtype == CMF_DT_F16) launch_t<_Float16>(c, p, s);
+    else launch_t<bf16_t>(c, p, s);
+    if (p.nsplit > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(((size_t)a.b * a.nh + 3) / 4)), dim3(256), 0, s, c);
+    return CMF_OK;
+}
+
+static int check_attention(const cmf_attention_args* p) {
+    if (!p) return fail("attention: null argument");
+    const auto& a = *p;
+    if (a.b < 1 || a.nh < 1 || a.nkv < 1 || a.nh % a.nkv) return fail("attention: b, nh, nkv of at least 1, nh a multiple of nkv");
+    if (a.b > (1 << 20) || a.nh > 4096) return fail("attention: at most 2^20 rows and 4096 heads");
+    if (!kv_dtype_ok(a.kv_dtype)) return fail("attention: kv_dtype must be f32, f16 or bf16");
+    if (a.pos0 < 0 || a.slots < 0 || a.window < 0 || a.sinks < 0) return fail("attention: pos0, slots, window and sinks of at least 0");
+    if (a.slots > (1 << 30) || a.window > (1 << 30) || a.sinks > (1 << 30)) return fail("attention: at most 2^30 positions");
+    if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) return fail("attention: scale must be finite");
+    if (a.d_mask && a.b > CMF_TREE_MAX) return fail("attention: a tree of at most 64 rows");
+    if (a.d_depth && !a.d_mask) return fail("attention: d_depth goes with d_mask");
+    if (a.d_mask && a.window && !a.d_depth) return fail("attention: a tree under a window needs d_depth");
+    if (!a.k_new != !a.v_new) return fail("attention: k_new and v_new go together");
+    if (a.ldq < a.nh * HD || a.ldq % 4 || a.ldo < a.nh * HD || a.ldo % 4) return fail("attention: ldq and ldo must hold the heads, multiples of 4");
+    if (a.row_stride < HD || a.row_stride % 8 || a.head_stride < 0 || a.head_stride % 8 ||
+        (a.k_new && (a.new_row_stride < HD || a.new_row_stride % 8 || a.new_head_stride < 0 || a.new_head_stride % 8)))
+        return fail("attention: strides must be multiples of 8 elements, rows of 128");
+    const long long need = (long long)a.pos0 + (a.k_new ? 0 : a.b);
+    if (!a.d_pos0 && need > a.slots) return fail("attention: positions past the cache's slots");
+    if (a.d_pos0 && (a.len_bound < 0 || (long long)a.len_bound + (a.k_new ? 0 : a.b) > a.slots))
+        return fail("attention: len_bound past the cache's slots");
+    return CMF_OK;
+}
+
+}  // namespace cmf
+
+using namespace cmf;
+
+extern "C" {
+
+size_t cmf_attention_workspace(const cmf_attention_args* a) {
+    if (check_attention(a) != CMF_OK) return 0;
+    return cache_attention_ws(*a);
+}
+
+int cmf_attention_dev(const cmf_attention_args* p) {
+    if (check_attention(p) != CMF_OK) return CMF_ERR;
+    const auto& a = *p;
+    if (!a.q || !a.out || ((!a.k || !a.v) && (a.slots > 0 || !a.k_new))) return fail("attention: null q, out, k or v");
+    for (const void* x : {(const void*)a.q, (const void*)a.out, a.k, a.v, a.k_new, a.v_new, (const void*)a.ws})
+        if (!aligned16(x)) return fail("attention: 16-byte aligned tensors");
+    OpScope sc;
+    if (sc.enter(a.stream, "attention") != CMF_OK) return CMF_ERR;
+    if (launch_cache_attention(a, sc.s) != CMF_OK) return CMF_ERR;
+    CMF_HIP(hipGetLastError());
+    return CMF_OK;
+}
+
+}  // extern "C"

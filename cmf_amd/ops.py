@@ -1,0 +1,278 @@
+"""Operators on device tensors around the verification of drafted tokens
+(libcmfhip cmf_*_dev): head norms with the rotation, attention of a token tree
+or through a sliding window over a cache, copies of cache rows, and log
+probabilities.
+
+The functions take device tensors by their pointers: anything with data_ptr(),
+shape, stride() and dtype, as DevTensor below or torch tensors (a process that
+uses torch on the GPU imports it before this library is loaded: both bring a
+HIP runtime, and the first one serves both).  Head rows have 128 elements and
+are contiguous; activations are f32, caches and logits f32, f16 or bf16.
+Nothing is allocated, checked on the device or waited for; outputs are written
+in place.  stream: None for the calling thread's library stream
+(cmf_amd.lib().cmf_sync() waits for it), or a HIP stream handle (torch:
+stream.cuda_stream; 0 is the null stream).  Raises CmfError when the library
+refuses the arguments.
+"""
+import ctypes as C
+
+import numpy as np
+
+from . import AttentionArgs, CmfError, DevBuf, KvCopyArgs, LogprobsArgs, QkRopeArgs, _ptr, check, lib
+
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+_DTYPES = {"torch.float32": DT_F32, "torch.float16": DT_F16, "torch.bfloat16": DT_BF16, "float32": DT_F32,
+           "float16": DT_F16, "bfloat16": DT_BF16}
+STREAM_NULL = 1  # CMF_STREAM_NULL
+WORKSPACE_MAX = 64 << 20  # no call asks for more scratch
+
+
+class DevTensor:
+    """A device tensor of the library: a strided view of a DevBuf."""
+    SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "int64": 8, "uint64": 8, "uint8": 1}
+
+    def __init__(self, buf, shape, strides, dtype, offset=0):
+        self.buf, self.shape, self._strides, self.dtype, self.offset = buf, tuple(shape), tuple(strides), dtype, offset
+
+    @classmethod
+    def of(cls, array, dtype=None):
+        """A numpy array on the device, as `dtype` (its own; f32 arrays also
+        rounded to float16 or bfloat16)."""
+        dtype = dtype or str(array.dtype)
+        a = np.ascontiguousarray(array)
+        if dtype == "bfloat16":
+            u = a.astype(np.float32).view(np.uint32)
+            up = ((u.astype(np.uint64) + 0x7fff + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+            a = np.where(np.isnan(a), np.uint16(0x7fc0), up)
+        else:
+            a = a.astype(dtype)
+        t = cls.empty(a.shape, dtype)
+        if a.size:
+            t.buf.upload(a)
+        return t
+
+    @classmethod
+    def empty(cls, shape, dtype="float32"):
+        shape = (shape,) if isinstance(shape, int) else tuple(shape)
+        strides = [int(np.prod(shape[i + 1:], dtype=np.int64)) for i in range(len(shape))]
+        n = int(np.prod(shape, dtype=np.int64))
+        return cls(DevBuf(max(16, n * cls.SIZES[dtype])), shape, strides, dtype)
+
+    def data_ptr(self):
+        return self.buf.p + self.offset * self.element_size()
+
+    def element_size(self):
+        return self.SIZES[self.dtype]
+
+    def stride(self):
+        return self._strides
+
+    def __getitem__(self, key):
+        key = key if isinstance(key, tuple) else (key,)
+        shape, strides, off = [], [], self.offset
+        for i, (n, st) in enumerate(zip(self.shape, self._strides)):
+            k = key[i] if i < len(key) else slice(None)
+            if isinstance(k, slice):
+                lo, hi, step = k.indices(n)
+                off += lo * st
+                shape.append(max(0, -(-(hi - lo) // step)))
+                strides.append(st * step)
+            else:
+                off += (k % n) * st
+        return DevTensor(self.buf, shape, strides, self.dtype, off)
+
+    def permute(self, *axes):
+        return DevTensor(self.buf, [self.shape[i] for i in axes], [self._strides[i] for i in axes], self.dtype, self.offset)
+
+    def numpy(self):
+        """The values on the host (16-bit floats as f32); waits for the calling
+        thread's library stream."""
+        check(lib().cmf_sync())
+        raw = {"bfloat16": "uint16"}.get(self.dtype, self.dtype)
+        flat = self.buf.download(self.buf.nbytes // self.element_size(), raw)
+        es = self.element_size()
+        a = np.lib.stride_tricks.as_strided(flat[self.offset:], self.shape, [s * es for s in self._strides]).copy()
+        if self.dtype == "bfloat16":
+            return (a.astype(np.uint32) << 16).view(np.float32)
+        return a.astype(np.float32) if self.dtype == "float16" else a
+
+
+def _dt(t):
+    try:
+        return _DTYPES[str(t.dtype)]
+    except KeyError:
+        raise CmfError(f"dtype {t.dtype}: f32, f16 or bf16") from None
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(s):
+    return None if s is None else (s or STREAM_NULL)
+
+
+def _want(ok, what):
+    if not ok:
+        raise CmfError(what)
+
+
+def _f32(t, what):
+    _want(_dt(t) == DT_F32, f"{what} must be f32")
+
+
+def _i32(t, n, what):
+    if t is not None:
+        _want(str(t.dtype) in ("torch.int32", "int32") and t.stride()[-1] == 1 and t.shape[0] >= n,
+              f"{what} must be int32, contiguous, of at least {n}")
+
+
+def _cache(k, v, what):
+    """k and v [nkv][slots][128] of one layout -> (nkv, slots, head, row)."""
+    _want(len(k.shape) == 3 and k.shape[2] == 128 and k.stride()[2] == 1, f"{what} must be [heads][rows][128]")
+    _want(k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype, f"{what}: k and v differ in layout")
+    return k.shape[0], k.shape[1], k.stride()[0], k.stride()[1]
+
+
+def _rows(t, what):
+    """t [b][heads][128] -> (b, heads, ld)."""
+    _want(len(t.shape) == 3 and t.shape[2] == 128 and t.stride()[2] == 1 and (t.shape[1] == 1 or t.stride()[1] == 128),
+          f"{what} must be [rows][heads][128] with contiguous heads")
+    b, h, _ = t.shape
+    return b, h, t.stride()[0] if b > 1 else max(t.stride()[0], h * 128)
+
+
+def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=None, at_pos=True, eps=1e-6, stream=None):
+    """cmf_qk_rope_dev: qkv [b][nh + 2 nkv][128], q [b][nh][128], k / v
+    [nkv][slots][128], rope [positions][64][2] (cos, sin).  Row i at position
+    pos0 + depth[i] (depth None: i; pos0_dev: an int32 tensor whose value is
+    added); its key and value go to row pos0 + i, or row i with
+    at_pos=False."""
+    b, hs, ldq = _rows(qkv, "qkv")
+    nkv, slots, hst, rst = _cache(k, v, "k / v")
+    bq, nh, ldo = _rows(q, "q")
+    _want(bq == b and hs == nh + 2 * nkv, "qkv must hold nh + 2 nkv heads of every row of q")
+    for t, w in ((qkv, "qkv"), (q, "q"), (rope, "rope")):
+        _f32(t, w)
+    for t in (q_norm, k_norm):
+        if t is not None:
+            _f32(t, "the norms")
+            _want(tuple(t.shape) == (128,) and t.stride()[0] == 1, "the norms must be [128]")
+    _want(tuple(rope.shape[1:]) == (64, 2) and tuple(rope.stride()) == (128, 2, 1), "rope must be [positions][64][2], contiguous")
+    _i32(depth, b, "depth")
+    _i32(pos0_dev, 1, "pos0_dev")
+    a = QkRopeArgs(_p(qkv), _p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(rope), _p(pos0_dev), _p(depth), eps, hst, rst,
+                   b, nh, nkv, ldq, ldo, _dt(k), rope.shape[0], pos0, slots, 1 if at_pos else 0, _stream(stream))
+    check(lib().cmf_qk_rope_dev(C.byref(a)))
+
+
+def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream):
+    b, nh, ldq = _rows(q, "q")
+    nkv, slots, hst, rst = _cache(k, v, "k / v")
+    _want(nkv >= 1 and nh % nkv == 0, "the query heads must be a multiple of the kv heads")
+    _f32(q, "q")
+    ldo = nh * 128
+    if out is not None:
+        _f32(out, "out")
+        bo, ho, ldo = _rows(out, "out")
+        _want((bo, ho) == (b, nh), "out must be shaped as q")
+    nhst = nrst = 0
+    if k_new is not None:
+        nk, rows, nhst, nrst = _cache(k_new, v_new, "k_new / v_new")
+        _want(nk == nkv and rows >= b and k_new.dtype == k.dtype, "k_new / v_new must hold b rows of k's type")
+    if mask is not None:
+        _want(str(mask.dtype) in ("torch.int64", "torch.uint64", "int64", "uint64") and mask.shape[0] >= b and
+              mask.stride()[0] == 1, "mask must be [b] of 64 bits")
+    _i32(depth, b, "depth")
+    _i32(pos0_dev, 1, "pos0_dev")
+    nb = 0 if ws is None else ws.shape[0] * ws.element_size()
+    return AttentionArgs(_p(q), _p(out), _p(k), _p(v), _p(k_new), _p(v_new), _p(mask), _p(pos0_dev), _p(depth), _p(ws), nb,
+                         hst, rst, nhst, nrst, b, nh, nkv, ldq, ldo, _dt(k), pos0, slots, len_bound, window, sinks, scale,
+                         _stream(stream))
+
+
+def attention_workspace(q, k, v, *, pos0=0, k_new=None, v_new=None, mask=None, depth=None, window=0, sinks=0,
+                        pos0_dev=None, len_bound=0):
+    """cmf_attention_workspace: bytes of scratch the call of these arguments
+    needs (never more than WORKSPACE_MAX)."""
+    a = _attention_args(q, k, v, None, None, pos0, k_new, v_new, mask, depth, window, sinks, 0.0, pos0_dev, len_bound, None)
+    return lib().cmf_attention_workspace(C.byref(a))
+
+
+def attention(q, k, v, out, ws, *, pos0=0, k_new=None, v_new=None, mask=None, depth=None, window=0, sinks=0, scale=0.0,
+              pos0_dev=None, len_bound=0, stream=None):
+    """cmf_attention_dev: q and out [b][nh][128]; k / v [nkv][slots][128] hold
+    pos0 cached positions; the rows' own keys and values are k_new / v_new
+    [nkv][>= b][128], or the cache's rows pos0 .. pos0 + b.  mask (int64 bits,
+    with depth under a window): a tree's visible new rows (tree_masks); without
+    it row i sees the rows up to its own.  window, sinks: only the last window
+    positions and the first sinks are seen (window 0: all).  ws: 1-d scratch
+    tensor of attention_workspace bytes (None: nothing)."""
+    a = _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream)
+    check(lib().cmf_attention_dev(C.byref(a)))
+
+
+def tree_masks(parents, pos0=0, window=0, sinks=0):
+    """cmf_tree_masks: (mask uint64 [b], depth int32 [b]) of the tree whose row
+    i has the earlier row parents[i] as its parent (-1: a root)."""
+    p = np.ascontiguousarray(parents, dtype=np.int32)
+    m, d = np.empty(len(p), np.uint64), np.empty(len(p), np.int32)
+    check(lib().cmf_tree_masks(_ptr(p), len(p), pos0, window, sinks, _ptr(m), _ptr(d)))
+    return m, d
+
+
+def kv_copy(dst_ptrs, src_ptrs, dst, src, *, n, pos0=0, idx=None, n_dev=None, pos0_dev=None, stream=None):
+    """cmf_kv_copy_dev: row pos0 + i of every buffer of dst_ptrs = row idx[i]
+    (None: i) of the buffer of src_ptrs, i < n (n_dev: and < its value).
+    dst_ptrs / src_ptrs: int64 device tensors of base pointers; dst / src: one
+    of the buffers of each side, [nkv][slots][128], for the layout."""
+    nkv, ds, dh, dr = _cache(dst, dst, "dst")
+    nk, ss, sh, sr = _cache(src, src, "src")
+    _want(nk == nkv and src.dtype == dst.dtype, "dst and src must have the same heads and type")
+    for t in (dst_ptrs, src_ptrs):
+        _want(str(t.dtype) in ("torch.int64", "int64") and t.stride()[0] == 1, "pointers must be int64, contiguous")
+    _want(dst_ptrs.shape[0] == src_ptrs.shape[0], "as many buffers on both sides")
+    _i32(idx, n, "idx")
+    _i32(n_dev, 1, "n_dev")
+    _i32(pos0_dev, 1, "pos0_dev")
+    a = KvCopyArgs(_p(dst_ptrs), _p(src_ptrs), _p(idx), _p(n_dev), _p(pos0_dev), dh, dr, sh, sr, dst_ptrs.shape[0], nkv,
+                   _dt(dst), n, pos0, ds, ss, _stream(stream))
+    check(lib().cmf_kv_copy_dev(C.byref(a)))
+
+
+def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws, stream):
+    _want(len(logits.shape) == 2 and logits.stride()[1] == 1, "logits must be [rows][V]")
+    rows, V = logits.shape
+    _i32(target, rows, "target")
+    for t, w in ((logprob, "logprob"), (entropy, "entropy")):
+        if t is not None:
+            _f32(t, w)
+            _want(t.shape[0] >= rows and t.stride()[0] == 1, f"{w} must be [rows]")
+    for t, w in ((top_ids, "top_ids"), (top_lp, "top_lp")):
+        if t is not None:
+            _want(len(t.shape) == 2 and t.shape[0] >= rows and t.shape[1] == top_k and tuple(t.stride()) == (top_k, 1),
+                  f"{w} must be [rows][top_k], contiguous")
+    if top_ids is not None:
+        _want(str(top_ids.dtype) in ("torch.int32", "int32"), "top_ids must be int32")
+    if top_lp is not None:
+        _f32(top_lp, "top_lp")
+    nb = 0 if ws is None else ws.shape[0] * ws.element_size()
+    return LogprobsArgs(_p(logits), _p(target), _p(logprob), _p(entropy), _p(top_ids), _p(top_lp), _p(ws), nb,
+                        logits.stride()[0] if rows > 1 else max(logits.stride()[0], V), rows, V, _dt(logits), top_k,
+                        _stream(stream))
+
+
+def logprobs_workspace(logits, top_k=0):
+    """cmf_logprobs_workspace: bytes of scratch for these logits."""
+    a = _logprobs_args(logits, None, None, None, None, None, top_k, None, None)
+    return lib().cmf_logprobs_workspace(C.byref(a))
+
+
+def logprobs(logits, target=None, logprob=None, entropy=None, top_ids=None, top_lp=None, ws=None, *, stream=None):
+    """cmf_logprobs_dev: logits [rows][V]; target int32 [rows] -> logprob f32
+    [rows]; entropy f32 [rows] (nats); top_ids int32 / top_lp f32 [rows][k] the
+    k most likely tokens (equal logits: the lowest id first).  Any output may be
+    None.  ws: 1-d scratch tensor of logprobs_workspace bytes."""
+    top = top_ids if top_ids is not None else top_lp
+    a = _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, 0 if top is None else top.shape[1], ws, stream)
+    check(lib().cmf_logprobs_dev(C.byref(a)))

@@ -377,6 +377,130 @@ int cmf_kv_export(cmf_model m, int li, int n, float* k, float* v);
 int cmf_time_attention(cmf_model m, int nb, int pos0, int merge, int iters, float* avg_ms);
 
 
+/* ---- operators of drafted trees over a cache (device pointers) --------- */
+/* No counterpart in the reference, whose drafts are a chain
+ * (pipeline.rs:3582-4213): the pieces of cmf_verify_tree, cmf_score and
+ * cmf_model_set_window for callers that hold their own activations and caches.
+ * Heads have 128 dims.  Activations are f32; caches and logits are f32, f16 or
+ * bf16 (the ids of the reference's dense tensors, types.rs:10-90).  Every call
+ * checks its arguments first (an error leaves the outputs as they were), then
+ * enqueues its kernels on `stream` and returns: it allocates nothing, waits
+ * for nothing and may be captured into a graph.  stream is a hipStream_t of
+ * the library's device; NULL: the calling thread's library stream;
+ * CMF_STREAM_NULL: the device's null stream.  Pointers named d_* and all
+ * tensors are device memory of the library's device, 16-byte aligned where a
+ * row of heads starts (strides: multiples of 8 elements). */
+#define CMF_DT_F32 0
+#define CMF_DT_F16 1
+#define CMF_DT_BF16 2
+#define CMF_STREAM_NULL ((void*)1)
+#define CMF_TREE_MAX 64 /* rows of a tree */
+#define CMF_TOP_MAX 64  /* top alternatives of a row of logits */
+
+/* The norm of every query and key head and the position rotation in one
+ * pass (rmsnorm_head + rope_rotate, attention.rs:606-624, 71-81):
+ *   y = x / sqrt(mean(x^2) + eps) * w        (q_norm / k_norm NULL: y = x)
+ *   (y[i], y[i + 64]) -> (a cos - b sin, a sin + b cos)
+ * Row i of qkv [b][ldq] (nh query, nkv key, nkv value heads) sits at position
+ * pos0 + (d_depth ? d_depth[i] : i), where d_pos0 adds a value read on the
+ * device (captured calls).  rope: (cos, sin) [max_pos][64]; a row whose
+ * position lies outside it is not written.  q_out [b][ldo]; the row's key and
+ * value (value as projected) go to row (at_pos ? pos0 + i : i) of k / v,
+ * rounded to kv_dtype; rows outside [0, slots) are not written.  k = v = NULL:
+ * queries only; q_out = NULL: keys and values only. */
+typedef struct {
+    const float* qkv;
+    float* q_out;
+    void *k, *v;
+    const float *q_norm, *k_norm, *rope;
+    const int32_t *d_pos0, *d_depth;
+    double eps;
+    long long head_stride, row_stride; /* of k and v, in elements */
+    int b, nh, nkv, ldq, ldo, kv_dtype, max_pos, pos0, slots, at_pos;
+    void* stream;
+} cmf_qk_rope_args;
+int cmf_qk_rope_dev(const cmf_qk_rope_args* a);
+
+/* Attention of b rows over a cache (attend_group, kv_cache.rs:521-690):
+ *   out_i = sum_x p_ix v_x,   p_i = softmax over the visible x of scale q_i.k_x
+ * The cache holds pos0 positions (d_pos0 adds a value read on the device, at
+ * most len_bound positions then); position x of kv head g is row x of
+ * k / v + g * head_stride.  The b new rows are k_new / v_new (row j of head g
+ * at g * new_head_stride + j * new_row_stride), or, where these are NULL, the
+ * cache's rows pos0 + j.  Row i sits at position P = pos0 + i, or pos0 +
+ * d_depth[i], and sees
+ *   the cached x with window == 0 or x > P - window or x < sinks;
+ *   the new rows j by bit j of d_mask[i] (b <= 64: cmf_tree_masks), or without
+ *   d_mask the rows j <= i under the same window (positions pos0 + j).
+ * A row that sees nothing gets zeros.  What a row does not see may hold
+ * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  ws: scratch of
+ * at least cmf_attention_workspace bytes (at most 64 MiB) that no other call
+ * uses meanwhile; captured graphs that may run at the same time need one
+ * each. */
+typedef struct {
+    const float* q;
+    float* out;
+    const void *k, *v, *k_new, *v_new;
+    const uint64_t* d_mask;
+    const int32_t *d_pos0, *d_depth;
+    void* ws;
+    size_t ws_bytes;
+    long long head_stride, row_stride, new_head_stride, new_row_stride; /* in elements */
+    int b, nh, nkv, ldq, ldo, kv_dtype, pos0, slots, len_bound, window, sinks;
+    float scale;
+    void* stream;
+} cmf_attention_args;
+size_t cmf_attention_workspace(const cmf_attention_args* a);
+int cmf_attention_dev(const cmf_attention_args* a);
+/* The masks and depths of a tree of b <= 64 rows given by parents (parent[i] <
+ * i; -1: a root), host arrays: bit j of mask[i] for row i itself and its
+ * ancestors, those nearer than window rows up where window > 0, and
+ * sinks - pos0 rows from the root where sinks reach past pos0. */
+int cmf_tree_masks(const int32_t* parent, int b, int pos0, int window, int sinks, uint64_t* mask, int32_t* depth);
+
+/* Rows copied between caches, all buffers in one launch: for every buffer j <
+ * nbuf and head g, row pos0 + i of dst[j] = row idx[i] of src[j] (d_idx NULL:
+ * row i), i < n, or i < *d_n where that is less.  d_dst / d_src: device arrays
+ * of nbuf base pointers; d_pos0 adds a value read on the device.  Rows outside
+ * [0, dst_slots) or [0, src_slots) are skipped, all others left as they were.
+ * dst and src must not overlap.  The commit of an accepted path
+ * (kv_cache.rs:883) out of a tree's rows, or a cache's prefix forked into
+ * another. */
+typedef struct {
+    void* const* d_dst;
+    const void* const* d_src;
+    const int32_t *d_idx, *d_n, *d_pos0;
+    long long dst_head_stride, dst_row_stride, src_head_stride, src_row_stride; /* in elements */
+    int nbuf, nkv, kv_dtype, n, pos0, dst_slots, src_slots;
+    void* stream;
+} cmf_kv_copy_args;
+int cmf_kv_copy_dev(const cmf_kv_copy_args* a);
+
+/* Of every row x of logits [rows][ld], first V of each: with m = max x, Z =
+ * sum e^(x - m),
+ *   logprob[r]  = x_t - m - log Z for t = target[r]  (NaN outside [0, V))
+ *   entropy[r]  = log Z - sum e^(x - m) (x - m) / Z  (nats)
+ *   top_ids / top_lp [rows][top_k]: the top_k largest, descending, equal
+ *                 values by ascending id, and their log probabilities.
+ * target / logprob, entropy and the top lists may each be NULL (top_k = 0).
+ * Logits of -inf have probability 0; a NaN or +inf makes the row's results NaN
+ * (NaN values rank last).  ws: at least cmf_logprobs_workspace bytes (at most
+ * 64 MiB), as cmf_attention_dev's. */
+typedef struct {
+    const void* logits;
+    const int32_t* target;
+    float *logprob, *entropy;
+    int32_t* top_ids;
+    float* top_lp;
+    void* ws;
+    size_t ws_bytes;
+    long long ld;
+    int rows, V, dtype, top_k;
+    void* stream;
+} cmf_logprobs_args;
+size_t cmf_logprobs_workspace(const cmf_logprobs_args* a);
+int cmf_logprobs_dev(const cmf_logprobs_args* a);
+
 /* ---- .cmf v2 container (cortiq-core/src/format.rs) ------------------- */
 /* Error kinds of the container calls (CmfError, format.rs; the message of
  * cmf_last_error() carries the details). */
