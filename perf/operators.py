@@ -26,7 +26,7 @@ HD = 128
 EPS = 1e-6
 THETA = 1e6
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
-WS_BYTES = 64 << 20  # the scratch a program keeps for the attention
+WS_BYTES = 64 << 20  # the scratch a program keeps for the attention and the log probabilities
 
 
 def listed():
@@ -161,7 +161,8 @@ def prepare(case, seed):
     x.scatter_add_(1, tgt[:, None], r.normal(rows, 1, std=4.0).abs())
     s.update(x=x.to(DTYPES[c["dtype"]]), tgt=tgt.to(torch.int32), lp=torch.empty(rows, device="cuda"),
              ent=torch.empty(rows, device="cuda"), ids=torch.empty(rows, c["k"], dtype=torch.int32, device="cuda"),
-             top=torch.empty(rows, c["k"], device="cuda"))
+             top=torch.empty(rows, c["k"], device="cuda"),
+             ws=torch.empty(WS_BYTES, dtype=torch.uint8, device="cuda"))
     return s
 
 
