@@ -12,11 +12,13 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include <string>
 #include <vector>
 
 #include "../../include/cmf_hip.h"
+#include "cache_ops.h"
 #include "common.h"
 #include "gemv.h"
 #include "layers.h"
@@ -105,6 +107,24 @@ __global__ __launch_bounds__(1024) void k_router_f32(const float* __restrict__ W
 
 using namespace cmf;
 
+// cmf_verify_tree: the rows of a tree through every layer.
+struct TreeRes {  // what the acceptance leaves
+    int a, next, n;
+    int path[CMF_TREE_MAX];  // the accepted rows, path[0] = 0
+    int argmax[CMF_TREE_MAX];
+    float lp[CMF_TREE_MAX], ent[CMF_TREE_MAX];
+};
+struct TreeBufs {
+    float *h = nullptr, *qkv = nullptr, *q = nullptr, *ao = nullptr, *gu = nullptr, *logits = nullptr, *path_h = nullptr;
+    float *k = nullptr, *v = nullptr;  // the rows' keys and values [layer][kv head][64][128]
+    void **dst = nullptr, **src = nullptr;  // the caches and those rows, per layer K then V
+    int *toks = nullptr, *path_toks = nullptr, *parent = nullptr, *depth = nullptr;
+    uint64_t* mask = nullptr;
+    float *am_v = nullptr, *top_lp = nullptr;
+    int *am_i = nullptr, *top_ids = nullptr;
+    TreeRes* res = nullptr;
+};
+
 struct cmf_model_s {
     cmf_model_config c{};
     std::vector<LayerDev> L;
@@ -174,6 +194,15 @@ struct cmf_model_s {
     bool xl_on = false;
     int xl_fallbacks = 0;   // calls re-run on the six-launch blocks after a failed check
     float* h_save = nullptr;  // the tip hidden before such a call
+    // sliding window of every block's attention (0: the whole cache) and the
+    // first positions that stay visible (cmf_model_set_window)
+    int window = 0, sinks = 0;
+    void* op_ws = nullptr;  // scratch of the windowed and the tree attention
+    TreeBufs tree;  // cmf_verify_tree's buffers (from its first call on)
+    bool has_tree = false;
+    float* sc_logits = nullptr;  // cmf_score: a batch of logit rows and its results
+    int32_t *sc_tgt = nullptr, *sc_ids = nullptr;
+    float *sc_lp = nullptr, *sc_ent = nullptr, *sc_top = nullptr;
 };
 
 namespace {
@@ -360,6 +389,75 @@ int moe_block_ffn(cmf_model_s* m, LayerDev& l, float* h, int nb, hipStream_t s) 
     return moe_ffn_launch(l.moe, src_norm(h, H, l.post_norm, c.eps), m->rlog, nb, h, H, true, s);
 }
 
+// Whether rows that reach max_len positions do not all see the whole cache
+// (position p sees (p - window, p] and [0, sinks): all of it up to window +
+// sinks positions, where the attention of the whole cache runs).
+bool windowed(const cmf_model_s* m, int max_len) {
+    return m->window > 0 && max_len > (long long)m->window + m->sinks;
+}
+
+cmf_qk_rope_args rope_args(cmf_model_s* m, const LayerDev& l, const float* qkv, float* q, int nb) {
+    const auto& c = m->c;
+    cmf_qk_rope_args r{};
+    r.qkv = qkv;
+    r.q_out = q;
+    r.q_norm = l.q_norm;
+    r.k_norm = l.k_norm;
+    r.rope = (const float*)m->rope;
+    r.eps = c.eps;
+    r.b = nb;
+    r.nh = c.n_heads;
+    r.nkv = c.n_kv;
+    r.ldq = (c.n_heads + 2 * c.n_kv) * c.head_dim;
+    r.ldo = c.n_heads * c.head_dim;
+    r.max_pos = c.max_seq;
+    r.row_stride = c.head_dim;
+    return r;
+}
+
+cmf_attention_args attention_args(cmf_model_s* m, const LayerDev& l, const float* q, float* ao, int nb) {
+    const auto& c = m->c;
+    cmf_attention_args a{};
+    a.q = q;
+    a.out = ao;
+    a.k = l.kc;
+    a.v = l.vc;
+    a.ws = m->op_ws;
+    a.ws_bytes = OP_WS_MAX;
+    a.head_stride = (long long)c.max_seq * c.head_dim;
+    a.row_stride = c.head_dim;
+    a.b = nb;
+    a.nh = c.n_heads;
+    a.nkv = c.n_kv;
+    a.ldq = a.ldo = c.n_heads * c.head_dim;
+    a.slots = c.max_seq;
+    a.window = m->window;
+    a.sinks = m->sinks;
+    return a;
+}
+
+// Attention of nb projected rows at positions *pb + padd + i through the
+// window: norms, rotation and append, then what the rows see.  max_len bounds
+// the positions stored with the rows.
+int window_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* q, float* ao, int nb, const int* pb, int padd,
+                     int max_len, hipStream_t s) {
+    const auto& c = m->c;
+    cmf_qk_rope_args r = rope_args(m, l, qkv, q, nb);
+    r.k = l.kc;
+    r.v = l.vc;
+    r.d_pos0 = pb;
+    r.pos0 = padd;
+    r.head_stride = (long long)c.max_seq * c.head_dim;
+    r.slots = c.max_seq;
+    r.at_pos = 1;
+    launch_qk_rope(r, s);
+    cmf_attention_args a = attention_args(m, l, q, ao, nb);
+    a.d_pos0 = pb;
+    a.pos0 = padd;
+    a.len_bound = std::max(0, std::min(max_len, c.max_seq) - nb);
+    return launch_cache_attention(a, s);
+}
+
 // One decoder block over nb rows of the residual h at positions *pb + padd
 // + i (forward_layers_span, pipeline.rs:7981-8700):
 //   h += Wo attn(qk-norm/RoPE(Wqkv rms_norm(h)))
@@ -379,8 +477,10 @@ void run_block(cmf_model_s* m, LayerDev& l, float* h, int nb, const int* pb, int
     // every merge wave writes its head's two 64-column chunks as int8 planes
     // with their own chunk scales, so the wo GEMV neither stages the rows nor
     // waits for a producer launch
-    const bool wo_planes = l.wo.dtype == DT_Q8ROW && (nh * hd) % 64 == 0;
-    for (int b0 = 0; b0 < nb; b0 += rows_per) {
+    const bool win = windowed(m, max_len);
+    const bool wo_planes = !win && l.wo.dtype == DT_Q8ROW && (nh * hd) % 64 == 0;
+    if (win) (void)window_attention(m, l, m->qkv_out, m->qrot, m->ao, nb, pb, padd, max_len, s);
+    for (int b0 = 0; b0 < nb && !win; b0 += rows_per) {
         AttnArgs at{m->qkv_out + (size_t)b0 * QKV, QKV, l.q_norm, l.k_norm, m->rope, l.kc, l.vc, c.max_seq,
                     std::min(rows_per, nb - b0), nh, nkv, c.eps, pb, padd + b0, m->pm, m->pl, m->po, m->nch_cap,
                     m->ao + (size_t)b0 * nh * hd, 1};
@@ -434,7 +534,7 @@ constexpr float XL_QK_NORM_MAX = 2048.f;
 bool xl_layer_ok(cmf_model_s* m, const LayerDev& l, int nb, int max_len) {
     return m->xl_on && !l.moe && l.kc && l.qkv.dtype == DT_Q8ROW && l.wo.dtype == DT_Q8ROW &&
            l.gu.dtype == DT_Q4T && l.down.dtype == DT_Q4T && l.qk_norm_max <= XL_QK_NORM_MAX &&
-           xl_shape_ok(m->xls, nb, max_len);
+           !windowed(m, max_len) && xl_shape_ok(m->xls, nb, max_len);
 }
 XlAttnW xl_aw(const LayerDev& l) {
     return XlAttnW{l.qkv.w, l.qkv.scale, l.wo.w, l.wo.scale, l.qkv.kchunks, l.wo.kchunks,
@@ -659,6 +759,10 @@ void prefill_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* ao,
                        bool attend, hipStream_t s) {
     const auto& c = m->c;
     const int hd = c.head_dim, nh = c.n_heads, nkv = c.n_kv, QKV = (nh + 2 * nkv) * hd;
+    if (attend && windowed(m, p0 + cnt)) {
+        (void)window_attention(m, l, qkv, m->pf_q, ao, cnt, pb, 0, p0 + cnt, s);
+        return;
+    }
     static const bool tiled = !(getenv("CMF_PREFILL_ATTN") && getenv("CMF_PREFILL_ATTN")[0] == '0');
     if (tiled && prefill_attention_fits(nh, nkv, hd)) {
         // the whole chunk at once: the tiled prefill attention (one launch
@@ -1052,7 +1156,54 @@ static int ready(cmf_model m) {
     return CMF_OK;
 }
 
-int cmf_prefill(cmf_model m, const int32_t* ids, int n) {
+// What cmf_score asks for, host arrays by row.
+struct ScoreOut {
+    float *lp, *ent;
+    int top_k;
+    int32_t* ids;
+    float* top;
+};
+constexpr int SCORE_ROWS = 256;  // logit rows of a batch: the head's weights are read once for that many
+
+// The head over cnt final hidden rows h (positions p0 ..) and what is asked of
+// their logits, a batch of rows at a time.
+static int score_rows(cmf_model m, const float* h, const int32_t* ids, int p0, int cnt, int n, const ScoreOut& o,
+                      hipStream_t s) {
+    const int H = m->c.hidden, V = m->c.vocab, k = o.top_k;
+    for (int r0 = 0; r0 < cnt; r0 += SCORE_ROWS) {
+        const int nr = std::min(SCORE_ROWS, cnt - r0), p = p0 + r0;
+        int32_t tgt[SCORE_ROWS];
+        for (int i = 0; i < nr; i++) tgt[i] = p + i + 1 < n ? ids[p + i + 1] : -1;
+        CMF_HIP(hipMemcpyAsync(m->sc_tgt, tgt, nr * sizeof(int32_t), hipMemcpyHostToDevice, s));
+        if (gemm(m->lm, src_norm(h + (size_t)r0 * H, H, m->final_norm, m->c.eps), nr, m->sc_logits, V, false, s) != CMF_OK)
+            return CMF_ERR;
+        cmf_logprobs_args a{};
+        a.logits = m->sc_logits;
+        a.target = m->sc_tgt;
+        a.logprob = m->sc_lp;
+        a.entropy = m->sc_ent;
+        a.top_ids = k ? m->sc_ids : nullptr;
+        a.top_lp = k ? m->sc_top : nullptr;
+        a.ws = m->op_ws;
+        a.ws_bytes = OP_WS_MAX;
+        a.ld = V;
+        a.rows = nr;
+        a.V = V;
+        a.dtype = CMF_DT_F32;
+        a.top_k = k;
+        launch_logprobs(a, s);
+        if (o.lp) CMF_HIP(hipMemcpyAsync(o.lp + p, m->sc_lp, nr * sizeof(float), hipMemcpyDeviceToHost, s));
+        if (o.ent) CMF_HIP(hipMemcpyAsync(o.ent + p, m->sc_ent, nr * sizeof(float), hipMemcpyDeviceToHost, s));
+        if (k && o.ids)
+            CMF_HIP(hipMemcpyAsync(o.ids + (size_t)p * k, m->sc_ids, (size_t)nr * k * 4, hipMemcpyDeviceToHost, s));
+        if (k && o.top)
+            CMF_HIP(hipMemcpyAsync(o.top + (size_t)p * k, m->sc_top, (size_t)nr * k * 4, hipMemcpyDeviceToHost, s));
+        CMF_HIP(hipStreamSynchronize(s));  // tgt and the results' buffers are used again
+    }
+    return CMF_OK;
+}
+
+static int prefill_impl(cmf_model m, const int32_t* ids, int n, const ScoreOut* score) {
     if (ready(m)) return CMF_ERR;
     if (!ids || n < 1 || n + 1 > m->c.max_seq) return fail("prefill: 1 <= n < max_seq");
     if (ensure_prefill_bufs(m)) return CMF_ERR;
@@ -1071,6 +1222,7 @@ int cmf_prefill(cmf_model m, const int32_t* ids, int n) {
         launch_embed(m->pf_toks, embed_src(m), H, m->pf_h, H, cnt, s);
         for (int li = 0; li < c.n_layers; li++)
             if (prefill_block(m, m->L[li], m->pf_h, cnt, pb, p0, s) != CMF_OK) return CMF_ERR;
+        if (score && score_rows(m, m->pf_h, ids, p0, cnt, n, *score, s) != CMF_OK) return CMF_ERR;
         if (m->has_mtp) {
             // MTP warm on the (h_p, id_{p+1}) pairs of the chunk (pipeline.rs:2275-2318)
             const int pairs = (p0 + cnt < n) ? cnt : cnt - 1;
@@ -1103,10 +1255,48 @@ int cmf_prefill(cmf_model m, const int32_t* ids, int n) {
     if (perr && !m->pf_xcd_off) {
         m->pf_xcd_off = true;
         if (clear_dev(m->pf_err, sizeof(int)) != CMF_OK) return CMF_ERR;
-        return cmf_prefill(m, ids, n);
+        return prefill_impl(m, ids, n, score);
     }
     m->next_pos_host = n;
     m->prefilled = true;
+    return CMF_OK;
+}
+
+int cmf_prefill(cmf_model m, const int32_t* ids, int n) { return prefill_impl(m, ids, n, nullptr); }
+
+static int ensure_op_ws(cmf_model m) {
+    if (m->op_ws) return CMF_OK;
+    return dalloc(m, &m->op_ws, OP_WS_MAX);
+}
+
+int cmf_score(cmf_model m, const int32_t* ids, int n, float* logprobs, float* entropy, int top_k, int32_t* top_ids,
+              float* top_lp) {
+    if (!m) return fail("null model");
+    if (top_k < 0 || top_k > CMF_TOP_MAX || top_k > m->c.vocab) return fail("score: top_k of 0 to 64, at most the vocabulary");
+    if (!top_k != (!top_ids && !top_lp)) return fail("score: top_k and a top list go together");
+    if (ready(m) || ensure_op_ws(m)) return CMF_ERR;
+    const size_t V = m->c.vocab;
+    if (!m->sc_logits) {  // one block: the logits, then what comes of them
+        const size_t R = SCORE_ROWS;
+        float* p = nullptr;
+        if (dalloc_t(m, &p, R * V + R * (3 + 2 * CMF_TOP_MAX)) != CMF_OK) return CMF_ERR;
+        m->sc_logits = p;
+        m->sc_lp = p + R * V;
+        m->sc_ent = m->sc_lp + R;
+        m->sc_tgt = (int32_t*)(m->sc_ent + R);
+        m->sc_ids = m->sc_tgt + R;
+        m->sc_top = (float*)(m->sc_ids + R * CMF_TOP_MAX);
+    }
+    const ScoreOut o{logprobs, entropy, top_k, top_ids, top_lp};
+    return prefill_impl(m, ids, n, &o);
+}
+
+int cmf_model_set_window(cmf_model m, int window, int sinks) {
+    if (!m || window < 0 || sinks < 0) return fail("set_window: window and sinks of at least 0");
+    if (window && ensure_op_ws(m)) return CMF_ERR;
+    drop_graph(m);
+    m->window = window;
+    m->sinks = window ? sinks : 0;
     return CMF_OK;
 }
 
@@ -1638,6 +1828,256 @@ int cmf_verify_step(cmf_model m, const int32_t* tokens, int b, int pos0, const c
                               next_token);
     }
     return rc == XL_RETRY ? fail("verify_step: XCD-partitioned blocks failed twice") : rc;
+}
+
+namespace {
+// The acceptance of a tree by one wave, lane i = row i.  A row's token has the
+// log probability lp under its parent's logits (the parent's largest logit
+// and the log probability of that: top_ids, top_lp).  Greedy (eps = 0): it is
+// accepted when it is the parent's argmax (ties to the highest id, as
+// everywhere in the decode); else when e^lp >= min(eps, delta e^-entropy).
+// From the root, the accepted child with the largest lp (then the lowest row)
+// is taken until a row has none.
+__global__ __launch_bounds__(64) void k_tree_accept(const float* __restrict__ logits, int V, const int* __restrict__ toks,
+                                                    const int* __restrict__ parent, const int* __restrict__ top_ids,
+                                                    const float* __restrict__ top_lp, int b, int pos0, float eps, float delta,
+                                                    TreeRes* r, DState* st, int* path_toks) {
+    const int i = threadIdx.x;
+    const bool in = i < b;
+    const int p = in ? parent[i] : -1, tok = in ? toks[i] : 0;
+    float lp = NAN;
+    bool ok = false;
+    if (p >= 0) {
+        const float* x = logits + (size_t)p * V;
+        lp = (x[tok] - x[top_ids[p]]) + top_lp[p];
+        ok = eps > 0.f ? expf(lp) >= fminf(eps, delta * expf(-r->ent[p])) : tok == r->argmax[p];
+    }
+    if (in) r->lp[i] = lp;
+    int cur = 0, n = 1;
+    if (i == 0) r->path[0] = 0;
+    while (true) {
+        uint64_t cand = __builtin_amdgcn_ballot_w64(ok && p == cur);
+        if (!cand) break;
+        const bool mine = cand >> i & 1;
+        const float best = wave_max(mine ? lp : -INFINITY);
+        const uint64_t top = __builtin_amdgcn_ballot_w64(mine && lp == best);
+        cur = __builtin_ctzll(top ? top : cand);
+        if (i == 0) {
+            r->path[n] = cur;
+            path_toks[n - 1] = toks[cur];
+        }
+        n++;
+    }
+    if (i == 0) {
+        r->a = n - 1;
+        r->n = n;
+        r->next = r->argmax[cur];
+        st->a = n - 1;
+        st->next_pos = pos0;  // (moved past the path at the end: the commit and the MTP rows are counted from here)
+        st->t_next = r->argmax[cur];
+    }
+}
+
+// The path's hidden rows in order, row j = path[min(j, a)], and the tokens
+// after them (0 past the path): the (hidden, next token) pairs of the MTP
+// cache; the last one is the tip.  grid (rows), block 256.
+__global__ __launch_bounds__(256) void k_tree_path(const float* __restrict__ h, int H, const TreeRes* __restrict__ r,
+                                                   float* __restrict__ out, float* __restrict__ tip) {
+    const int j = blockIdx.x, a = r->a;
+    const float* x = h + (size_t)r->path[min(j, a)] * H;
+    for (int i = threadIdx.x; i < H; i += 256) {
+        out[(size_t)j * H + i] = x[i];
+        if (j == a) tip[i] = x[i];
+    }
+}
+__global__ void k_tree_commit(DState* st) { st->next_pos += st->a + 1; }
+
+int ensure_tree(cmf_model_s* m) {
+    if (m->has_tree) return CMF_OK;
+    const auto& c = m->c;
+    const size_t R = CMF_TREE_MAX, H = c.hidden, Q = (size_t)c.n_heads * c.head_dim, KV = (size_t)c.n_kv * c.head_dim;
+    const size_t V = c.vocab, L = c.n_layers, ns = (V + 4095) / 4096;
+    TreeBufs t;
+    // one block of memory, carved up in 256-byte steps: a refused allocation
+    // leaves nothing behind
+    for (char* base = nullptr;;) {
+        size_t at = 0;
+        auto take = [&](auto*& p, size_t n) {
+            p = (std::remove_reference_t<decltype(p)>)(base ? base + at : nullptr);
+            at += (n * sizeof(*p) + 255) / 256 * 256;
+        };
+        take(t.h, R * H), take(t.qkv, R * (Q + 2 * KV)), take(t.q, R * Q), take(t.ao, R * Q), take(t.gu, R * 2 * c.inter);
+        take(t.logits, R * V), take(t.path_h, R * H), take(t.k, L * KV * R), take(t.v, L * KV * R);
+        take(t.dst, 2 * L), take(t.src, 2 * L), take(t.toks, R), take(t.path_toks, R), take(t.parent, R);
+        take(t.depth, R), take(t.mask, R), take(t.am_v, R * ns), take(t.am_i, R * ns), take(t.top_lp, R);
+        take(t.top_ids, R), take(t.res, 1);
+        if (base) break;
+        if (dalloc(m, (void**)&base, at) != CMF_OK) return CMF_ERR;
+    }
+    for (size_t li = 0; li < L; li++) {  // (a layer keeps its cache when it is set again)
+        void* dst[2] = {m->L[li].kc, m->L[li].vc};
+        void* src[2] = {t.k + li * KV * R, t.v + li * KV * R};
+        CMF_HIP(hipMemcpy(t.dst + 2 * li, dst, sizeof(dst), hipMemcpyHostToDevice));
+        CMF_HIP(hipMemcpy(t.src + 2 * li, src, sizeof(src), hipMemcpyHostToDevice));
+    }
+    m->tree = t;
+    m->has_tree = true;
+    return CMF_OK;
+}
+
+// One decoder block over the b rows of a tree behind pos0 cached positions;
+// their keys and values stay beside the cache until the acceptance.  Up to 16
+// rows take the decode GEMVs, more the large-batch GEMMs (every weight read
+// once).
+int tree_block(cmf_model_s* m, int li, int b, int pos0, hipStream_t s) {
+    const auto& c = m->c;
+    LayerDev& l = m->L[li];
+    TreeBufs& t = m->tree;
+    const int H = c.hidden, hd = c.head_dim, Q = c.n_heads * hd, QKV = Q + 2 * c.n_kv * hd, I = c.inter;
+    const bool few = b <= MAXB;
+    auto mul = [&](const DevWeight& w, const XSrc& x, float* y, int ldy, bool resid) {
+        return few ? gemv_f(m, w, x, y, ldy, b, resid, s) : gemm(w, x, b, y, ldy, resid, s);
+    };
+    int rc = mul(l.qkv, src_norm(t.h, H, l.in_norm, c.eps), t.qkv, QKV, false);
+    if (rc != CMF_OK) return rc;
+    const size_t at = (size_t)li * c.n_kv * CMF_TREE_MAX * hd;
+    cmf_qk_rope_args r = rope_args(m, l, t.qkv, t.q, b);
+    r.k = t.k + at;
+    r.v = t.v + at;
+    r.head_stride = (long long)CMF_TREE_MAX * hd;
+    r.slots = CMF_TREE_MAX;
+    r.pos0 = pos0;
+    r.d_depth = t.depth;
+    launch_qk_rope(r, s);
+    cmf_attention_args a = attention_args(m, l, t.q, t.ao, b);
+    a.k_new = t.k + at;
+    a.v_new = t.v + at;
+    a.new_head_stride = r.head_stride;
+    a.new_row_stride = hd;
+    a.d_mask = t.mask;
+    a.d_depth = t.depth;
+    a.pos0 = pos0;
+    if ((rc = launch_cache_attention(a, s)) != CMF_OK) return rc;
+    XSrc ra{};
+    ra.mode = XS_ROWS;
+    ra.x = t.ao;
+    ra.ldx = Q;
+    if ((rc = mul(l.wo, ra, t.h, H, true)) != CMF_OK) return rc;
+    if (l.moe) {
+        for (int b0 = 0; b0 < b; b0 += MAXB)
+            if ((rc = moe_block_ffn(m, l, t.h + (size_t)b0 * H, std::min(MAXB, b - b0), s)) != CMF_OK) return rc;
+        return CMF_OK;
+    }
+    XSrc sd{};
+    sd.x = t.gu;
+    if (few) {
+        if ((rc = gemv_f(m, l.gu, src_norm(t.h, H, l.post_norm, c.eps), t.gu, I, b, false, s, EPI_SWIGLU)) != CMF_OK) return rc;
+        sd.mode = XS_ROWS;
+        sd.ldx = I;
+    } else {
+        if ((rc = gemm(l.gu, src_norm(t.h, H, l.post_norm, c.eps), b, t.gu, 2 * I, false, s)) != CMF_OK) return rc;
+        sd.mode = XS_SILU8;
+        sd.ldx = 2 * I;
+        sd.K = I;
+    }
+    return mul(l.down, sd, t.h, H, true);
+}
+}  // namespace
+
+int cmf_verify_tree(cmf_model m, const int32_t* tokens, const int32_t* parent, int b, int pos0, float eps, float delta,
+                    int32_t* path, int32_t* accepted, int32_t* next_token, float* logprobs, float* entropy,
+                    int32_t* argmax_out, float* logits_out) {
+    if (!m) return fail("null model");
+    if (!tokens || !parent || b < 1 || b > CMF_TREE_MAX) return fail("verify_tree: 1 to 64 rows of tokens and parents");
+    if (!(eps >= 0.f) || !(delta >= 0.f) || eps - eps != 0.f || delta - delta != 0.f)
+        return fail("verify_tree: eps and delta must be finite and at least 0");
+    if (ready(m)) return CMF_ERR;
+    const auto& c = m->c;
+    const int H = c.hidden, V = c.vocab;
+    if (!m->prefilled || pos0 != m->next_pos_host)
+        return fail("verify_tree: pos0 must be the committed position (" + std::to_string(m->next_pos_host) +
+                    ", after cmf_prefill / cmf_forward_batch / a decode or verify step)");
+    if (pos0 < 1) return fail("verify_tree: pos0 of at least 1");
+    uint64_t mask[CMF_TREE_MAX];
+    int32_t depth[CMF_TREE_MAX];
+    if (cmf_tree_masks(parent, b, pos0, m->window, m->sinks, mask, depth) != CMF_OK) return CMF_ERR;
+    int deepest = 0;
+    for (int i = 0; i < b; i++) {
+        if ((parent[i] < 0) != (i == 0)) return fail("verify_tree: row 0 is the only root");
+        if (tokens[i] < 0 || tokens[i] >= V) return fail("verify_tree: token id out of range");
+        deepest = std::max(deepest, (int)depth[i]);
+    }
+    if (pos0 + deepest + 2 > c.max_seq) return fail("verify_tree: the tree's depth passes max_seq");
+    if (ensure_op_ws(m) || ensure_tree(m)) return CMF_ERR;
+    TreeBufs& t = m->tree;
+    hipStream_t s = stream();
+    CMF_HIP(hipMemcpyAsync(t.toks, tokens, b * sizeof(int), hipMemcpyHostToDevice, s));
+    CMF_HIP(hipMemcpyAsync(t.parent, parent, b * sizeof(int), hipMemcpyHostToDevice, s));
+    CMF_HIP(hipMemcpyAsync(t.depth, depth, b * sizeof(int), hipMemcpyHostToDevice, s));
+    CMF_HIP(hipMemcpyAsync(t.mask, mask, b * sizeof(uint64_t), hipMemcpyHostToDevice, s));
+    int* pb = &m->st->next_pos;
+    hipLaunchKernelGGL(k_set_int, dim3(1), dim3(1), 0, s, pb, pos0);
+    // the MTP row of the root, as cmf_verify_step writes it
+    if (m->has_mtp) mtp_warm(m, t.toks, m->h_tip, 1, pb, -1, pos0, s);
+    launch_embed(t.toks, embed_src(m), H, t.h, H, b, s);
+    for (int li = 0; li < c.n_layers; li++)
+        if (tree_block(m, li, b, pos0, s) != CMF_OK) return CMF_ERR;
+    const XSrc fin = src_norm(t.h, H, m->final_norm, c.eps);
+    if ((b <= MAXB ? gemv_f(m, m->lm, fin, t.logits, V, b, false, s) : gemm(m->lm, fin, b, t.logits, V, false, s)) != CMF_OK)
+        return CMF_ERR;
+    launch_argmax(t.logits, V, V, b, t.am_v, t.am_i, t.res->argmax, s);
+    cmf_logprobs_args a{};
+    a.logits = t.logits;
+    a.entropy = t.res->ent;
+    a.top_ids = t.top_ids;
+    a.top_lp = t.top_lp;
+    a.ws = m->op_ws;
+    a.ws_bytes = OP_WS_MAX;
+    a.ld = V;
+    a.rows = b;
+    a.V = V;
+    a.dtype = CMF_DT_F32;
+    a.top_k = 1;
+    launch_logprobs(a, s);
+    hipLaunchKernelGGL(k_tree_accept, dim3(1), dim3(64), 0, s, t.logits, V, t.toks, t.parent, t.top_ids, t.top_lp, b, pos0,
+                       eps, delta, t.res, m->st, t.path_toks);
+    // the accepted path into every layer's cache
+    cmf_kv_copy_args k{};
+    k.d_dst = t.dst;
+    k.d_src = (const void* const*)t.src;
+    k.d_idx = t.res->path;
+    k.d_n = &t.res->n;
+    k.dst_head_stride = (long long)c.max_seq * c.head_dim;
+    k.src_head_stride = (long long)CMF_TREE_MAX * c.head_dim;
+    k.dst_row_stride = k.src_row_stride = c.head_dim;
+    k.nbuf = 2 * c.n_layers;
+    k.nkv = c.n_kv;
+    k.kv_dtype = CMF_DT_F32;
+    k.n = deepest + 1;
+    k.pos0 = pos0;
+    k.dst_slots = c.max_seq;
+    k.src_slots = CMF_TREE_MAX;
+    launch_kv_copy(k, s);
+    hipLaunchKernelGGL(k_tree_path, dim3(deepest + 1), dim3(256), 0, s, t.h, H, t.res, t.path_h, m->h_tip);
+    if (m->has_mtp)
+        for (int j = 0; j < deepest; j += MAXB)
+            mtp_warm(m, t.path_toks + j, t.path_h + (size_t)j * H, std::min(MAXB, deepest - j), pb, j, pos0 + deepest + 1, s);
+    hipLaunchKernelGGL(k_tree_commit, dim3(1), dim3(1), 0, s, m->st);
+    if (logits_out)
+        CMF_HIP(hipMemcpyAsync(logits_out, t.logits, (size_t)b * V * sizeof(float), hipMemcpyDeviceToHost, s));
+    TreeRes r;
+    CMF_HIP(hipMemcpyAsync(&r, t.res, sizeof(r), hipMemcpyDeviceToHost, s));
+    CMF_HIP(hipStreamSynchronize(s));
+    CMF_HIP(hipGetLastError());
+    m->next_pos_host = pos0 + r.n;
+    m->decoding = false;
+    if (accepted) *accepted = r.a;
+    if (next_token) *next_token = r.next;
+    if (path) std::copy(r.path, r.path + r.n, path);
+    if (logprobs) std::copy(r.lp, r.lp + b, logprobs);
+    if (entropy) std::copy(r.ent, r.ent + b, entropy);
+    if (argmax_out) std::copy(r.argmax, r.argmax + b, argmax_out);
+    return CMF_OK;
 }
 
 int cmf_sparse_distribution(cmf_model m, const float* logits, const cmf_sampler_config* sc, int32_t* ids,

@@ -161,6 +161,42 @@ class Model:
             raise CmfError("verify declined (sampler config beyond the device sampler)")
         return a.value, nxt.value, am, lg
 
+    def verify_tree(self, tokens, parents, pos0, eps=0.0, delta=0.0, want_logits=False):
+        """cmf_verify_tree: a tree of drafts (row 0 the token to emit, row i a
+        draft after row parents[i]).  Returns a dict: path (the accepted rows,
+        row 0 first), next_token, logprobs (row i's token after its parent),
+        entropy and argmax of every row, logits [b][vocab] or None."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        parents = np.ascontiguousarray(parents, dtype=np.int32)
+        b = len(tokens)
+        if len(parents) != b:
+            raise CmfError("verify_tree: one parent per token")
+        path, am = np.empty(b, np.int32), np.empty(b, np.int32)
+        lp, ent = np.empty(b, np.float32), np.empty(b, np.float32)
+        lg = np.empty((b, self.cfg["vocab"]), np.float32) if want_logits else None
+        a, nxt = C.c_int(), C.c_int()
+        check(lib().cmf_verify_tree(self.h, _ptr(tokens), _ptr(parents), b, pos0, eps, delta, _ptr(path), C.byref(a),
+                                    C.byref(nxt), _ptr(lp), _ptr(ent), _ptr(am), _ptr(lg)))
+        return dict(path=path[:a.value + 1].copy(), next_token=nxt.value, logprobs=lp, entropy=ent, argmax=am, logits=lg)
+
+    def score(self, ids, top_k=0):
+        """cmf_score: prefill(ids), and for every row p the log probability of
+        ids[p + 1] (the last: NaN), the entropy, and with top_k the most likely
+        tokens.  Returns (logprobs [n], entropy [n], top_ids [n][top_k], top_lp
+        [n][top_k])."""
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        n = len(ids)
+        lp, ent = np.empty(n, np.float32), np.empty(n, np.float32)
+        ti, tl = np.empty((n, top_k), np.int32), np.empty((n, top_k), np.float32)
+        check(lib().cmf_score(self.h, _ptr(ids), n, _ptr(lp), _ptr(ent), top_k, _ptr(ti) if top_k else None,
+                              _ptr(tl) if top_k else None))
+        return lp, ent, ti, tl
+
+    def set_window(self, window, sinks=0):
+        """cmf_model_set_window: from the next call on every position sees the
+        last `window` positions and the first `sinks` (window 0: all)."""
+        check(lib().cmf_model_set_window(self.h, window, sinks))
+
     def sparse_distribution(self, logits, sampler):
         logits = np.ascontiguousarray(logits, dtype=np.float32)
         ids = np.empty(SPARSE_CAP, np.int32)

@@ -352,6 +352,40 @@ int cmf_forward_batch(cmf_model m, const int32_t* tokens, int b, int pos0, float
 int cmf_verify_step(cmf_model m, const int32_t* tokens, int b, int pos0, const cmf_sampler_config* sc,
                     const int32_t* q_ids, const float* q_probs, const int32_t* q_n, const float* uniforms,
                     int32_t* argmax_out, float* logits_out, int32_t* accepted, int32_t* next_token);
+/* cmf_verify_step for a tree of drafts (no counterpart in the reference, whose
+ * drafts are a chain): b <= 64 rows, row 0 = [t_next] at pos0 (the committed
+ * position), row i a draft that follows row parent[i] < i (parent[0] = -1).
+ * Every row is a token after its ancestors: it sits at position pos0 + depth
+ * and sees the cache and them (through the model's window, if it has one).
+ * Row i's token is accepted after its parent when
+ *   eps == 0: it is the argmax of the parent's logits (ties to the highest id);
+ *   eps > 0 : its probability p >= min(eps, delta e^-H), H the entropy of the
+ *             parent's distribution (nats): likely enough, the less the surer
+ *             the model is.
+ * From row 0 on, the accepted child with the largest probability (then the
+ * lowest row) is taken until there is none: path [b] gets the taken rows
+ * (path[0] = 0, *accepted + 1 of them), *next_token the argmax after the last.
+ * Commit as cmf_verify_step: trunk KV [0, pos0 + accepted + 1), the tip hidden
+ * of the last row, the MTP cache's pairs along the path.  logprobs [b]: of row
+ * i's token under its parent (row 0: NaN), entropy [b] of row i's own next
+ * token, argmax_out [b], logits_out [b][vocab]; all outputs may be NULL. */
+int cmf_verify_tree(cmf_model m, const int32_t* tokens, const int32_t* parent, int b, int pos0, float eps, float delta,
+                    int32_t* path, int32_t* accepted, int32_t* next_token, float* logprobs, float* entropy,
+                    int32_t* argmax_out, float* logits_out);
+/* cmf_prefill of ids, and of every row p < n (the distribution after ids[0..p]):
+ * logprobs[p] = log probability of ids[p + 1] (the last row: NaN), entropy[p]
+ * in nats, top_ids / top_lp [n][top_k] the top_k <= 64 most likely tokens,
+ * descending, equal logits by ascending id.  Any output may be NULL (top_k =
+ * 0 without the lists).  The reference scores nothing: perplexity, re-ranking
+ * and checks of a quantization need it. */
+int cmf_score(cmf_model m, const int32_t* ids, int n, float* logprobs, float* entropy, int top_k, int32_t* top_ids,
+              float* top_lp);
+/* A sliding window for the attention of every block (the MTP block's too):
+ * position p sees (p - window, p] and the first sinks positions; window 0: the
+ * whole cache.  For the calls after it, whatever the cache holds; keys keep
+ * their positions' rotation.  Up to window + sinks positions nothing changes;
+ * past them a token costs the window's bytes, not the context's. */
+int cmf_model_set_window(cmf_model m, int window, int sinks);
 /* sparse_distribution_into (sampler.rs:440-514) of one logits row [vocab]
  * (host) on the device sampler: ids ascending and their probabilities
  * (capacity CMF_SPARSE_CAP); returns the count (>= 1: a fully filtered
