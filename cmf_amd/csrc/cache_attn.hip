@@ -9,6 +9,8 @@
 #include <math.h>
 
 #include <algorithm>
+#include <mutex>
+#include <set>
 #include <string>
 
 #include "cache_ops.h"
@@ -23,6 +25,13 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int HD = CACHE_HD;
 constexpr float LOG2E = 1.4426950408889634f;
+
+// the largest of the wave (the same in every lane)
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
 
 // max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float lanes4_max(float v) {
@@ -291,6 +300,443 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many queries per kv head (prompt chunks, larger trees): tiles of 64 keys in
+// LDS as f16 halves, scores and values on the 32x32x16 f16 MFMA: q.k = qh.kh +
+// qh.kl + ql.kh and p.v likewise (22-bit operands, f32 sums; a 16-bit cache has
+// no kl and vl), three products at 16 times the f32 MFMA's rate.
+//
+// f16 has 5 exponent bits, so every operand is scaled by a power of two first
+// (exact): a query row and a tile of keys to a largest magnitude in [2^14,
+// 2^15), undone in the scores; values by the largest of all tiles so far (the
+// accumulated output follows when that grows); weights are 2^(s - m + 14).
+// What the halves drop is then 2^-22 of an element, and elements down to
+// 2^-29 of the largest keep 11 bits.  A tile that holds infinities or NaN
+// (anything in a row that some query does not see) is left for a second walk
+// without MFMAs, so that it reaches only the queries that see it.
+//
+// S^T = K Q^T: a lane (query n = lane % 32, h = lane / 32) ends up with the
+// keys 8 a + 4 h + b of a 32-key block in register 4 a + b, which is the B
+// operand of O^T = V^T P^T when V's slots hold the same keys: the weights stay
+// in registers.  Eight waves: four groups of 32 queries, the two 32-key blocks
+// of a tile on different waves, joined at the end.  Two tile buffers: while one
+// is multiplied, the next tile, in registers since the tile before, is split
+// into the other, and the one after is loaded; one barrier a tile.
+//
+// Bound by the MFMAs: 1536 cycles per tile and wave at f32.
+// grid (nsplit ceil(b hpk / 128), nkv), block 512, LDS Tile<T>::LDS.
+// ---------------------------------------------------------------------------
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+constexpr int KT = 64, TQ = 128;     // keys of a tile, queries of a workgroup
+constexpr int KFRAG = 528;           // 32 keys x 8 dims (512 B), padded against bank conflicts
+constexpr int K_BYTES = 32 * KFRAG;  // one half (hi or lo) of the keys
+constexpr int VGROUP = 2048;         // 8 keys x 128 dims: [dim % 2][dim / 2][8 keys]
+constexpr int V_BYTES = 8 * VGROUP;
+constexpr int JOIN_ROW = 67, JOIN_BYTES = 4 * 64 * JOIN_ROW * 4;  // the second block's states at the end
+template <class T>
+struct Tile {
+    static constexpr bool LO = sizeof(T) == 4;
+    static constexpr int HALVES = LO ? 2 : 1, BUF = HALVES * (K_BYTES + V_BYTES);
+    static constexpr int USE = 2 * BUF + 2 * 64;  // and the waves' maxima, 8 of K and 8 of V, twice
+    static constexpr int LDS = USE > JOIN_BYTES ? USE : JOIN_BYTES;
+};
+static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
+
+// the larger magnitude; NaN stays
+__device__ __forceinline__ float mag(float m, float x) { return __builtin_elementwise_maximum(m, fabsf(x)); }
+// the exponent e of a positive finite x in [2^e, 2^(e+1)), 0 for 0
+__device__ __forceinline__ int exponent_of(float x) {
+    return x == 0.f ? 0 : (int)(__float_as_uint(x) >> 23 & 255) - 127;
+}
+// 2^n for any n (what f32 cannot hold ends at its largest power)
+__device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, min(n, 127)); }
+
+struct Split8 {
+    half8 hi, lo;
+};
+template <bool LO>
+__device__ __forceinline__ Split8 split8(const float (&x)[8], float scale) {
+    Split8 r;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2v y = {x[i] * scale, x[i + 1] * scale};
+        const half2v h = __builtin_convertvector(y, half2v);
+        r.hi[i] = h[0], r.hi[i + 1] = h[1];
+        if constexpr (LO) {
+            const float2v d = {y[0] - (float)h[0], y[1] - (float)h[1]};
+            const half2v l = __builtin_convertvector(d, half2v);
+            r.lo[i] = l[0], r.lo[i + 1] = l[1];
+        }
+    }
+    return r;
+}
+__device__ __forceinline__ float lanes2_max(float v) {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lanes2_sum(float v) {
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// N elements as they lie in memory, and as f32
+template <class T, int N>
+struct Raw {
+    typedef uint32_t vec __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+    vec v;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (N * sizeof(T) == 32) {  // two loads of 16 bytes
+            typedef uint32_t q4 __attribute__((ext_vector_type(4)));
+            const q4 a = ((const q4*)p)[0], b = ((const q4*)p)[1];
+            v = vec{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        } else {
+            v = *(const vec*)p;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(v[i]);
+        } else {
+            const uint16_t u = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+            return to_f32(__builtin_bit_cast(T, u));
+        }
+    }
+};
+template <class T>
+__global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
+    const cmf_attention_args& a = c.a;
+    constexpr bool LO = Tile<T>::LO;
+    constexpr int BUF = Tile<T>::BUF, KL = K_BYTES, VH = Tile<T>::HALVES * K_BYTES, VL = VH + V_BYTES;
+    extern __shared__ __align__(16) uint8_t sm[];
+    uint32_t* tmax = (uint32_t*)(sm + 2 * BUF);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 31, h = lane >> 5, g = blockIdx.y, split = blockIdx.x % c.nsplit;
+    const int q0 = blockIdx.x / c.nsplit * TQ, nq = a.b * c.hpk;
+    const int r0 = q0 / c.hpk, r1 = (min(q0 + TQ, nq) - 1) / c.hpk;
+    const Keys ks = keys_of(a, r0, r1);
+    const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + KT - 1) / KT * KT;
+    const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
+    const int qg = wave & 3, kb = wave >> 2;  // the wave's queries and 32-key block
+
+    // the wave's queries: lane (n, h) holds dims 16 j + 8 h + i
+    const int qi = min(q0 + 32 * qg + n, nq - 1), row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
+    const int P = ks.npos0 + (a.d_depth ? a.d_depth[row] : row);
+    const uint64_t mask = ks.tree ? a.d_mask[row] : 0;
+    half8 qh[8], ql[8];
+    float cq;  // the scores' factor: scale * log2(e) * 2^(eq - 14)
+    {
+        const float* q = a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * h;
+        float x[8][8], mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            load8(q + 16 * j, x[j]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[j][i]));
+        }
+        const int eq = exponent_of(lanes2_max(mx));  // (an infinite or NaN query ends as NaN by itself)
+        const float sc = pow2(14 - eq);
+        cq = ldexpf(c.qscale, eq - 14);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const Split8 s = split8<true>(x[j], sc);
+            qh[j] = s.hi;
+            ql[j] = s.lo;
+        }
+    }
+
+    // what thread t stages of a tile: dims 8 kd .. of keys kk and kk + 32, and
+    // dims 2 lane, 2 lane + 1 of the keys vk + {0 .. 3, 8 .. 11} (the slots of
+    // group (block, 16-key half, h) = wave)
+    const int kd = t & 15, kk = t >> 4, vk = 32 * (wave >> 2) + 16 * (wave >> 1 & 1) + 4 * (wave & 1);
+    Raw<T, 8> kx[2];
+    Raw<T, 2> vx[8];
+    auto load = [&](int v0) {
+        const int p0 = ks.pos(v0);
+        if (v0 >= ks.s && v0 + KT <= ks.nv && (p0 + KT <= ks.npos0 || !a.k_new)) {  // one run of the cache
+            const size_t o = (size_t)g * a.head_stride + (size_t)p0 * a.row_stride;
+            const T *kp = (const T*)a.k + o + (size_t)kk * a.row_stride + 8 * kd;
+            const T *vp = (const T*)a.v + o + (size_t)vk * a.row_stride + 2 * lane;
+#pragma unroll
+            for (int r = 0; r < 2; r++) kx[r].load(kp + (size_t)(32 * r) * a.row_stride);
+#pragma unroll
+            for (int i = 0; i < 8; i++) vx[i].load(vp + (size_t)(8 * (i >> 2) + (i & 3)) * a.row_stride);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + kk + 32 * r, ks.nv - 1)), g, kp, vp);
+                kx[r].load(kp + 8 * kd);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1)), g, kp, vp);
+                vx[i].load(vp + 2 * lane);
+            }
+        }
+    };
+    // the largest magnitudes of the tile in registers, into slot `at` (as bits:
+    // NaN is above infinity)
+    auto publish = [&](int at) {
+        float mk = 0.f, mv = 0.f;
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) mk = mag(mk, kx[r].get(i));
+#pragma unroll
+        for (int i = 0; i < 8; i++) mv = mag(mag(mv, vx[i].get(0)), vx[i].get(1));
+        const uint32_t uk = wave_max_u32(__float_as_uint(mk)), uv = wave_max_u32(__float_as_uint(mv));
+        if (lane == 0) {
+            tmax[16 * at + wave] = uk;
+            tmax[16 * at + 8 + wave] = uv;
+        }
+    };
+    auto stage = [&](uint8_t* buf, float sk, float sv) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = kx[r].get(i);
+            const Split8 s = split8<LO>(x, sk);
+            const int o = (r * 16 + kd) * KFRAG + kk * 16;
+            *(half8*)(buf + o) = s.hi;
+            if (LO) *(half8*)(buf + KL + o) = s.lo;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = vx[i].get(j);
+            const Split8 s = split8<LO>(x, sv);
+            const int o = wave * VGROUP + j * 1024 + lane * 16;
+            *(half8*)(buf + VH + o) = s.hi;
+            if (LO) *(half8*)(buf + VL + o) = s.lo;
+        }
+    };
+
+    float16v acc[4];
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    int ev = -1000;  // the values' exponent so far
+    bool odd = false;
+    struct {         // a tile in LDS: what its keys and values were scaled by, whether it is finite
+        int ek, ev;
+        bool fin;
+    } cur{0, -1000, true}, nxt{0, -1000, true};
+
+    // the tile in registers goes to buffer `at` (as nxt, behind cur): scales
+    // from all waves' maxima
+    auto take = [&](int at) {
+        uint32_t uk = 0, uv = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            uk = max(uk, tmax[16 * at + w]);
+            uv = max(uv, tmax[16 * at + 8 + w]);
+        }
+        uk = __builtin_amdgcn_readfirstlane(uk);
+        uv = __builtin_amdgcn_readfirstlane(uv);
+        nxt.fin = max(uk, uv) < 0x7f800000u;
+        odd |= !nxt.fin;
+        nxt.ek = exponent_of(__uint_as_float(uk));
+        nxt.ev = nxt.fin && uv ? max(cur.ev, exponent_of(__uint_as_float(uv))) : cur.ev;
+        if (nxt.fin) stage(sm + at * BUF, pow2(14 - nxt.ek), pow2(14 - max(nxt.ev, -999)));
+    };
+
+    if (v_lo < v_hi) {
+        load(v_lo);
+        publish(0);
+        __syncthreads();
+        take(0);
+        if (v_lo + KT < v_hi) load(v_lo + KT);
+    }
+    for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
+        // the next tile's maxima; then this tile is whole and the other buffer free
+        cur = nxt;
+        if (v0 + KT < v_hi) publish(at ^ 1);
+        __syncthreads();
+        if (v0 + KT < v_hi) take(at ^ 1);
+        if (v0 + 2 * KT < v_hi) load(v0 + 2 * KT);
+        if (!cur.fin) continue;
+        const uint8_t* buf = sm + at * BUF;
+        if (cur.ev != ev) {
+            if (ev > -1000) {
+                const float f = ldexpf(1.0f, max(ev - cur.ev, -300));
+#pragma unroll
+                for (int d = 0; d < 4; d++) acc[d] *= f;
+            }
+            ev = cur.ev;
+        }
+        // whether every query of the block sees the whole tile
+        const int pa = ks.pos(v0), pb = ks.pos(min(v0 + KT - 1, ks.nv - 1));
+        const bool all = v0 + KT <= v_hi && pb <= (ks.tree ? ks.npos0 - 1 : ks.min_p) &&
+                         (!a.window || (pa >= ks.lo && pa > ks.max_p - a.window) || pb < a.sinks);
+        const float cs = ldexpf(cq, cur.ek - 14);
+        float16v s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.f;
+        {
+            const uint8_t* kp = buf + (kb * 16 + h) * KFRAG + n * 16;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const half8 x = *(const half8*)(kp + 2 * j * KFRAG);
+                if constexpr (LO) {
+                    const half8 y = *(const half8*)(kp + KL + 2 * j * KFRAG);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], s, 0, 0, 0);
+                }
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], s, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] *= cs;
+        if (!all) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int v = v0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3), pos = ks.pos(v), j = pos - ks.npos0;
+                const bool near = !a.window || pos > P - a.window || pos < a.sinks;
+                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask >> (j & 63) & 1) : (j <= row && near));
+                s[i] = vis ? s[i] : -INFINITY;
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[i]);
+        mx = lanes2_max(mx);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        if (__builtin_amdgcn_ballot_w64(mx != m)) {
+            const float al = exp2f(m - ref);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < 4; d++) acc[d] *= al;
+            m = mx;
+        }
+        const float r14 = ref - 14.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[i] = exp2f(s[i] - r14);
+            l += s[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = s[8 * u + i];
+            const Split8 w = split8<true>(x, 1.0f);
+            const uint8_t* vp = buf + VH + (kb * 4 + u * 2 + h) * VGROUP + (n >> 4) * 1024 + (n & 15) * 16;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const half8 x1 = *(const half8*)(vp + d * 256);
+                if constexpr (LO) {
+                    const half8 y1 = *(const half8*)(vp + V_BYTES + d * 256);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y1, w.hi, acc[d], 0, 0, 0);
+                }
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, w.lo, acc[d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, w.hi, acc[d], 0, 0, 0);
+            }
+        }
+    }
+
+    // row r = 8 a + 4 h + b of block d is dim 32 d + 16 (a % 2) + 8 h + 2 b + a / 2
+    if (odd) {
+        // the tiles left out: every wave walks its keys again and takes those of
+        // the tiles that hold infinities or NaN, a weight per key through LDS
+        // (-1: not seen), values by comparison
+        __syncthreads();
+        float* pw = (float*)sm + wave * 1024;
+        const float* q = a.q + (size_t)row * a.ldq + (size_t)head * HD;
+        const float sv = ev > -1000 ? pow2(14 - ev) : 1.f;
+#pragma unroll 1
+        for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
+            bool bad = false;
+            {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + lane, ks.nv - 1)), g, kp, vp);
+#pragma unroll 1
+                for (int u = 0; u < HD; u++) bad |= !(fabsf(to_f32(kp[u])) < INFINITY) || !(fabsf(to_f32(vp[u])) < INFINITY);
+            }
+            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+            float mx = m;
+#pragma unroll 1
+            for (int i = 0; i < 16; i++) {
+                const int kn = 8 * (i >> 2) + 4 * h + (i & 3), v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));
+                const int j = pos - ks.npos0;
+                const bool near = !a.window || pos > P - a.window || pos < a.sinks;
+                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask >> (j & 63) & 1) : (j <= row && near));
+                const T *kp, *vp;
+                key_row(a, ks, pos, g, kp, vp);
+                float d = 0.f;
+#pragma unroll 1
+                for (int u = 0; u < HD; u++) d += q[u] * to_f32(kp[u]);
+                d = vis ? d * c.qscale : -INFINITY;
+                pw[kn * 32 + n] = d;
+                mx = fmaxf(mx, d);
+            }
+            mx = lanes2_max(mx);
+            const float ref = mx == -INFINITY ? 0.f : mx, al = exp2f(m - ref);
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < 4; d++) acc[d] *= al;
+            m = mx;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int kn = 0; kn < 32; kn++) {
+                const float sc = pw[kn * 32 + n], w = exp2f(sc - (ref - 14.f));
+                const bool seen = sc != -INFINITY;
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + 32 * kb + kn, ks.nv - 1)), g, kp, vp);
+                if (h == (kn >> 2 & 1) && seen) l += w;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const float x = to_f32(vp[32 * d + 16 * (i >> 2 & 1) + 8 * h + 2 * (i & 3) + (i >> 3)]);
+                        acc[d][i] += seen ? w * (x * sv) : 0.f;
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    l = lanes2_sum(l);
+    const size_t rh = (size_t)row * a.nh + head;
+    // the second block's waves hand their state to the first's
+    __syncthreads();
+    float* so = (float*)sm + (qg * 64 + lane) * JOIN_ROW;
+    if (kb) {
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) so[16 * d + i] = acc[d][i];
+        so[64] = m;
+        so[65] = l;
+    }
+    __syncthreads();
+    if (kb || q0 + 32 * qg + n >= nq) return;
+    const float m2 = so[64], l2 = so[65], mx = fmaxf(m, m2);
+    const float f1 = m == -INFINITY ? 0.f : exp2f(m - mx), f2 = m2 == -INFINITY ? 0.f : exp2f(m2 - mx);
+    l = l * f1 + l2 * f2;
+    const float un = ev > -1000 ? pow2(ev - 14) : 1.f;
+    const float f = c.nsplit > 1 ? un : l == 0.f ? 0.f : un / l;
+    float* o = c.nsplit > 1 ? c.po + (rh * c.nsplit + split) * HD : a.out + (size_t)row * a.ldo + (size_t)head * HD;
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float x = acc[d][i] * f1 + so[16 * d + i] * f2, y = acc[d][8 + i] * f1 + so[16 * d + 8 + i] * f2;
+            *(float2*)(o + 32 * d + 16 * (i >> 2) + 8 * h + 2 * (i & 3)) = make_float2(x * f, y * f);
+        }
+    if (c.nsplit > 1 && h == 0) {
+        c.pm[rh * c.nsplit + split] = mx;
+        c.pl[rh * c.nsplit + split] = l;
+    }
+}
+
 // The splits of one (row, head) by one wave: out = sum w_c o_c / sum w_c l_c,
 // w_c = 2^(m_c - M); lane = dim pair.  Bound by latency.  grid (b nh / 4).
 __global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
@@ -343,19 +789,24 @@ long long keys_bound(const cmf_attention_args& a, int rows) {
 }
 
 struct Plan {
-    int qb = 1, groups = 1, nsplit = 1;
+    bool tiles = false;  // k_attn_tiles, else k_attn_rows
+    int nb = 1;          // k_attn_rows: 16-query columns of a wave
+    int groups = 1, nsplit = 1;
     size_t bytes = 0;
 };
 
 Plan plan_of(const cmf_attention_args& a) {
     Plan p;
-    const long long nq = (long long)a.b * (a.nh / a.nkv);
-    p.qb = nq <= 16 ? 1 : 2;
-    p.groups = (int)((nq + 16 * p.qb - 1) / (16 * p.qb));
-    const int rows = std::min<long long>(a.b, 16 * p.qb / (a.nh / a.nkv) + 2);
+    const int hpk = a.nh / a.nkv;
+    const long long nq = (long long)a.b * hpk;
+    p.tiles = nq > 32;
+    p.nb = nq <= 16 ? 1 : 2;
+    const int per_wg = p.tiles ? TQ : 16 * p.nb;
+    p.groups = (int)((nq + per_wg - 1) / per_wg);
+    const int rows = (int)std::min<long long>(a.b, per_wg / hpk + 2);
     const long long nv = keys_bound(a, rows);
-    // about two workgroups a CU; a split of at least 64 keys
-    long long ns = 512 / std::max(1ll, (long long)a.nkv * p.groups);
+    // one workgroup a CU of the tiles, two of the rows; a split of at least 64 keys
+    long long ns = (p.tiles ? 256 : 512) / std::max(1ll, (long long)a.nkv * p.groups);
     ns = std::max(1ll, std::min(ns, (nv + 63) / 64));
     const size_t per = (size_t)a.b * a.nh * (HD + 2) * sizeof(float);
     while (ns > 1 && per * ns > OP_WS_MAX) ns--;
@@ -364,11 +815,32 @@ Plan plan_of(const cmf_attention_args& a) {
     return p;
 }
 
+// Allows kernel f its dynamic LDS (once a kernel).
+int allow_lds(const void* f, int bytes) {
+    static std::mutex mu;
+    static std::set<const void*> done;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done.count(f)) {
+        CMF_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.insert(f);
+    }
+    return CMF_OK;
+}
+
 template <class T>
-void launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
+int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
     const dim3 grid((unsigned)c.nsplit * p.groups, c.a.nkv);
-    if (p.qb == 1) hipLaunchKernelGGL((k_attn_rows<T, 1>), grid, dim3(256), 0, s, c);
-    else hipLaunchKernelGGL((k_attn_rows<T, 2>), grid, dim3(256), 0, s, c);
+    if (!p.tiles) {
+        if (p.nb == 1) hipLaunchKernelGGL((k_attn_rows<T, 1>), grid, dim3(256), 0, s, c);
+        else hipLaunchKernelGGL((k_attn_rows<T, 2>), grid, dim3(256), 0, s, c);
+        return CMF_OK;
+    }
+    const void* f = (const void*)k_attn_tiles<T>;
+    if (allow_lds(f, Tile<T>::LDS) != CMF_OK) return CMF_ERR;
+    AttnCall arg = c;
+    void* args[] = {&arg};
+    CMF_HIP(hipLaunchKernel(f, grid, dim3(512), args, Tile<T>::LDS, s));
+    return CMF_OK;
 }
 
 }  // namespace
@@ -385,9 +857,10 @@ int launch_cache_attention(const cmf_attention_args& a, hipStream_t s) {
         c.pm = c.po + rh * HD;
         c.pl = c.pm + rh;
     }
-    if (a.kv_dtype == CMF_DT_F32) launch_t<float>(c, p, s);
-    else if (a.kv_dtype == CMF_DT_F16) launch_t<_Float16>(c, p, s);
-    else launch_t<bf16_t>(c, p, s);
+    const int rc = a.kv_dtype == CMF_DT_F32   ? launch_t<float>(c, p, s)
+                   : a.kv_dtype == CMF_DT_F16 ? launch_t<_Float16>(c, p, s)
+                                              : launch_t<bf16_t>(c, p, s);
+    if (rc != CMF_OK) return rc;
     if (p.nsplit > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(((size_t)a.b * a.nh + 3) / 4)), dim3(256), 0, s, c);
     return CMF_OK;
 }
