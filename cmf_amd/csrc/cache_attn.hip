@@ -25,12 +25,21 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int HD = CACHE_HD;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr long long MAX_ROW_STRIDE = 1 << 22;  // a tile's offsets stay in 32 bits
 
 // the largest of the wave (the same in every lane)
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
+    auto step = [&](auto ctrl) {
+        v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    step(std::integral_constant<int, 0xb1>{});   // quad_perm [1,0,3,2]
+    step(std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
+    step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    step(std::integral_constant<int, 0x140>{});  // row_mirror
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
 }
 
 // max / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -89,6 +98,22 @@ __device__ __forceinline__ Keys keys_of(const cmf_attention_args& a, int r0, int
     return k;
 }
 
+// What a query row sees, as tests without branches: new row j (negative: a
+// cached position) with j <= lim or bit j of mask, and pos > far, pos < sinks
+// or j >= free.
+struct Sight {
+    int lim, far, free;
+    uint64_t mask;
+};
+__device__ __forceinline__ Sight sight_of(const cmf_attention_args& a, const Keys& k, int row) {
+    const int P = k.npos0 + (a.d_depth ? a.d_depth[row] : row);
+    return Sight{k.tree ? -1 : row, a.window ? P - a.window : -1, k.tree ? 0 : 0x7fffffff, k.tree ? a.d_mask[row] : 0};
+}
+__device__ __forceinline__ bool sees(const cmf_attention_args& a, const Keys& k, const Sight& s, int pos) {
+    const int j = pos - k.npos0;
+    return ((j <= s.lim) | ((s.mask >> (j & 63) & 1) != 0)) & ((pos > s.far) | (pos < a.sinks) | (j >= s.free));
+}
+
 template <class T>
 __device__ __forceinline__ void key_row(const cmf_attention_args& a, const Keys& k, int pos, int g, const T*& kp,
                                         const T*& vp) {
@@ -137,14 +162,11 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
 
     // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n
     float qf[QB][32];
-    int row[QB], P[QB];
-    uint64_t mask[QB];
+    Sight see[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         const int qi = min(q0 + 16 * qb + n, nq - 1), r = qi / c.hpk, h = g * c.hpk + qi - r * c.hpk;
-        row[qb] = r;
-        P[qb] = ks.npos0 + (a.d_depth ? a.d_depth[r] : r);
-        mask[qb] = ks.tree ? a.d_mask[r] : 0;
+        see[qb] = sight_of(a, ks, r);
         const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 8 * kq;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -207,11 +229,8 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
             float mx = m[qb];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int v = v0 + 4 * kq + e, pos = ks.pos(v);
-                const int j = pos - ks.npos0;
-                const bool near = !a.window || pos > P[qb] - a.window || pos < a.sinks;
-                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask[qb] >> (j & 63) & 1) : (j <= row[qb] && near));
-                s[e] = vis ? s[e] * c.qscale : -INFINITY;
+                const int v = v0 + 4 * kq + e;
+                s[e] = (sees(a, ks, see[qb], ks.pos(v)) & (v < v_hi)) ? s[e] * c.qscale : -INFINITY;
                 mx = fmaxf(mx, s[e]);
             }
             mx = lanes4_max(mx);
@@ -306,12 +325,14 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
 // qh.kl + ql.kh and p.v likewise (22-bit operands, f32 sums; a 16-bit cache has
 // no kl and vl), three products at 16 times the f32 MFMA's rate.
 //
-// f16 has 5 exponent bits, so every operand is scaled by a power of two first
-// (exact): a query row and a tile of keys to a largest magnitude in [2^14,
-// 2^15), undone in the scores; values by the largest of all tiles so far (the
-// accumulated output follows when that grows); weights are 2^(s - m + 14).
-// What the halves drop is then 2^-22 of an element, and elements down to
-// 2^-29 of the largest keep 11 bits.  A tile that holds infinities or NaN
+// f16 has 5 exponent bits, so operands of an unusual size are scaled by a power
+// of two first (exact): 4 keys or 8 keys' values at a time whose largest
+// magnitude is not in [2^-2, 2^6) to [2^2, 2^3), a query row always, to [2^14,
+// 2^15).  The keys' factor is undone in the scores, the values' in the weights
+// (2^(s - m + 6), m at most 8 below the maximum), relative to the largest
+// factor so far (the accumulated output follows when that grows).  What the
+// halves drop is then 2^-23 of an element or of its group's largest.
+// A block of 32 keys that holds infinities, NaN or values 2^12 from the others'
 // (anything in a row that some query does not see) is left for a second walk
 // without MFMAs, so that it reaches only the queries that see it.
 //
@@ -321,10 +342,18 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
 // in registers.  Eight waves: four groups of 32 queries, the two 32-key blocks
 // of a tile on different waves, joined at the end.  Two tile buffers: while one
 // is multiplied, the next tile, in registers since the tile before, is split
-// into the other, and the one after is loaded; one barrier a tile.
+// into the other, and the one after is loaded; one barrier a tile.  The two
+// waves of a SIMD (block 0 and 1) go through a tile half a turn apart, so that
+// the vector work of one runs beside the products of the other:
+//   block 0: scores t | weights t       | values t           | stage t + 1
+//   block 1: weights t - 1 | values t - 1 | stage K t + 1, V t | scores t
+// (only block 1's waves stage and read its values, a tile later).
 //
 // Bound by the MFMAs: 1536 cycles per tile and wave at f32.
-// grid (nsplit ceil(b hpk / 128), nkv), block 512, LDS Tile<T>::LDS.
+// grid nsplit ceil(b hpk / 128) nkv, block 512, LDS Tile<T>::LDS: the items
+// (split fastest, then query block, then kv head) in eight runs, one to an
+// XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
+// same keys.
 // ---------------------------------------------------------------------------
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -332,17 +361,19 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int KT = 64, TQ = 128;     // keys of a tile, queries of a workgroup
+constexpr float SHIFT = 6.f, LAZY = 8.f;  // weights are 2^(s - m + SHIFT) <= 2^(SHIFT + LAZY)
 constexpr int KFRAG = 528;           // 32 keys x 8 dims (512 B), padded against bank conflicts
 constexpr int K_BYTES = 32 * KFRAG;  // one half (hi or lo) of the keys
 constexpr int VGROUP = 2048;         // 8 keys x 128 dims: [dim % 2][dim / 2][8 keys]
 constexpr int V_BYTES = 8 * VGROUP;
-constexpr int JOIN_ROW = 67, JOIN_BYTES = 4 * 64 * JOIN_ROW * 4;  // the second block's states at the end
+constexpr int OROW = HD + 4;  // f32 rows in LDS: the queries at the start, the eight waves' outputs (32 rows each) at the end
+constexpr int END_BYTES = 8 * 32 * (OROW + 2) * 4;
 template <class T>
 struct Tile {
     static constexpr bool LO = sizeof(T) == 4;
     static constexpr int HALVES = LO ? 2 : 1, BUF = HALVES * (K_BYTES + V_BYTES);
-    static constexpr int USE = 2 * BUF + 2 * 64;  // and the waves' maxima, 8 of K and 8 of V, twice
-    static constexpr int LDS = USE > JOIN_BYTES ? USE : JOIN_BYTES;
+    static constexpr int USE = 2 * (BUF + 128);  // and the exponents of their groups: a block's 8 of K, 4 of V, in 64 bytes
+    static constexpr int LDS = USE > END_BYTES ? USE : END_BYTES;
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
 
@@ -352,18 +383,33 @@ __device__ __forceinline__ float mag(float m, float x) { return __builtin_elemen
 __device__ __forceinline__ int exponent_of(float x) {
     return x == 0.f ? 0 : (int)(__float_as_uint(x) >> 23 & 255) - 127;
 }
+constexpr int SCHED_MFMA = 8, SCHED_LDS = 0x100;  // of sched_group_barrier: MFMAs, LDS reads
 // 2^n for any n (what f32 cannot hold ends at its largest power)
-__device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, min(n, 127)); }
+__device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, max(-300, min(n, 127))); }
+// A group's scale 2^(PLAIN - e) by the largest magnitude of the wave's elements:
+// e = PLAIN where f16 halves take them as they are; all zeros; infinities, NaN
+constexpr int PLAIN = 2, NO_EXP = -1000, BAD_EXP = 1000;
+constexpr int FAR = 12;  // values 2^FAR apart are not summed with each other's halves
+__device__ __forceinline__ int exponent_class(uint32_t u) {  // of a magnitude's bits
+    const int e = (int)(u >> 23) - 127;
+    return u >= 0x7f800000u ? BAD_EXP : u == 0 ? NO_EXP : e >= -2 && e < 6 ? PLAIN : e;
+}
+__device__ __forceinline__ int group_exponent(float mx) {
+    return exponent_class(__builtin_amdgcn_readfirstlane(wave_max_u32(__float_as_uint(mx))));
+}
+__device__ __forceinline__ bool scaled(int e) { return e != PLAIN && e != NO_EXP; }
+__device__ __forceinline__ float group_scale(int e) { return scaled(e) ? pow2(PLAIN - e) : 1.0f; }
 
 struct Split8 {
     half8 hi, lo;
 };
+// x as f16 halves: hi = f16(x), lo = f16(x - hi)
 template <bool LO>
-__device__ __forceinline__ Split8 split8(const float (&x)[8], float scale) {
+__device__ __forceinline__ Split8 split8(const float (&x)[8]) {
     Split8 r;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        const float2v y = {x[i] * scale, x[i + 1] * scale};
+        const float2v y = {x[i], x[i + 1]};
         const half2v h = __builtin_convertvector(y, half2v);
         r.hi[i] = h[0], r.hi[i + 1] = h[1];
         if constexpr (LO) {
@@ -387,7 +433,10 @@ template <class T, int N>
 struct Raw {
     typedef uint32_t vec __attribute__((ext_vector_type(N * sizeof(T) / 4)));
     vec v;
-    __device__ __forceinline__ void load(const T* p) {
+    // from element `off` (below 2^30 bytes) on: a wave-uniform base stays in
+    // scalar registers
+    __device__ __forceinline__ void load(const T* base, uint32_t off) {
+        const char* p = (const char*)base + (uint32_t)(off * sizeof(T));
         if constexpr (N * sizeof(T) == 32) {  // two loads of 16 bytes
             typedef uint32_t q4 __attribute__((ext_vector_type(4)));
             const q4 a = ((const q4*)p)[0], b = ((const q4*)p)[1];
@@ -405,30 +454,99 @@ struct Raw {
         }
     }
 };
+// item of workgroup id of n: the eighth of the items that id's XCD takes
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
+    const uint32_t x = id & 7, k = n >> 3, r = n & 7;
+    return x * k + min(x, r) + (id >> 3);
+}
+
 template <class T>
 __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     const cmf_attention_args& a = c.a;
     constexpr bool LO = Tile<T>::LO;
     constexpr int BUF = Tile<T>::BUF, KL = K_BYTES, VH = Tile<T>::HALVES * K_BYTES, VL = VH + V_BYTES;
     extern __shared__ __align__(16) uint8_t sm[];
-    uint32_t* tmax = (uint32_t*)(sm + 2 * BUF);
+    int* texp = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: 4 of K, 2 of V
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int n = lane & 31, h = lane >> 5, g = blockIdx.y, split = blockIdx.x % c.nsplit;
-    const int q0 = blockIdx.x / c.nsplit * TQ, nq = a.b * c.hpk;
+    const int n = lane & 31, h = lane >> 5, nq = a.b * c.hpk;
+    const uint32_t item = xcd_run(blockIdx.x, gridDim.x), groups = (nq + TQ - 1) / TQ;
+    const int split = item % c.nsplit, g = item / c.nsplit / groups;
+    const int q0 = (item / c.nsplit - g * groups) * TQ;
     const int r0 = q0 / c.hpk, r1 = (min(q0 + TQ, nq) - 1) / c.hpk;
     const Keys ks = keys_of(a, r0, r1);
     const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + KT - 1) / KT * KT;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
     const int qg = wave & 3, kb = wave >> 2;  // the wave's queries and 32-key block
 
+    // what thread t stages of a tile: dims 8 kd .. of keys kk and kk + 32, and
+    // dims 2 lane, 2 lane + 1 of the keys vk + {0 .. 3, 8 .. 11} (the slots of
+    // group (block, 16-key half, h) = wave)
+    const int kd = t & 15, kk = t >> 4, vk = 32 * (wave >> 2) + 16 * (wave >> 1 & 1) + 4 * (wave & 1);
+    Raw<T, 8> kx[2];
+    Raw<T, 2> vx[8];
+    auto one_run = [&](int v0) {  // of the cache
+        return v0 >= ks.s && v0 + KT <= ks.nv && (ks.pos(v0) + KT <= ks.npos0 || !a.k_new);
+    };
+    auto load_k = [&](int v0) {
+        if (one_run(v0)) {
+            const T* kp = (const T*)a.k + (size_t)g * a.head_stride + (size_t)ks.pos(v0) * a.row_stride;
+            uint32_t rs = (uint32_t)a.row_stride;
+            asm("" : "+s"(rs));  // (the offset is not kept over the loop)
+            const uint32_t ko = kk * rs + 8 * kd;
+#pragma unroll
+            for (int r = 0; r < 2; r++) kx[r].load(kp + (size_t)(32 * r) * a.row_stride, ko);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + kk + 32 * r, ks.nv - 1)), g, kp, vp);
+                kx[r].load(kp, 8 * kd);
+            }
+        }
+    };
+    auto load_v = [&](int v0) {
+        if (one_run(v0)) {
+            const T* vp = (const T*)a.v + (size_t)g * a.head_stride + (size_t)(ks.pos(v0) + vk) * a.row_stride;
+#pragma unroll
+            for (int i = 0; i < 8; i++) vx[i].load(vp + (size_t)(8 * (i >> 2) + (i & 3)) * a.row_stride, 2 * lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1)), g, kp, vp);
+                vx[i].load(vp, 2 * lane);
+            }
+        }
+    };
+    if (v_lo < v_hi) {  // under way while the queries are split
+        load_k(v_lo);
+        load_v(v_lo);
+    }
+
     // the wave's queries: lane (n, h) holds dims 16 j + 8 h + i
-    const int qi = min(q0 + 32 * qg + n, nq - 1), row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
-    const int P = ks.npos0 + (a.d_depth ? a.d_depth[row] : row);
-    const uint64_t mask = ks.tree ? a.d_mask[row] : 0;
+    // (row and head are worked out where they are needed: the loop has no
+    // registers left for them)
+    struct Query {
+        int row, head;
+    };
+    auto this_lane = [&]() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); };
+    auto query = [&]() {
+        const int qi = min(q0 + 32 * qg + (this_lane() & 31), nq - 1), row = qi / c.hpk;
+        return Query{row, g * c.hpk + qi - row * c.hpk};
+    };
     half8 qh[8], ql[8];
-    float cq;  // the scores' factor: scale * log2(e) * 2^(eq - 14)
+    float cq;  // the scores' factor: |scale| * log2(e) * 2^(eq - 14)
     {
-        const float* q = a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * h;
+        // whole rows through LDS
+        float* sq = (float*)sm;
+#pragma unroll
+        for (int k = 0; k < TQ / 16; k++) {
+            const int i = 16 * k + (t >> 5), qi = min(q0 + i, nq - 1), row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
+            *(float4*)(sq + i * OROW + 4 * (t & 31)) =
+                *(const float4*)(a.q + (size_t)row * a.ldq + (size_t)head * HD + 4 * (t & 31));
+        }
+        __syncthreads();
+        const float* q = sq + (32 * qg + n) * OROW + 8 * h;
         float x[8][8], mx = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -437,84 +555,66 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[j][i]));
         }
         const int eq = exponent_of(lanes2_max(mx));  // (an infinite or NaN query ends as NaN by itself)
-        const float sc = pow2(14 - eq);
-        cq = ldexpf(c.qscale, eq - 14);
+        const float sc = c.qscale < 0.f ? -pow2(14 - eq) : pow2(14 - eq);
+        cq = fmaxf(fabsf(ldexpf(c.qscale, eq - 14)), 1e-37f);  // (not 0: a score that is not seen is -inf)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const Split8 s = split8<true>(x[j], sc);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[j][i] *= sc;
+            const Split8 s = split8<true>(x[j]);
             qh[j] = s.hi;
             ql[j] = s.lo;
         }
+        __syncthreads();
     }
 
-    // what thread t stages of a tile: dims 8 kd .. of keys kk and kk + 32, and
-    // dims 2 lane, 2 lane + 1 of the keys vk + {0 .. 3, 8 .. 11} (the slots of
-    // group (block, 16-key half, h) = wave)
-    const int kd = t & 15, kk = t >> 4, vk = 32 * (wave >> 2) + 16 * (wave >> 1 & 1) + 4 * (wave & 1);
-    Raw<T, 8> kx[2];
-    Raw<T, 2> vx[8];
-    auto load = [&](int v0) {
-        const int p0 = ks.pos(v0);
-        if (v0 >= ks.s && v0 + KT <= ks.nv && (p0 + KT <= ks.npos0 || !a.k_new)) {  // one run of the cache
-            const size_t o = (size_t)g * a.head_stride + (size_t)p0 * a.row_stride;
-            const T *kp = (const T*)a.k + o + (size_t)kk * a.row_stride + 8 * kd;
-            const T *vp = (const T*)a.v + o + (size_t)vk * a.row_stride + 2 * lane;
-#pragma unroll
-            for (int r = 0; r < 2; r++) kx[r].load(kp + (size_t)(32 * r) * a.row_stride);
-#pragma unroll
-            for (int i = 0; i < 8; i++) vx[i].load(vp + (size_t)(8 * (i >> 2) + (i & 3)) * a.row_stride);
-        } else {
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + kk + 32 * r, ks.nv - 1)), g, kp, vp);
-                kx[r].load(kp + 8 * kd);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1)), g, kp, vp);
-                vx[i].load(vp + 2 * lane);
-            }
-        }
-    };
-    // the largest magnitudes of the tile in registers, into slot `at` (as bits:
-    // NaN is above infinity)
-    auto publish = [&](int at) {
-        float mk = 0.f, mv = 0.f;
+    // The tile in registers into buffer `at`.  This wave stages keys 4 wave ..
+    // 4 wave + 3 of both blocks (with one scale) and the values of group `wave`.
+    auto stage_k = [&](int at) {
+        uint8_t* buf = sm + at * BUF;
+        int* te = texp + at * 32;
+        float mx = 0.f;
 #pragma unroll
         for (int r = 0; r < 2; r++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) mk = mag(mk, kx[r].get(i));
-#pragma unroll
-        for (int i = 0; i < 8; i++) mv = mag(mag(mv, vx[i].get(0)), vx[i].get(1));
-        const uint32_t uk = wave_max_u32(__float_as_uint(mk)), uv = wave_max_u32(__float_as_uint(mv));
-        if (lane == 0) {
-            tmax[16 * at + wave] = uk;
-            tmax[16 * at + 8 + wave] = uv;
-        }
-    };
-    auto stage = [&](uint8_t* buf, float sk, float sv) {
+            for (int i = 0; i < 8; i++) mx = mag(mx, kx[r].get(i));
+        const int e = group_exponent(mx);
+        const float f = group_scale(e);
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = kx[r].get(i);
-            const Split8 s = split8<LO>(x, sk);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] *= f;
+            const Split8 s = split8<LO>(x);
             const int o = (r * 16 + kd) * KFRAG + kk * 16;
             *(half8*)(buf + o) = s.hi;
             if (LO) *(half8*)(buf + KL + o) = s.lo;
+            te[16 * r + 8 * (wave & 1) + (wave >> 1)] = e;  // (all lanes the same)
         }
+    };
+    auto stage_v = [&](int at) {
+        uint8_t* buf = sm + at * BUF;
+        int* te = texp + at * 32;
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mx = mag(mag(mx, vx[i].get(0)), vx[i].get(1));
+        const int e = group_exponent(mx);
+        const float f = group_scale(e);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = vx[i].get(j);
-            const Split8 s = split8<LO>(x, sv);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] *= f;
+            const Split8 s = split8<LO>(x);
             const int o = wave * VGROUP + j * 1024 + lane * 16;
             *(half8*)(buf + VH + o) = s.hi;
             if (LO) *(half8*)(buf + VL + o) = s.lo;
         }
+        te[16 * (wave >> 2) + 8 * (wave & 1) + 4 + (wave >> 1 & 1)] = e;
     };
 
     float16v acc[4];
@@ -523,112 +623,106 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    int ev = -1000;  // the values' exponent so far
+    int ev = NO_EXP;  // the values' exponent so far
     bool odd = false;
-    struct {         // a tile in LDS: what its keys and values were scaled by, whether it is finite
-        int ek, ev;
-        bool fin;
-    } cur{0, -1000, true}, nxt{0, -1000, true};
 
-    // the tile in registers goes to buffer `at` (as nxt, behind cur): scales
-    // from all waves' maxima
-    auto take = [&](int at) {
-        uint32_t uk = 0, uv = 0;
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            uk = max(uk, tmax[16 * at + w]);
-            uv = max(uv, tmax[16 * at + 8 + w]);
-        }
-        uk = __builtin_amdgcn_readfirstlane(uk);
-        uv = __builtin_amdgcn_readfirstlane(uv);
-        nxt.fin = max(uk, uv) < 0x7f800000u;
-        odd |= !nxt.fin;
-        nxt.ek = exponent_of(__uint_as_float(uk));
-        nxt.ev = nxt.fin && uv ? max(cur.ev, exponent_of(__uint_as_float(uv))) : cur.ev;
-        if (nxt.fin) stage(sm + at * BUF, pow2(14 - nxt.ek), pow2(14 - max(nxt.ev, -999)));
-    };
-
-    if (v_lo < v_hi) {
-        load(v_lo);
-        publish(0);
-        __syncthreads();
-        take(0);
-        if (v_lo + KT < v_hi) load(v_lo + KT);
-    }
-    for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
-        // the next tile's maxima; then this tile is whole and the other buffer free
-        cur = nxt;
-        if (v0 + KT < v_hi) publish(at ^ 1);
-        __syncthreads();
-        if (v0 + KT < v_hi) take(at ^ 1);
-        if (v0 + 2 * KT < v_hi) load(v0 + 2 * KT);
-        if (!cur.fin) continue;
+    constexpr int RD = LO ? 2 : 1, MM = LO ? 3 : 2;  // fragments read and products of a step
+    float16v s;         // the block's scores, by 1 / cq
+    bool kbad = false;  // its keys hold infinities or NaN
+    // the scores of the wave's block of the tile at v0, in buffer `at`
+    auto scores = [&](int v0, int at) {
         const uint8_t* buf = sm + at * BUF;
-        if (cur.ev != ev) {
-            if (ev > -1000) {
-                const float f = ldexpf(1.0f, max(ev - cur.ev, -300));
+        const int4 ek = *(const int4*)(texp + at * 32 + 16 * kb + 8 * h);
+        const uint8_t* kp = buf + (kb * 16 + h) * KFRAG + n * 16;
 #pragma unroll
-                for (int d = 0; d < 4; d++) acc[d] *= f;
+        for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const half8 x = *(const half8*)(kp + 2 * j * KFRAG);
+            if constexpr (LO) {
+                const half8 y = *(const half8*)(kp + KL + 2 * j * KFRAG);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], s, 0, 0, 0);
             }
-            ev = cur.ev;
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], s, 0, 0, 0);
         }
-        // whether every query of the block sees the whole tile
+        // the fragments of three steps are read ahead of the products
+        __builtin_amdgcn_sched_group_barrier(SCHED_LDS, 3 * RD + 1, 0);
+#pragma unroll
+        for (int j = 0; j < 5; j++) {
+            __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, MM, 0);
+            __builtin_amdgcn_sched_group_barrier(SCHED_LDS, RD, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 3 * MM, 0);
+        kbad = false;
+        if (__builtin_amdgcn_ballot_w64((int)scaled(ek.x) | (int)scaled(ek.y) | (int)scaled(ek.z) | (int)scaled(ek.w))) {
+            kbad = __builtin_amdgcn_ballot_w64(max(max(ek.x, ek.y), max(ek.z, ek.w)) == BAD_EXP) != 0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int e = i == 0 ? ek.x : i == 4 ? ek.y : i == 8 ? ek.z : ek.w;
+                const float f = scaled(e) ? ldexpf(1.0f, e - PLAIN) : 1.0f;
+#pragma unroll
+                for (int b = 0; b < 4; b++) s[i + b] *= f;
+            }
+        }
+        // whether every query of the workgroup sees the whole tile
         const int pa = ks.pos(v0), pb = ks.pos(min(v0 + KT - 1, ks.nv - 1));
         const bool all = v0 + KT <= v_hi && pb <= (ks.tree ? ks.npos0 - 1 : ks.min_p) &&
                          (!a.window || (pa >= ks.lo && pa > ks.max_p - a.window) || pb < a.sinks);
-        const float cs = ldexpf(cq, cur.ek - 14);
-        float16v s;
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.f;
-        {
-            const uint8_t* kp = buf + (kb * 16 + h) * KFRAG + n * 16;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const half8 x = *(const half8*)(kp + 2 * j * KFRAG);
-                if constexpr (LO) {
-                    const half8 y = *(const half8*)(kp + KL + 2 * j * KFRAG);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[j], s, 0, 0, 0);
-                }
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[j], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[j], s, 0, 0, 0);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] *= cs;
         if (!all) {
+            const Sight see = sight_of(a, ks, query().row);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int v = v0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3), pos = ks.pos(v), j = pos - ks.npos0;
-                const bool near = !a.window || pos > P - a.window || pos < a.sinks;
-                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask >> (j & 63) & 1) : (j <= row && near));
-                s[i] = vis ? s[i] : -INFINITY;
+                const int v = v0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                s[i] = (sees(a, ks, see, ks.pos(v)) & (v < v_hi)) ? s[i] : -INFINITY;
             }
         }
-        float mx = m;
+    };
+    // their weights and the values' sum, from buffer `at`
+    auto values = [&](int at) {
+        const int2 ew = *(const int2*)(texp + at * 32 + 16 * kb + 8 * h + 4);
+        int follow = 0;
+        if (kbad || __builtin_amdgcn_ballot_w64((ew.x != ev) | (ew.y != ev))) {
+            // other scales than so far: all zeros, a new largest one (the output so
+            // far follows), or too far from it for the weights' halves
+            int hi = max(ew.x, ew.y), lo = min(ew.x == NO_EXP ? BAD_EXP : ew.x, ew.y == NO_EXP ? BAD_EXP : ew.y);
+            hi = max(ev, max(__builtin_amdgcn_readlane(hi, 0), __builtin_amdgcn_readlane(hi, 32)));
+            lo = min(ev == NO_EXP ? BAD_EXP : ev, min(__builtin_amdgcn_readlane(lo, 0), __builtin_amdgcn_readlane(lo, 32)));
+            if (kbad || hi == BAD_EXP || (lo < BAD_EXP && hi - lo > FAR)) {
+                odd = true;
+                return;
+            }
+            follow = ev == NO_EXP ? 0 : ev - hi;
+            ev = hi;
+        }
+        // m is the largest score up to 2^LAZY: the sums follow only when a score
+        // passes that
+        float mx = s[0];
 #pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[i]);
-        mx = lanes2_max(mx);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        if (__builtin_amdgcn_ballot_w64(mx != m)) {
-            const float al = exp2f(m - ref);
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+        mx = lanes2_max(mx) * cq;
+        if (follow || __builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
+            const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1)), f = ldexpf(al, follow);
             l *= al;
 #pragma unroll
-            for (int d = 0; d < 4; d++) acc[d] *= al;
-            m = mx;
+            for (int d = 0; d < 4; d++) acc[d] *= f;
+            m = m1;
         }
-        const float r14 = ref - 14.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            s[i] = exp2f(s[i] - r14);
-            l += s[i];
-        }
+        const float ref = (m == -INFINITY ? 0.f : m) - SHIFT;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            float x[8];
+            // the weights in units of the values' scale, their sum in its own
+            const int e = u ? ew.y : ew.x, de = e == NO_EXP ? 0 : e - ev;
+            const float ru = ref - (float)de;
+            float x[8], lu = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = s[8 * u + i];
-            const Split8 w = split8<true>(x, 1.0f);
-            const uint8_t* vp = buf + VH + (kb * 4 + u * 2 + h) * VGROUP + (n >> 4) * 1024 + (n & 15) * 16;
+            for (int i = 0; i < 8; i++) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], cq, -ru));
+                lu += x[i];
+            }
+            l = fmaf(lu, ldexpf(1.0f, -de), l);
+            const Split8 w = split8<true>(x);
+            const uint8_t* vp = sm + at * BUF + VH + (kb * 4 + u * 2 + h) * VGROUP + (n >> 4) * 1024 + (n & 15) * 16;
 #pragma unroll
             for (int d = 0; d < 4; d++) {
                 const half8 x1 = *(const half8*)(vp + d * 256);
@@ -640,100 +734,156 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, w.hi, acc[d], 0, 0, 0);
             }
         }
-    }
+        __builtin_amdgcn_sched_group_barrier(SCHED_LDS, 2 * RD, 1);
+#pragma unroll
+        for (int j = 0; j < 6; j++) {
+            __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, MM, 1);
+            __builtin_amdgcn_sched_group_barrier(SCHED_LDS, RD, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 2 * MM, 1);
+    };
 
-    // row r = 8 a + 4 h + b of block d is dim 32 d + 16 (a % 2) + 8 h + 2 b + a / 2
-    if (odd) {
-        // the tiles left out: every wave walks its keys again and takes those of
-        // the tiles that hold infinities or NaN, a weight per key through LDS
-        // (-1: not seen), values by comparison
-        __syncthreads();
-        float* pw = (float*)sm + wave * 1024;
-        const float* q = a.q + (size_t)row * a.ldq + (size_t)head * HD;
-        const float sv = ev > -1000 ? pow2(14 - ev) : 1.f;
-#pragma unroll 1
-        for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
-            bool bad = false;
-            {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + lane, ks.nv - 1)), g, kp, vp);
-#pragma unroll 1
-                for (int u = 0; u < HD; u++) bad |= !(fabsf(to_f32(kp[u])) < INFINITY) || !(fabsf(to_f32(vp[u])) < INFINITY);
-            }
-            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
-            float mx = m;
-#pragma unroll 1
-            for (int i = 0; i < 16; i++) {
-                const int kn = 8 * (i >> 2) + 4 * h + (i & 3), v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));
-                const int j = pos - ks.npos0;
-                const bool near = !a.window || pos > P - a.window || pos < a.sinks;
-                const bool vis = v < v_hi && (j < 0 ? near : ks.tree ? (mask >> (j & 63) & 1) : (j <= row && near));
-                const T *kp, *vp;
-                key_row(a, ks, pos, g, kp, vp);
-                float d = 0.f;
-#pragma unroll 1
-                for (int u = 0; u < HD; u++) d += q[u] * to_f32(kp[u]);
-                d = vis ? d * c.qscale : -INFINITY;
-                pw[kn * 32 + n] = d;
-                mx = fmaxf(mx, d);
-            }
-            mx = lanes2_max(mx);
-            const float ref = mx == -INFINITY ? 0.f : mx, al = exp2f(m - ref);
-            l *= al;
-#pragma unroll
-            for (int d = 0; d < 4; d++) acc[d] *= al;
-            m = mx;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-            for (int kn = 0; kn < 32; kn++) {
-                const float sc = pw[kn * 32 + n], w = exp2f(sc - (ref - 14.f));
-                const bool seen = sc != -INFINITY;
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + 32 * kb + kn, ks.nv - 1)), g, kp, vp);
-                if (h == (kn >> 2 & 1) && seen) l += w;
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const float x = to_f32(vp[32 * d + 16 * (i >> 2 & 1) + 8 * h + 2 * (i & 3) + (i >> 3)]);
-                        acc[d][i] += seen ? w * (x * sv) : 0.f;
-                    }
-            }
-            __builtin_amdgcn_wave_barrier();
+    if (v_lo < v_hi) {
+        stage_k(0);
+        if (kb == 0) stage_v(0);
+        if (v_lo + KT < v_hi) {
+            load_k(v_lo + KT);
+            if (kb == 0) load_v(v_lo + KT);
         }
     }
-    l = lanes2_sum(l);
-    const size_t rh = (size_t)row * a.nh + head;
-    // the second block's waves hand their state to the first's
+    if (kb == 0) {
+        for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
+            __syncthreads();  // this tile is whole, the other buffer free
+            scores(v0, at);
+            values(at);
+            if (v0 + KT < v_hi) {
+                stage_k(at ^ 1);
+                stage_v(at ^ 1);
+                if (v0 + 2 * KT < v_hi) {
+                    load_k(v0 + 2 * KT);
+                    load_v(v0 + 2 * KT);
+                }
+            }
+        }
+        __syncthreads();
+    } else {
+        int at = 0;
+        for (int v0 = v_lo; v0 < v_hi; v0 += KT, at ^= 1) {
+            __syncthreads();
+            if (v0 > v_lo) values(at ^ 1);
+            stage_v(at);
+            if (v0 + KT < v_hi) {
+                stage_k(at ^ 1);
+                load_v(v0 + KT);
+                if (v0 + 2 * KT < v_hi) load_k(v0 + 2 * KT);
+            }
+            scores(v0, at);
+        }
+        __syncthreads();
+        if (v_lo < v_hi) values(at ^ 1);
+    }
+
+    // The wave's state into LDS, in the values' own units (row r = 8 a + 4 h + b
+    // of block d is dim 32 d + 16 (a % 2) + 8 h + 2 b + a / 2), the weights by
+    // 2^-(SHIFT + LAZY) so that sums of large values stay finite.
     __syncthreads();
-    float* so = (float*)sm + (qg * 64 + lane) * JOIN_ROW;
-    if (kb) {
+    float* so = (float*)sm + wave * 32 * OROW;
+    float2* ml = (float2*)((float*)sm + 8 * 32 * OROW) + wave * 32;  // (m, l)
+    const int lane1 = this_lane(), n1 = lane1 & 31, h1 = lane1 >> 5;
+    {
+        const float un = ldexpf(ev > NO_EXP ? pow2(ev - PLAIN) : 1.f, -(int)(SHIFT + LAZY));
 #pragma unroll
         for (int d = 0; d < 4; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) so[16 * d + i] = acc[d][i];
-        so[64] = m;
-        so[65] = l;
+            for (int i = 0; i < 8; i++)
+                *(float2*)(so + n1 * OROW + 32 * d + 16 * (i >> 2) + 8 * h1 + 2 * (i & 3)) =
+                    make_float2(acc[d][i] * un, acc[d][8 + i] * un);
+        l = ldexpf(lanes2_sum(l), -(int)(SHIFT + LAZY));  // (m and l: the same in both lanes of a query)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __syncthreads();
-    if (kb || q0 + 32 * qg + n >= nq) return;
-    const float m2 = so[64], l2 = so[65], mx = fmaxf(m, m2);
-    const float f1 = m == -INFINITY ? 0.f : exp2f(m - mx), f2 = m2 == -INFINITY ? 0.f : exp2f(m2 - mx);
-    l = l * f1 + l2 * f2;
-    const float un = ev > -1000 ? pow2(ev - 14) : 1.f;
-    const float f = c.nsplit > 1 ? un : l == 0.f ? 0.f : un / l;
-    float* o = c.nsplit > 1 ? c.po + (rh * c.nsplit + split) * HD : a.out + (size_t)row * a.ldo + (size_t)head * HD;
-#pragma unroll
-    for (int d = 0; d < 4; d++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float x = acc[d][i] * f1 + so[16 * d + i] * f2, y = acc[d][8 + i] * f1 + so[16 * d + 8 + i] * f2;
-            *(float2*)(o + 32 * d + 16 * (i >> 2) + 8 * h + 2 * (i & 3)) = make_float2(x * f, y * f);
+    if (odd) {
+        // The blocks left out: the wave walks its blocks again, with the scales
+        // that the first walk went through (es), and takes those it left key by
+        // key, in f32; lane (n, h) has half the dims of its query.
+        const Query w = query();
+        const Sight see = sight_of(a, ks, w.row);
+        const float* q = a.q + (size_t)w.row * a.ldq + (size_t)w.head * HD + 64 * h1;
+        float* o = so + n1 * OROW + 64 * h1;
+        int es = NO_EXP;
+#pragma unroll 1
+        for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
+            bool bad = false;  // infinities or NaN among the tile's keys
+            float mv = 0.f;    // the largest of value row n of the block
+#pragma unroll 1
+            for (int r = 0; r < 2; r++) {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + 32 * r + n1, ks.nv - 1)), g, kp, vp);
+#pragma unroll 1
+                for (int u = 0; u < HD; u++) {
+                    bad |= !(fabsf(to_f32(kp[u])) < INFINITY);
+                    if (r == kb) mv = mag(mv, to_f32(vp[u]));
+                }
+            }
+            uint32_t um = __float_as_uint(mv);  // of its group: keys 16 u + 4 h1 + {0 .. 3, 8 .. 11}
+            um = max(um, (uint32_t)__shfl_xor((int)um, 1));
+            um = max(um, (uint32_t)__shfl_xor((int)um, 2));
+            um = max(um, (uint32_t)__shfl_xor((int)um, 8));
+            int hi = exponent_class(um), lo = hi == NO_EXP ? BAD_EXP : hi;
+            hi = max(hi, __shfl_xor(hi, 4));
+            lo = min(lo, __shfl_xor(lo, 4));
+            hi = max(hi, __shfl_xor(hi, 16));
+            lo = min(lo, __shfl_xor(lo, 16));
+            hi = max(es, __builtin_amdgcn_readfirstlane(hi));
+            lo = min(es == NO_EXP ? BAD_EXP : es, __builtin_amdgcn_readfirstlane(lo));
+            if (!__builtin_amdgcn_ballot_w64(bad) && hi != BAD_EXP && !(lo < BAD_EXP && hi - lo > FAR)) {
+                es = hi;
+                continue;
+            }
+#pragma unroll 1
+            for (int kn = 0; kn < 32; kn++) {
+                const int v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));
+                const bool vis = sees(a, ks, see, pos) & (v < v_hi);
+                const T *kp, *vp;
+                key_row(a, ks, pos, g, kp, vp);
+                float d = 0.f;
+#pragma unroll 4
+                for (int u = 0; u < 64; u++) d = fmaf(q[u], to_f32(kp[64 * h1 + u]), d);
+                d = lanes2_sum(d) * c.qscale;
+                if (!vis) continue;
+                const float m1 = fmaxf(m, d), ref = m1 == -INFINITY ? 0.f : m1, al = exp2f(m - ref), wt = ldexpf(exp2f(d - ref), -(int)LAZY);
+#pragma unroll 4
+                for (int u = 0; u < 64; u++) o[u] = o[u] * al + wt * to_f32(vp[64 * h1 + u]);
+                l = l * al + wt;
+                m = m1;
+            }
         }
-    if (c.nsplit > 1 && h == 0) {
-        c.pm[rh * c.nsplit + split] = mx;
-        c.pl[rh * c.nsplit + split] = l;
+    }
+    if (h1 == 0) ml[n1] = make_float2(m, l);
+    __syncthreads();
+    // The two blocks of every query meet; whole rows out, 32 lanes each.
+    const int t1 = wave * 64 + lane1;
+#pragma unroll 4
+    for (int k = t1 >> 5; k < TQ; k += 16) {
+        const int qi = q0 + k;
+        if (qi >= nq) continue;
+        const float* x = (const float*)sm + k * OROW + 4 * (t1 & 31);
+        const float2* e = (const float2*)((const float*)sm + 8 * 32 * OROW) + k;
+        const float2 e1 = e[0], e2 = e[TQ];
+        const float mx = fmaxf(e1.x, e2.x);
+        const float f1 = e1.x == -INFINITY ? 0.f : exp2f(e1.x - mx), f2 = e2.x == -INFINITY ? 0.f : exp2f(e2.x - mx);
+        const float lt = e1.y * f1 + e2.y * f2, f = c.nsplit > 1 ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
+        const float4v y = (*(const float4v*)x * f1 + *(const float4v*)(x + TQ * OROW) * f2) * f;
+        const int row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
+        if (c.nsplit > 1) {
+            const size_t at = ((size_t)row * a.nh + head) * c.nsplit + split;
+            *(float4v*)(c.po + at * HD + 4 * (t1 & 31)) = y;
+            if ((t1 & 31) == 0) {
+                c.pm[at] = mx;
+                c.pl[at] = lt;
+            }
+        } else {
+            *(float4v*)(a.out + (size_t)row * a.ldo + (size_t)head * HD + 4 * (t1 & 31)) = y;
+        }
     }
 }
 
@@ -839,7 +989,7 @@ int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
     if (allow_lds(f, Tile<T>::LDS) != CMF_OK) return CMF_ERR;
     AttnCall arg = c;
     void* args[] = {&arg};
-    CMF_HIP(hipLaunchKernel(f, grid, dim3(512), args, Tile<T>::LDS, s));
+    CMF_HIP(hipLaunchKernel(f, dim3(grid.x * grid.y), dim3(512), args, Tile<T>::LDS, s));
     return CMF_OK;
 }
 
@@ -882,6 +1032,7 @@ static int check_attention(const cmf_attention_args* p) {
     if (a.row_stride < HD || a.row_stride % 8 || a.head_stride < 0 || a.head_stride % 8 ||
         (a.k_new && (a.new_row_stride < HD || a.new_row_stride % 8 || a.new_head_stride < 0 || a.new_head_stride % 8)))
         return fail("attention: strides must be multiples of 8 elements, rows of 128");
+    if (a.row_stride > MAX_ROW_STRIDE) return fail("attention: row_stride of at most 2^22 elements");
     const long long need = (long long)a.pos0 + (a.k_new ? 0 : a.b);
     if (!a.d_pos0 && need > a.slots) return fail("attention: positions past the cache's slots");
     if (a.d_pos0 && (a.len_bound < 0 || (long long)a.len_bound + (a.k_new ? 0 : a.b) > a.slots))

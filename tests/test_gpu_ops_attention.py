@@ -201,6 +201,25 @@ def test_garbage_seen_by_some_rows_of_a_chunk(ops, ws, bad, what):
     assert not np.isfinite(out[40:60]).any()
 
 
+@pytest.mark.parametrize("big", [1e4, 1e10, 1e30])
+@pytest.mark.parametrize("b", [5, 64])
+def test_values_of_another_size_seen_by_some_rows(ops, ws, b, big):
+    """A leaf of a tree, and a cached position that only the first rows see
+    through their window, hold values `big` times the others': the rows that do
+    not see them keep their accuracy."""
+    ctx, window = 300, 280
+    r = np.random.default_rng(13)
+    q, k, v = tensors(r, b, ctx, 16, 4, "float32")
+    _, kn, vn = tensors(r, b, b, 16, 4, "float32")
+    mask, depth = ops.tree_masks([-1] + [max(0, i - 2) for i in range(1, b)], pos0=ctx, window=window)
+    v[:, ctx - window + 1] *= np.float32(big)  # seen at depth 0 alone
+    vn[:, b - 1] *= np.float32(big)
+    see = visible(b, ctx, window, 0, mask, depth)
+    want, tol = reference(q, np.concatenate([k, kn], 1), np.concatenate([v, vn], 1), see)
+    out = run_tree(ops, ws, q, k, v, kn, vn, "float32", ctx, mask, depth, window)
+    check(out, want, tol)
+
+
 @pytest.mark.parametrize("size", [1e-18, 1e18])
 @pytest.mark.parametrize("b", [4, 64])
 def test_far_ranges(ops, ws, b, size):
