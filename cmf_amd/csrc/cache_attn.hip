@@ -21,7 +21,18 @@ namespace cmf {
 
 namespace {
 
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 constexpr int HD = CACHE_HD;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -56,15 +67,28 @@ __device__ __forceinline__ float lanes4_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// the larger magnitude; NaN stays
+__device__ __forceinline__ float mag(float m, float x) { return __builtin_elementwise_maximum(m, fabsf(x)); }
+// the exponent e of a positive finite x in [2^e, 2^(e+1)), 0 for 0
+__device__ __forceinline__ int exponent_of(float x) {
+    return x == 0.f ? 0 : (int)(__float_as_uint(x) >> 23 & 255) - 127;
+}
+// 2^n for any n (what f32 cannot hold ends at its largest power)
+__device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, max(-300, min(n, 127))); }
+
 // A call as the kernels take it.
 struct AttnCall {
     cmf_attention_args a;
     int hpk;         // query heads per kv head
+    uint32_t inv;    // ceil(2^32 / hpk): query / hpk = high word of query * inv
     int nsplit;      // key splits per query block; 1: the output itself
     float qscale;    // scale * log2(e)
     float *pm, *pl;  // [b * nh][nsplit] partial maxima (log2 units) and sums
     float* po;       // [b * nh][nsplit][128], relative to the maximum
 };
+
+// row of query qi (exact: queries and hpk multiply to less than 2^32)
+__device__ __forceinline__ int row_of(const AttnCall& c, int qi) { return c.hpk == 1 ? qi : (int)__umulhi((uint32_t)qi, c.inv); }
 
 // The keys that the rows [r0, r1] of a block see, numbered [0, nv): positions
 // [0, s), then [lo, lo + nv - s).
@@ -128,6 +152,89 @@ __device__ __forceinline__ void key_row(const cmf_attention_args& a, const Keys&
     }
 }
 
+// N elements as they lie in memory, and as f32
+template <class T, int N>
+struct Raw {
+    typedef uint32_t vec __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+    vec v;
+    // from element `off` (below 2^30 bytes) on: a wave-uniform base stays in
+    // scalar registers
+    __device__ __forceinline__ void load(const T* base, uint32_t off) {
+        const char* p = (const char*)base + (uint32_t)(off * sizeof(T));
+        if constexpr (N * sizeof(T) == 32) {  // two loads of 16 bytes
+            const uint4v a = ((const uint4v*)p)[0], b = ((const uint4v*)p)[1];
+            v = vec{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        } else {
+            v = *(const vec*)p;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(v[i]);
+        } else {
+            const uint16_t u = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+            return to_f32(__builtin_bit_cast(T, u));
+        }
+    }
+};
+// A 16-bit cache's elements are MFMA operands as they are; the f32 side comes in
+// parts of their type that add up to it: two of f16 (22 bits, from values
+// scaled into f16's range), three of bf16 (24 bits, f32's range).
+template <class T>
+struct Part;
+template <>
+struct Part<_Float16> {
+    static constexpr int N = 2;
+    static constexpr float SHIFT = 6.f, LAZY = 8.f;  // weights 2^(s - m + SHIFT) <= 2^(SHIFT + LAZY) < 65504
+    static constexpr bool SCALED = true;
+    static constexpr uint32_t INF = 0x7c00;
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{x, y}), half2v));
+    }
+    static __device__ __forceinline__ float lo(uint32_t u) { return (float)__builtin_bit_cast(half2v, u)[0]; }
+    static __device__ __forceinline__ float hi(uint32_t u) { return (float)__builtin_bit_cast(half2v, u)[1]; }
+    static __device__ __forceinline__ float4v mm32(uint4v a, uint4v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4v mm16(uint2v a, uint2v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Part<bf16_t> {
+    static constexpr int N = 3;
+    static constexpr float SHIFT = 0.f, LAZY = 12.f;
+    static constexpr bool SCALED = false;
+    static constexpr uint32_t INF = 0x7f80;
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{x, y}), bf2v));
+    }
+    static __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u << 16); }
+    static __device__ __forceinline__ float hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+    static __device__ __forceinline__ float4v mm32(uint4v a, uint4v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4v mm16(uint2v a, uint2v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, a), __builtin_bit_cast(short4v, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Part<float> {
+    static constexpr int N = 1;
+    static constexpr float SHIFT = 0.f, LAZY = 12.f;
+    static constexpr bool SCALED = false;
+};
+// x as the parts p[0 .. N) of two values
+template <class T>
+__device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::N]) {
+#pragma unroll
+    for (int k = 0; k < Part<T>::N; k++) {
+        p[k] = Part<T>::pack(x, y);
+        x -= Part<T>::lo(p[k]);
+        y -= Part<T>::hi(p[k]);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Few queries per kv head (decode rows, small trees): the scores and values
 // in f32 on the 16x16x4 MFMA, K and V straight from memory into its operands.
@@ -140,45 +247,96 @@ __device__ __forceinline__ void key_row(const cmf_attention_args& a, const Keys&
 // loads 8 consecutive dims 32 j + 8 kq of key m (K) and 16 bytes at a time of
 // keys 4 kq + e (V).  Softmax with a running maximum, one column a lane.
 // Four waves take a workgroup's 16-key tiles in turn and meet in LDS in wave
-// order.  f32 operands: no rounding of the inputs, any range.
+// order.  f32 caches: f32 operands, no rounding of the inputs, any range.
+// 16-bit caches: K (16x16x32) and V (16x16x16, its four keys per lane packed by
+// dim) are operands as they lie in memory, the queries and weights in parts.
 //
 // Bound by the cache's bytes: 16 KiB of f32 K/V per tile against 64 MFMAs of
-// 32 cycles per 16 queries.
-// grid (nsplit ceil(b hpk / 16 QB), nkv), block 256.
+// 32 cycles per 16 queries, 8 KiB of f16 against 24 of 16.
+// grid (nsplit, nkv, ceil(b hpk / 16 QB) <= 2), block 256.
 // ---------------------------------------------------------------------------
 template <class T, int QB>
-__global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
+__global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     const cmf_attention_args& a = c.a;
-    constexpr int NW = 4, QN = 16 * QB;
+    constexpr int NW = 4, QN = 16 * QB, OROW = HD + 4;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr float SHIFT = Part<T>::SHIFT, LAZY = Part<T>::LAZY;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 15, kq = lane >> 4, split = blockIdx.x % c.nsplit, g = blockIdx.y, q0 = blockIdx.x / c.nsplit * QN;
+    const int n = lane & 15, kq = lane >> 4, split = blockIdx.x, g = blockIdx.y, q0 = blockIdx.z * QN;
     const int nq = a.b * c.hpk;
-    const int r0 = q0 / c.hpk, r1 = (min(q0 + QN, nq) - 1) / c.hpk;
+    const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + QN, nq) - 1);
     const Keys ks = keys_of(a, r0, r1);
 
-    // this split's keys, whole rounds of the four waves
-    const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + 16 * NW - 1) / (16 * NW) * (16 * NW);
+    // this split's keys, whole tiles
+    const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + 15) / 16 * 16;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
 
+    // A tile as it lies in memory: K row n, and V rows 4 kq + e, 16 bytes at a
+    // time (component i of lane m is dim 64 (i / 4) + 4 m + i % 4 of f32 rows,
+    // 8 m + i of 16-bit ones).  Numbers past the end read the last key.
+    constexpr int VP = sizeof(T) == 4 ? 2 : 1;
+    Raw<T, 8> kn[4];
+    Raw<T, 16 / sizeof(T)> vn[4][VP];
+    auto load = [&](int v0) {
+        const T *kp, *vp;
+        key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+#pragma unroll
+        for (int j = 0; j < 4; j++) kn[j].load(kp, 32 * j + 8 * kq);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const T *kp2, *vp2;
+            key_row(a, ks, ks.pos(min(v0 + 4 * kq + e, ks.nv - 1)), g, kp2, vp2);
+#pragma unroll
+            for (int u = 0; u < VP; u++) vn[e][u].load(vp2, 64 * u + (VP == 2 ? 4 : 8) * n);
+        }
+    };
+    if (v_lo + 16 * wave < v_hi) load(v_lo + 16 * wave);
+
     // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n
-    float qf[QB][32];
+    constexpr int QF = F32 ? 32 : 1, QP = F32 ? 1 : 4;
+    float qf[QB][QF], cq[QB];  // cq: what the scores are multiplied by, positive
+    uint4v qp[QB][QP][Part<T>::N];
     Sight see[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
-        const int qi = min(q0 + 16 * qb + n, nq - 1), r = qi / c.hpk, h = g * c.hpk + qi - r * c.hpk;
+        const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
         see[qb] = sight_of(a, ks, r);
         const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 8 * kq;
+        float x[32];
+        float f = c.qscale < 0.f ? -1.f : 1.f;
+        int eq = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float t[8];
             load8(q + 32 * j, t);
 #pragma unroll
-            for (int i = 0; i < 8; i++) qf[qb][8 * j + i] = t[i];
+            for (int i = 0; i < 8; i++) x[8 * j + i] = t[i];
+        }
+        if constexpr (Part<T>::SCALED) {
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(x[i]));
+            eq = exponent_of(lanes4_max(mx)) - 14;
+            f *= pow2(-eq);
+        }
+        cq[qb] = fmaxf(fabsf(ldexpf(c.qscale, eq)), 1e-37f);  // (not 0: a score that is not seen is -inf)
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) qf[qb][i] = x[i] * f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                uint32_t p[Part<T>::N];
+                parts2<T>(x[i] * f, x[i + 1] * f, p);
+#pragma unroll
+                for (int k = 0; k < Part<T>::N; k++) qp[qb][i >> 3][k][(i & 7) >> 1] = p[k];
+            }
         }
     }
 
     float4v acc[QB][8];
     float m[QB], l[QB];
+    bool odd = false;
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         m[qb] = -INFINITY;
@@ -188,123 +346,193 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
     }
 
     for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
-        // K row n, then V rows 4 kq + e (numbers past the end read the last key)
-        float kf[32], vf[4][8];
-        const T *kp, *vp;
-        key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+        // a tile with infinities or NaN in V (0 * v is NaN then) is left for the
+        // walk at the end
+        bool bad;
+        if constexpr (F32) {
+            float x = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float t[8];
-            load8(kp + 32 * j + 8 * kq, t);
+            for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) kf[8 * j + i] = t[i];
+                for (int i = 0; i < 8; i++) x = fmaf(vn[e][i / (8 / VP)].get(i % (8 / VP)), 0.f, x);
+            bad = x != x;
+        } else {
+            ushort2v x = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    x = __builtin_elementwise_max(x, __builtin_bit_cast(ushort2v, vn[e][0].v[i] & 0x7fff7fffu));
+            bad = max((int)x[0], (int)x[1]) >= (int)Part<std::conditional_t<F32, bf16_t, T>>::INF;
         }
-        // dims of component i of lane m: f32 64 (i / 4) + 4 m + i % 4, else 8 m + i
+        if (__builtin_amdgcn_ballot_w64(bad) == 0) {
+            float4v s[QB];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const T *kp2, *vp2;
-            key_row(a, ks, ks.pos(min(v0 + 4 * kq + e, ks.nv - 1)), g, kp2, vp2);
-            if constexpr (sizeof(T) == 4) {
-                const float4 x = ((const float4*)vp2)[n], y = ((const float4*)vp2)[16 + n];
-                vf[e][0] = x.x, vf[e][1] = x.y, vf[e][2] = x.z, vf[e][3] = x.w;
-                vf[e][4] = y.x, vf[e][5] = y.y, vf[e][6] = y.z, vf[e][7] = y.w;
+            for (int qb = 0; qb < QB; qb++) s[qb] = float4v{0.f, 0.f, 0.f, 0.f};
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++)
+                        s[qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kn[i >> 3].get(i & 7), qf[qb][i], s[qb], 0, 0, 0);
             } else {
-                load8(vp2 + 8 * n, vf[e]);
+#pragma unroll
+                for (int k = Part<T>::N - 1; k >= 0; k--)  // the small parts first
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int qb = 0; qb < QB; qb++)
+                            s[qb] = Part<T>::mm32(__builtin_bit_cast(uint4v, kn[j].v), qp[qb][j][k], s[qb]);
             }
-        }
-        // infinities and NaN in V (0 * v is NaN then): such a tile's values go
-        // by comparisons, not by products with weights of zero
-        float odd = 0.f;
+            const bool inside = v0 + 16 <= v_hi;
+            bool grow = false;
+            float mx[QB];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+            for (int qb = 0; qb < QB; qb++) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) odd = fmaf(vf[e][i], 0.f, odd);
-        const bool finite = __builtin_amdgcn_ballot_w64(odd != odd) == 0;
-
-#pragma unroll
-        for (int qb = 0; qb < QB; qb++) {
-            float4v s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 32; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i], qf[qb][i], s, 0, 0, 0);
-            float mx = m[qb];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int v = v0 + 4 * kq + e;
-                s[e] = (sees(a, ks, see[qb], ks.pos(v)) & (v < v_hi)) ? s[e] * c.qscale : -INFINITY;
-                mx = fmaxf(mx, s[e]);
+                for (int e = 0; e < 4; e++) {
+                    const int v = v0 + 4 * kq + e;
+                    s[qb][e] = (sees(a, ks, see[qb], ks.pos(v)) & (inside | (v < v_hi))) ? s[qb][e] * cq[qb] : -INFINITY;
+                }
+                mx[qb] = lanes4_max(fmaxf(fmaxf(s[qb][0], s[qb][1]), fmaxf(s[qb][2], s[qb][3])));
+                grow |= mx[qb] > m[qb] + LAZY;
             }
-            mx = lanes4_max(mx);
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            const float al = exp2f(m[qb] - ref);
-            m[qb] = mx;
-            float4v p;
+            if (__builtin_amdgcn_ballot_w64(grow)) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = exp2f(s[e] - ref);
-            l[qb] = l[qb] * al + (p[0] + p[1] + p[2] + p[3]);
+                for (int qb = 0; qb < QB; qb++) {
+                    const float m1 = fmaxf(m[qb], mx[qb]), al = exp2f(m[qb] - (m1 == -INFINITY ? 0.f : m1));
+                    m[qb] = m1;
+                    l[qb] *= al;
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[qb][i] *= al;
-            if (finite) {
+                    for (int i = 0; i < 8; i++) acc[qb][i] *= al;
+                }
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) {
+                const float ref = (m[qb] == -INFINITY ? 0.f : m[qb]) - SHIFT;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[qb][e] = __builtin_amdgcn_exp2f(s[qb][e] - ref);
+                    l[qb] += s[qb][e];
+                }
+            }
+            if constexpr (F32) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        acc[qb][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][i], p[e], acc[qb][i], 0, 0, 0);
+#pragma unroll
+                        for (int qb = 0; qb < QB; qb++)
+                            acc[qb][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vn[e][i / (8 / VP)].get(i % (8 / VP)), s[qb][e],
+                                                                             acc[qb][i], 0, 0, 0);
             } else {
-                // output row 4 kq + e2 of block i is component i of lane 4 kq + e2
-                for (int k = 0; k < 16; k++) {
-                    const int e = k & 3, from = (lane & 15) + 16 * (k >> 2);
-                    const float pe = e == 0 ? p[0] : e == 1 ? p[1] : e == 2 ? p[2] : p[3];
-                    const float se = e == 0 ? s[0] : e == 1 ? s[1] : e == 2 ? s[2] : s[3];
-                    const float pk = __shfl(pe, from), sk = __shfl(se, from);
+                uint2v w[QB][Part<T>::N];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float ve = e == 0 ? vf[0][i] : e == 1 ? vf[1][i] : e == 2 ? vf[2][i] : vf[3][i];
+                for (int qb = 0; qb < QB; qb++)
 #pragma unroll
-                        for (int e2 = 0; e2 < 4; e2++) {
-                            const float vv = __shfl(ve, 16 * (k >> 2) + 4 * kq + e2);
-                            acc[qb][i][e2] += sk == -INFINITY ? 0.f : pk * vv;
-                        }
+                    for (int e = 0; e < 4; e += 2) {
+                        uint32_t p[Part<T>::N];
+                        parts2<T>(s[qb][e], s[qb][e + 1], p);
+#pragma unroll
+                        for (int k = 0; k < Part<T>::N; k++) w[qb][k][e >> 1] = p[k];
                     }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    // dim 8 n + i of the lane's four keys
+                    const uint32_t sel = i & 1 ? 0x07060302 : 0x05040100;
+                    const uint2v x = {__builtin_amdgcn_perm(vn[1][0].v[i >> 1], vn[0][0].v[i >> 1], sel),
+                                      __builtin_amdgcn_perm(vn[3][0].v[i >> 1], vn[2][0].v[i >> 1], sel)};
+#pragma unroll
+                    for (int k = Part<T>::N - 1; k >= 0; k--)
+#pragma unroll
+                        for (int qb = 0; qb < QB; qb++) acc[qb][i] = Part<T>::mm16(x, w[qb][k], acc[qb][i]);
                 }
             }
+        } else {
+            odd = true;
         }
+        if (v0 + 16 * NW < v_hi) load(v0 + 16 * NW);
     }
 
-    // the four waves' states, in wave order
-    __shared__ float sm[NW][QN], sl[NW][QN];
-    __shared__ __align__(16) float so[NW][QN][HD + 4];
+    // the wave's state into LDS
+    __shared__ float2 sml[NW][QN];
+    __shared__ __align__(16) float so[NW][QN][OROW];
+    const float un = pow2(-(int)(SHIFT + LAZY));  // (sums of large values stay finite)
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
-        const float lt = lanes4_sum(l[qb]);
-        if (kq == 0) {
-            sm[wave][16 * qb + n] = m[qb];
-            sl[wave][16 * qb + n] = lt;
-        }
+        l[qb] = lanes4_sum(l[qb]) * un;
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int r = 4 * kq + e;
-                so[wave][16 * qb + n][sizeof(T) == 4 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[qb][i][e];
+                so[wave][16 * qb + n][VP == 2 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[qb][i][e] * un;
             }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (odd) {
+        // the tiles left out, key by key; lane (n, kq) has 32 dims of its query
+#pragma unroll 1
+        for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
+            bool bad = false;
+            {
+                const T *kp, *vp;
+                key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+#pragma unroll 1
+                for (int u = 0; u < 32; u++) bad |= !(fabsf(to_f32(vp[32 * kq + u])) < INFINITY);
+            }
+            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+#pragma unroll 1
+            for (int k = 0; k < 16; k++) {
+                const int v = v0 + k, pos = ks.pos(min(v, ks.nv - 1));
+                const T *kp, *vp;
+                key_row(a, ks, pos, g, kp, vp);
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) {
+                    const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
+                    const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 32 * kq;
+                    float d = 0.f;
+#pragma unroll 4
+                    for (int u = 0; u < 32; u++) d = fmaf(q[u], to_f32(kp[32 * kq + u]), d);
+                    d = lanes4_sum(d) * c.qscale;
+                    if (!(sees(a, ks, see[qb], pos) & (v < v_hi))) continue;
+                    float* o = &so[wave][16 * qb + n][32 * kq];
+                    const float m1 = fmaxf(m[qb], d), ref = m1 == -INFINITY ? 0.f : m1;
+                    const float al = exp2f(m[qb] - ref), wt = exp2f(d - ref - LAZY);
+#pragma unroll 4
+                    for (int u = 0; u < 32; u++) o[u] = o[u] * al + wt * to_f32(vp[32 * kq + u]);
+                    l[qb] = l[qb] * al + wt;
+                    m[qb] = m1;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++)
+        if (kq == 0) sml[wave][16 * qb + n] = make_float2(m[qb], l[qb]);
     __syncthreads();
+    // the four waves meet, in wave order; whole rows out
+#pragma unroll
     for (int t = threadIdx.x; t < QN * 32; t += 256) {
         const int qq = t >> 5, d = (t & 31) * 4, qi = q0 + qq;
         if (qi >= nq) continue;
-        float M = sm[0][qq];
+        float2 e[NW];
+        float M = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < NW; w++) M = fmaxf(M, sm[w][qq]);
+        for (int w = 0; w < NW; w++) {
+            e[w] = sml[w][qq];
+            M = fmaxf(M, e[w].x);
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         float4v o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = sm[w][qq] == -INFINITY ? 0.f : exp2f(sm[w][qq] - M);
-            L += sl[w][qq] * f;
-            const float4v x = *(const float4v*)&so[w][qq][d];
-            if (sm[w][qq] != -INFINITY) o += x * f;
+            const float f = exp2f(e[w].x - ref);  // (a wave without keys: 0, and its state is zeros)
+            L += e[w].y * f;
+            o += *(const float4v*)&so[w][qq][d] * f;
         }
-        const int r = qi / c.hpk, h = g * c.hpk + qi - r * c.hpk;
+        const int r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
         if (c.nsplit == 1) {
             const float inv = L == 0.f ? 0.f : 1.0f / L;
             *(float4v*)(a.out + (size_t)r * a.ldo + (size_t)h * HD + d) = o * inv;
@@ -355,10 +583,6 @@ __global__ __launch_bounds__(256) void k_attn_rows(AttnCall c) {
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
 // same keys.
 // ---------------------------------------------------------------------------
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float float2v __attribute__((ext_vector_type(2)));
-typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int KT = 64, TQ = 128;     // keys of a tile, queries of a workgroup
 constexpr float SHIFT = 6.f, LAZY = 8.f;  // weights are 2^(s - m + SHIFT) <= 2^(SHIFT + LAZY)
@@ -377,15 +601,7 @@ struct Tile {
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
 
-// the larger magnitude; NaN stays
-__device__ __forceinline__ float mag(float m, float x) { return __builtin_elementwise_maximum(m, fabsf(x)); }
-// the exponent e of a positive finite x in [2^e, 2^(e+1)), 0 for 0
-__device__ __forceinline__ int exponent_of(float x) {
-    return x == 0.f ? 0 : (int)(__float_as_uint(x) >> 23 & 255) - 127;
-}
 constexpr int SCHED_MFMA = 8, SCHED_LDS = 0x100;  // of sched_group_barrier: MFMAs, LDS reads
-// 2^n for any n (what f32 cannot hold ends at its largest power)
-__device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, max(-300, min(n, 127))); }
 // A group's scale 2^(PLAIN - e) by the largest magnitude of the wave's elements:
 // e = PLAIN where f16 halves take them as they are; all zeros; infinities, NaN
 constexpr int PLAIN = 2, NO_EXP = -1000, BAD_EXP = 1000;
@@ -428,32 +644,6 @@ __device__ __forceinline__ float lanes2_sum(float v) {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-// N elements as they lie in memory, and as f32
-template <class T, int N>
-struct Raw {
-    typedef uint32_t vec __attribute__((ext_vector_type(N * sizeof(T) / 4)));
-    vec v;
-    // from element `off` (below 2^30 bytes) on: a wave-uniform base stays in
-    // scalar registers
-    __device__ __forceinline__ void load(const T* base, uint32_t off) {
-        const char* p = (const char*)base + (uint32_t)(off * sizeof(T));
-        if constexpr (N * sizeof(T) == 32) {  // two loads of 16 bytes
-            typedef uint32_t q4 __attribute__((ext_vector_type(4)));
-            const q4 a = ((const q4*)p)[0], b = ((const q4*)p)[1];
-            v = vec{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        } else {
-            v = *(const vec*)p;
-        }
-    }
-    __device__ __forceinline__ float get(int i) const {
-        if constexpr (sizeof(T) == 4) {
-            return __uint_as_float(v[i]);
-        } else {
-            const uint16_t u = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
-            return to_f32(__builtin_bit_cast(T, u));
-        }
-    }
-};
 // item of workgroup id of n: the eighth of the items that id's XCD takes
 __device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t n) {
     const uint32_t x = id & 7, k = n >> 3, r = n & 7;
@@ -472,7 +662,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     const uint32_t item = xcd_run(blockIdx.x, gridDim.x), groups = (nq + TQ - 1) / TQ;
     const int split = item % c.nsplit, g = item / c.nsplit / groups;
     const int q0 = (item / c.nsplit - g * groups) * TQ;
-    const int r0 = q0 / c.hpk, r1 = (min(q0 + TQ, nq) - 1) / c.hpk;
+    const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + TQ, nq) - 1);
     const Keys ks = keys_of(a, r0, r1);
     const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + KT - 1) / KT * KT;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
@@ -531,7 +721,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     };
     auto this_lane = [&]() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); };
     auto query = [&]() {
-        const int qi = min(q0 + 32 * qg + (this_lane() & 31), nq - 1), row = qi / c.hpk;
+        const int qi = min(q0 + 32 * qg + (this_lane() & 31), nq - 1), row = row_of(c, qi);
         return Query{row, g * c.hpk + qi - row * c.hpk};
     };
     half8 qh[8], ql[8];
@@ -541,7 +731,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         float* sq = (float*)sm;
 #pragma unroll
         for (int k = 0; k < TQ / 16; k++) {
-            const int i = 16 * k + (t >> 5), qi = min(q0 + i, nq - 1), row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
+            const int i = 16 * k + (t >> 5), qi = min(q0 + i, nq - 1), row = row_of(c, qi), head = g * c.hpk + qi - row * c.hpk;
             *(float4*)(sq + i * OROW + 4 * (t & 31)) =
                 *(const float4*)(a.q + (size_t)row * a.ldq + (size_t)head * HD + 4 * (t & 31));
         }
@@ -873,7 +1063,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         const float f1 = e1.x == -INFINITY ? 0.f : exp2f(e1.x - mx), f2 = e2.x == -INFINITY ? 0.f : exp2f(e2.x - mx);
         const float lt = e1.y * f1 + e2.y * f2, f = c.nsplit > 1 ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
         const float4v y = (*(const float4v*)x * f1 + *(const float4v*)(x + TQ * OROW) * f2) * f;
-        const int row = qi / c.hpk, head = g * c.hpk + qi - row * c.hpk;
+        const int row = row_of(c, qi), head = g * c.hpk + qi - row * c.hpk;
         if (c.nsplit > 1) {
             const size_t at = ((size_t)row * a.nh + head) * c.nsplit + split;
             *(float4v*)(c.po + at * HD + 4 * (t1 & 31)) = y;
@@ -888,40 +1078,37 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 }
 
 // The splits of one (row, head) by one wave: out = sum w_c o_c / sum w_c l_c,
-// w_c = 2^(m_c - M); lane = dim pair.  Bound by latency.  grid (b nh / 4).
-__global__ __launch_bounds__(256) void k_attn_join(AttnCall c) {
+// w_c = 2^(m_c - M); lane = dim pair.  The maxima, the sums and CB splits'
+// outputs are requested together, so that up to CB splits take one memory
+// round trip.  Bound by latency.  grid (b nh), block 64.
+template <int CB>
+__global__ __launch_bounds__(64) void k_attn_join(AttnCall c) {
     const cmf_attention_args& a = c.a;
-    const int lane = threadIdx.x & 63;
-    const size_t rh = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (rh >= (size_t)a.b * a.nh) return;
-    const int ns = c.nsplit;
+    const int lane = threadIdx.x, ns = c.nsplit;
+    const size_t rh = blockIdx.x;
     const float* pm = c.pm + rh * ns;
     const float* pl = c.pl + rh * ns;
-    const float2* po = (const float2*)(c.po + rh * ns * HD);
-    float M = -INFINITY;
-    for (int j = lane; j < ns; j += 64) M = fmaxf(M, pm[j]);
-    M = wave_max(M);
-    float L = 0.f;
+    const float2* po = (const float2*)(c.po + rh * ns * HD) + lane;
+    float M = -INFINITY, L = 0.f;
     float2 o = make_float2(0.f, 0.f);
-    for (int j0 = 0; j0 < ns; j0 += 64) {
+    for (int j0 = 0; j0 < ns; j0 += CB) {
+        float2 x[CB];
+#pragma unroll
+        for (int u = 0; u < CB; u++) x[u] = po[(size_t)min(j0 + u, ns - 1) * 64];
         const int j = j0 + lane;
-        const float mj = j < ns ? pm[j] : -INFINITY, lj = j < ns ? pl[j] : 0.f;
-        const float w = mj == -INFINITY ? 0.f : exp2f(mj - M);
-        L += wave_sum(w * lj);
-        const int je = min(64, ns - j0);
-        for (int t0 = 0; t0 < je; t0 += 8) {
-            float2 x[8];
+        const bool in = lane < CB && j < ns;
+        const float mj = in ? pm[min(j, ns - 1)] : -INFINITY, lj = in ? pl[min(j, ns - 1)] : 0.f;
+        const float M1 = fmaxf(M, wave_max(mj)), ref = M1 == -INFINITY ? 0.f : M1;
+        const float al = exp2f(M - ref), w = exp2f(mj - ref);
+        M = M1;
+        L = L * al + wave_sum(w * lj);
+        o.x *= al;
+        o.y *= al;
 #pragma unroll
-            for (int u = 0; u < 8; u++) x[u] = po[(size_t)(j0 + min(t0 + u, je - 1)) * 64 + lane];
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float wu = __shfl(w, min(t0 + u, 63));
-                const float mu = __shfl(mj, min(t0 + u, 63));
-                if (t0 + u < je && mu != -INFINITY) {
-                    o.x += wu * x[u].x;
-                    o.y += wu * x[u].y;
-                }
-            }
+        for (int u = 0; u < CB; u++) {
+            const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), u));
+            o.x = fmaf(wu, x[u].x, o.x);
+            o.y = fmaf(wu, x[u].y, o.y);
         }
     }
     const float inv = L == 0.f ? 0.f : 1.0f / L;
@@ -979,8 +1166,8 @@ int allow_lds(const void* f, int bytes) {
 
 template <class T>
 int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
-    const dim3 grid((unsigned)c.nsplit * p.groups, c.a.nkv);
     if (!p.tiles) {
+        const dim3 grid(c.nsplit, c.a.nkv, p.groups);
         if (p.nb == 1) hipLaunchKernelGGL((k_attn_rows<T, 1>), grid, dim3(256), 0, s, c);
         else hipLaunchKernelGGL((k_attn_rows<T, 2>), grid, dim3(256), 0, s, c);
         return CMF_OK;
@@ -989,7 +1176,7 @@ int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
     if (allow_lds(f, Tile<T>::LDS) != CMF_OK) return CMF_ERR;
     AttnCall arg = c;
     void* args[] = {&arg};
-    CMF_HIP(hipLaunchKernel(f, dim3(grid.x * grid.y), dim3(512), args, Tile<T>::LDS, s));
+    CMF_HIP(hipLaunchKernel(f, dim3((unsigned)c.nsplit * p.groups * c.a.nkv), dim3(512), args, Tile<T>::LDS, s));
     return CMF_OK;
 }
 
@@ -1000,7 +1187,8 @@ size_t cache_attention_ws(const cmf_attention_args& a) { return plan_of(a).bytes
 int launch_cache_attention(const cmf_attention_args& a, hipStream_t s) {
     const Plan p = plan_of(a);
     if (p.bytes > a.ws_bytes || (p.bytes && !a.ws)) return fail("attention: the workspace is too small (cmf_attention_workspace)");
-    AttnCall c{a, a.nh / a.nkv, p.nsplit, (a.scale == 0.f ? 0.08838834764831845f : a.scale) * LOG2E, nullptr, nullptr, nullptr};
+    const uint32_t hpk = a.nh / a.nkv;
+    AttnCall c{a, (int)hpk, (uint32_t)(((1ull << 32) + hpk - 1) / hpk), p.nsplit, (a.scale == 0.f ? 0.08838834764831845f : a.scale) * LOG2E, nullptr, nullptr, nullptr};
     if (p.nsplit > 1) {
         const size_t rh = (size_t)a.b * a.nh * p.nsplit;
         c.po = (float*)a.ws;
@@ -1011,7 +1199,9 @@ int launch_cache_attention(const cmf_attention_args& a, hipStream_t s) {
                    : a.kv_dtype == CMF_DT_F16 ? launch_t<_Float16>(c, p, s)
                                               : launch_t<bf16_t>(c, p, s);
     if (rc != CMF_OK) return rc;
-    if (p.nsplit > 1) hipLaunchKernelGGL(k_attn_join, dim3((unsigned)(((size_t)a.b * a.nh + 3) / 4)), dim3(256), 0, s, c);
+    const dim3 rows((unsigned)(a.b * a.nh));
+    if (p.nsplit > 16) hipLaunchKernelGGL(k_attn_join<32>, rows, dim3(64), 0, s, c);
+    else if (p.nsplit > 1) hipLaunchKernelGGL(k_attn_join<16>, rows, dim3(64), 0, s, c);
     return CMF_OK;
 }
 
@@ -1019,7 +1209,8 @@ static int check_attention(const cmf_attention_args* p) {
     if (!p) return fail("attention: null argument");
     const auto& a = *p;
     if (a.b < 1 || a.nh < 1 || a.nkv < 1 || a.nh % a.nkv) return fail("attention: b, nh, nkv of at least 1, nh a multiple of nkv");
-    if (a.b > (1 << 20) || a.nh > 4096) return fail("attention: at most 2^20 rows and 4096 heads");
+    if (a.b > (1 << 19) || a.nh > 4096 || a.nh / a.nkv > 64)
+        return fail("attention: at most 2^19 rows, 4096 heads, 64 query heads per kv head");
     if (!kv_dtype_ok(a.kv_dtype)) return fail("attention: kv_dtype must be f32, f16 or bf16");
     if (a.pos0 < 0 || a.slots < 0 || a.window < 0 || a.sinks < 0) return fail("attention: pos0, slots, window and sinks of at least 0");
     if (a.slots > (1 << 30) || a.window > (1 << 30) || a.sinks > (1 << 30)) return fail("attention: at most 2^30 positions");

@@ -52,7 +52,7 @@ def attn(**kw):
     (dict(k_new=X, v_new=X, new_row_stride=4), "strides"), (dict(pos0=-1), "at least 0"), (dict(window=-1), "at least 0"),
     (dict(sinks=-2), "at least 0"), (dict(pos0=255), "slots"), (dict(d_pos0=X, len_bound=255), "len_bound"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=X + 8), "aligned"),
-    (dict(b=1 << 21, slots=1 << 30), "2^20"), (dict(slots=(1 << 30) + 1), "2^30"),
+    (dict(b=1 << 20, slots=1 << 30), "2^19"), (dict(nh=130, nkv=2, ldq=130 * 128, ldo=130 * 128), "64 query heads"), (dict(slots=(1 << 30) + 1), "2^30"),
 ])
 def test_attention_refuses(kw, word):
     refused("cmf_attention_dev", attn(**kw), word)
