@@ -6,7 +6,8 @@
 // one is worked on.  Every lane keeps a softmax state of its own (running
 // maximum, sum of weights, sum of weighted differences), every wave the 64
 // largest of its logits, one a lane, in order: a round's logits are compared
-// with the k-th of them and only the few that pass are looked at further.
+// with the k-th of them and only the few that pass are looked at further.  In
+// the first round the k-th of the lanes' own maxima bounds them.
 // The waves and then the slices of a row meet in a fixed order.
 // Bound by the logits' bytes for many rows, by latency for few.
 #include <math.h>
@@ -38,9 +39,8 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) {
     return (uint64_t)u << 32 | (uint32_t)~id;
 }
 __device__ __forceinline__ int key_id(uint64_t k) { return (int)~(uint32_t)k; }
-__device__ __forceinline__ float key_val(uint64_t k) {
+__device__ __forceinline__ float key_val(uint64_t k) {  // (what is below -inf's key: a NaN)
     const uint32_t u = (uint32_t)(k >> 32);
-    if (u == 0) return NAN;
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
@@ -62,11 +62,11 @@ __device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, int lane) {
     for (int o = 32; o; o >>= 1) v = exchange(v, lane, o, !(lane & o));
     return v;
 }
-__device__ __forceinline__ uint64_t wave_sort(uint64_t v, int lane) {
-#pragma unroll
-    for (int n = 2; n <= 64; n <<= 1)
-#pragma unroll
-        for (int o = n >> 1; o; o >>= 1) v = exchange(v, lane, o, !(lane & o) == !(lane & n));
+// Lanes hold sorted lists of n lanes (a power of two), the even ones descending
+// and the odd ones ascending: the wave sorted, descending.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t v, int n, int lane) {
+    for (int m = 2 * n; m <= 64; m <<= 1)
+        for (int o = m >> 1; o; o >>= 1) v = exchange(v, lane, o, !(lane & o) == !(lane & m));
     return v;
 }
 // the 64 largest of two descending lists
@@ -79,7 +79,7 @@ __device__ __forceinline__ uint64_t top_join(uint64_t a, uint64_t b, int lane) {
 // and join about 250).
 __device__ __forceinline__ uint64_t top_take(uint64_t best, uint64_t key, uint64_t bound, int k, int lane) {
     uint64_t pass = __builtin_amdgcn_ballot_w64(key > bound);
-    if (__builtin_popcountll(pass) > 12) return top_join(best, wave_sort(key, lane), lane);
+    if (__builtin_popcountll(pass) > 12) return top_join(best, merge_lists(key, 1, lane), lane);
     while (pass) {
         const uint64_t x = lane64(key, __builtin_ctzll(pass));
         pass &= pass - 1;
@@ -104,12 +104,10 @@ __device__ __forceinline__ Soft soft_join(const Soft& a, const Soft& b) {
     return Soft{m, a.z * fa + b.z * fb, (a.h + a.z * da) * fa + (b.h + b.z * db) * fb};
 }
 __device__ __forceinline__ Soft soft_wave(Soft s) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const Soft t{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.h, o)};
-        s = soft_join(s, t);
-    }
-    return s;
+    const auto add = [](float a, float b) { return a + b; };
+    const float m = wave_reduce_f32(s.m, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+    const float d = fmaxf((s.m - (m == -INFINITY ? 0.f : m)) * LOG2E, -1000.f), f = exp2f(d);
+    return Soft{m, wave_reduce_f32(s.z * f, 0.f, add), wave_reduce_f32((s.h + s.z * d) * f, 0.f, add)};
 }
 
 struct LpCall {
@@ -123,6 +121,24 @@ struct LpShared {
     Soft soft[LT / 64];
     uint64_t top[LT / 64][64];
 };
+
+// The largest of `lists` sorted lists of k keys: list j's key e is at
+// src[j * ld + e].  As many lists as fit the wave's lanes are merged at a time,
+// starting from list `from` groups in and `step` groups on.
+__device__ __forceinline__ uint64_t top_lists(const uint64_t* src, int ld, int lists, int k, int from, int step, int lane) {
+    const int n = k <= 1 ? 1 : 1 << (32 - __builtin_clz(k - 1)), each = 64 / n;
+    const int j = lane / n, e = j & 1 ? n - 1 - (lane & (n - 1)) : lane & (n - 1);
+    auto load = [&](int g) { return g * each + j < lists && e < k ? src[(size_t)(g * each + j) * ld + e] : 0; };
+    const int groups = (lists + each - 1) / each;
+    uint64_t best = 0, next = from < groups ? load(from) : 0;
+    for (int g = from; g < groups; g += step) {
+        uint64_t v = next;
+        if (g + step < groups) next = load(g + step);
+        v = merge_lists(v, n, lane);
+        best = g == from ? v : top_join(best, v, lane);
+    }
+    return best;
+}
 
 // the row's results from its state and list (wave 0, all lanes hold s)
 __device__ __forceinline__ void lp_write(const cmf_logprobs_args& a, int row, const Soft& s, uint64_t best, float xt,
@@ -196,12 +212,24 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
         s.m = mx;
 #pragma unroll
         for (int i = 0; i < LV; i++) {
-            const float d = (v[i] - ref) * LOG2E, p = exp2f(d);
+            const float d = (v[i] - ref) * LOG2E, p = __builtin_amdgcn_exp2f(d);  // (what is under 2^-126 adds nothing to 1)
             s.z += p;
             s.h = fmaf(p, fmaxf(d, -1000.f), s.h);
         }
         if constexpr (TOP) {
             uint64_t bound = lane64(best, a.top_k - 1);
+            if (r0 == lo) {
+                // top_k lanes' maxima are at or above this: the upper half of its bits, one by one
+                // (a lane whose maximum is -inf may hold no logit, or NaN: not counted)
+                const uint32_t u = mx > -INFINITY ? (uint32_t)(key_of(mx, 0) >> 32) : 0;
+                uint32_t b = 0;
+#pragma unroll
+                for (int bit = 31; bit >= 16; bit--) {
+                    const uint32_t up = b | 1u << bit;
+                    if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(u >= up)) >= a.top_k) b = up;
+                }
+                bound = (uint64_t)b << 32;
+            }
             float bv = key_val(bound);
 #pragma unroll
             for (int i = 0; i < LV; i++) {
@@ -210,7 +238,8 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
                 const bool may = !(v[i] < bv) && id >= 0 && id < a.V && r0 + (long long)(i / VE * LT + t) * VE < hi;
                 if (__builtin_amdgcn_ballot_w64(may)) {
                     best = top_take(best, may ? key_of(v[i], id) : 0, bound, a.top_k, lane);
-                    bound = lane64(best, a.top_k - 1);
+                    const uint64_t last = lane64(best, a.top_k - 1);
+                    bound = last > bound ? last : bound;
                     bv = key_val(bound);
                 }
             }
@@ -227,10 +256,7 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
     s = sh.soft[0];
 #pragma unroll
     for (int w = 1; w < LT / 64; w++) s = soft_join(s, sh.soft[w]);
-    if constexpr (TOP) {
-#pragma unroll
-        for (int w = 1; w < LT / 64; w++) best = top_join(best, sh.top[w][lane], lane);
-    }
+    if constexpr (TOP) best = top_lists(sh.top[0], 64, LT / 64, a.top_k, 0, 1, lane);
     if (c.nslice == 1) {
         lp_write(a, row, s, best, xt, lane);
         return;
@@ -258,10 +284,7 @@ __global__ __launch_bounds__(LT) void k_logprobs_join(LpCall c) {
     if (lane == 0) sh.soft[wave] = s;
     uint64_t best = 0;
     if constexpr (TOP) {
-        for (int j = wave; j < c.nslice; j += LT / 64) {
-            const uint64_t b = lane < a.top_k ? c.top[(at + j) * a.top_k + lane] : 0;
-            best = j == wave ? b : top_join(best, b, lane);
-        }
+        best = top_lists(c.top + at * a.top_k, a.top_k, c.nslice, a.top_k, wave, LT / 64, lane);
         sh.top[wave][lane] = best;
     }
     __syncthreads();
@@ -269,10 +292,7 @@ __global__ __launch_bounds__(LT) void k_logprobs_join(LpCall c) {
     s = sh.soft[0];
 #pragma unroll
     for (int w = 1; w < LT / 64; w++) s = soft_join(s, sh.soft[w]);
-    if constexpr (TOP) {
-#pragma unroll
-        for (int w = 1; w < LT / 64; w++) best = top_join(best, sh.top[w][lane], lane);
-    }
+    if constexpr (TOP) best = top_lists(sh.top[0], 64, LT / 64, a.top_k, 0, 1, lane);
     lp_write(a, row, s, best, xt, lane);
 }
 

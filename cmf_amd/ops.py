@@ -21,8 +21,7 @@ import numpy as np
 from . import AttentionArgs, CmfError, DevBuf, KvCopyArgs, LogprobsArgs, QkRopeArgs, _ptr, check, lib
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
-_DTYPES = {"torch.float32": DT_F32, "torch.float16": DT_F16, "torch.bfloat16": DT_BF16, "float32": DT_F32,
-           "float16": DT_F16, "bfloat16": DT_BF16}
+_DTYPES = {"float32": DT_F32, "float16": DT_F16, "bfloat16": DT_BF16}
 STREAM_NULL = 1  # CMF_STREAM_NULL
 WORKSPACE_MAX = 64 << 20  # no call asks for more scratch
 
@@ -97,9 +96,22 @@ class DevTensor:
         return a.astype(np.float32) if self.dtype == "float16" else a
 
 
+# The wrappers are on the path of every drafted token, so they read each of a
+# tensor's properties once and write a message only when it is needed.
+_SEEN = {}  # dtype object -> its plain name ("float32")
+
+
+def _name(t):
+    d = t.dtype
+    try:
+        return _SEEN[d]
+    except KeyError:
+        return _SEEN.setdefault(d, str(d).replace("torch.", ""))
+
+
 def _dt(t):
     try:
-        return _DTYPES[str(t.dtype)]
+        return _DTYPES[_name(t)]
     except KeyError:
         raise CmfError(f"dtype {t.dtype}: f32, f16 or bf16") from None
 
@@ -118,28 +130,32 @@ def _want(ok, what):
 
 
 def _f32(t, what):
-    _want(_dt(t) == DT_F32, f"{what} must be f32")
+    if _name(t) != "float32":
+        raise CmfError(f"{what} must be f32")
 
 
 def _i32(t, n, what):
-    if t is not None:
-        _want(str(t.dtype) in ("torch.int32", "int32") and t.stride()[-1] == 1 and t.shape[0] >= n,
-              f"{what} must be int32, contiguous, of at least {n}")
+    if t is not None and not (_name(t) == "int32" and t.stride()[-1] == 1 and t.shape[0] >= n):
+        raise CmfError(f"{what} must be int32, contiguous, of at least {n}")
 
 
 def _cache(k, v, what):
     """k and v [nkv][slots][128] of one layout -> (nkv, slots, head, row)."""
-    _want(len(k.shape) == 3 and k.shape[2] == 128 and k.stride()[2] == 1, f"{what} must be [heads][rows][128]")
-    _want(k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype, f"{what}: k and v differ in layout")
-    return k.shape[0], k.shape[1], k.stride()[0], k.stride()[1]
+    shape, st = k.shape, k.stride()
+    if not (len(shape) == 3 and shape[2] == 128 and st[2] == 1):
+        raise CmfError(f"{what} must be [heads][rows][128]")
+    if v is not k and not (v.shape == shape and v.stride() == st and v.dtype == k.dtype):
+        raise CmfError(f"{what}: k and v differ in layout")
+    return shape[0], shape[1], st[0], st[1]
 
 
 def _rows(t, what):
     """t [b][heads][128] -> (b, heads, ld)."""
-    _want(len(t.shape) == 3 and t.shape[2] == 128 and t.stride()[2] == 1 and (t.shape[1] == 1 or t.stride()[1] == 128),
-          f"{what} must be [rows][heads][128] with contiguous heads")
-    b, h, _ = t.shape
-    return b, h, t.stride()[0] if b > 1 else max(t.stride()[0], h * 128)
+    shape, st = t.shape, t.stride()
+    if not (len(shape) == 3 and shape[2] == 128 and st[2] == 1 and (shape[1] == 1 or st[1] == 128)):
+        raise CmfError(f"{what} must be [rows][heads][128] with contiguous heads")
+    b, h, _ = shape
+    return b, h, st[0] if b > 1 else max(st[0], h * 128)
 
 
 def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=None, at_pos=True, eps=1e-6, stream=None):
@@ -181,7 +197,7 @@ def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, s
         nk, rows, nhst, nrst = _cache(k_new, v_new, "k_new / v_new")
         _want(nk == nkv and rows >= b and k_new.dtype == k.dtype, "k_new / v_new must hold b rows of k's type")
     if mask is not None:
-        _want(str(mask.dtype) in ("torch.int64", "torch.uint64", "int64", "uint64") and mask.shape[0] >= b and
+        _want(_name(mask) in ("int64", "uint64") and mask.shape[0] >= b and
               mask.stride()[0] == 1, "mask must be [b] of 64 bits")
     _i32(depth, b, "depth")
     _i32(pos0_dev, 1, "pos0_dev")
@@ -230,7 +246,7 @@ def kv_copy(dst_ptrs, src_ptrs, dst, src, *, n, pos0=0, idx=None, n_dev=None, po
     nk, ss, sh, sr = _cache(src, src, "src")
     _want(nk == nkv and src.dtype == dst.dtype, "dst and src must have the same heads and type")
     for t in (dst_ptrs, src_ptrs):
-        _want(str(t.dtype) in ("torch.int64", "int64") and t.stride()[0] == 1, "pointers must be int64, contiguous")
+        _want(_name(t) == "int64" and t.stride()[0] == 1, "pointers must be int64, contiguous")
     _want(dst_ptrs.shape[0] == src_ptrs.shape[0], "as many buffers on both sides")
     _i32(idx, n, "idx")
     _i32(n_dev, 1, "n_dev")
@@ -253,7 +269,7 @@ def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws,
             _want(len(t.shape) == 2 and t.shape[0] >= rows and t.shape[1] == top_k and tuple(t.stride()) == (top_k, 1),
                   f"{w} must be [rows][top_k], contiguous")
     if top_ids is not None:
-        _want(str(top_ids.dtype) in ("torch.int32", "int32"), "top_ids must be int32")
+        _want(_name(top_ids) == "int32", "top_ids must be int32")
     if top_lp is not None:
         _f32(top_lp, "top_lp")
     nb = 0 if ws is None else ws.shape[0] * ws.element_size()
