@@ -129,28 +129,64 @@ struct Sight {
     int lim, far, free;
     uint64_t mask;
 };
+// A row's depth and mask bits as read; without them its queries' first bytes,
+// not used (no branch: the loads are under way together).
+struct SightIn {
+    int depth;
+    uint64_t mask;
+};
+__device__ __forceinline__ SightIn sight_in(const cmf_attention_args& a, int row) {
+    const float* q = a.q + (size_t)row * a.ldq;
+    return SightIn{*(a.d_depth ? a.d_depth + row : (const int*)q),
+                   *(a.d_mask ? (const uint64_t*)a.d_mask + row : (const uint64_t*)q)};
+}
+__device__ __forceinline__ Sight sight_of(const cmf_attention_args& a, const Keys& k, int row, const SightIn& in) {
+    const int P = k.npos0 + (a.d_depth ? in.depth : row);
+    return Sight{k.tree ? -1 : row, a.window ? P - a.window : -1, k.tree ? 0 : 0x7fffffff, k.tree ? in.mask : 0};
+}
 __device__ __forceinline__ Sight sight_of(const cmf_attention_args& a, const Keys& k, int row) {
-    const int P = k.npos0 + (a.d_depth ? a.d_depth[row] : row);
-    return Sight{k.tree ? -1 : row, a.window ? P - a.window : -1, k.tree ? 0 : 0x7fffffff, k.tree ? a.d_mask[row] : 0};
+    return sight_of(a, k, row, sight_in(a, row));
 }
 __device__ __forceinline__ bool sees(const cmf_attention_args& a, const Keys& k, const Sight& s, int pos) {
     const int j = pos - k.npos0;
     return ((j <= s.lim) | ((s.mask >> (j & 63) & 1) != 0)) & ((pos > s.far) | (pos < a.sinks) | (j >= s.free));
 }
 
+// The key and value rows of a kv head, as cached rows and new ones.  The
+// addresses are held in registers: chosen among the arguments themselves, a row
+// would cost a load of the chosen argument before its own.
 template <class T>
-__device__ __forceinline__ void key_row(const cmf_attention_args& a, const Keys& k, int pos, int g, const T*& kp,
-                                        const T*& vp) {
-    if (pos < k.npos0 || !a.k_new) {
-        const size_t o = (size_t)g * a.head_stride + (size_t)pos * a.row_stride;
-        kp = (const T*)a.k + o;
-        vp = (const T*)a.v + o;
-    } else {
-        const size_t o = (size_t)g * a.new_head_stride + (size_t)(pos - k.npos0) * a.new_row_stride;
-        kp = (const T*)a.k_new + o;
-        vp = (const T*)a.v_new + o;
+struct KvRows {
+    uintptr_t k, v, kn, vn;
+    uint32_t rs, nrs;  // bytes between rows
+    int n0;
+    __device__ __forceinline__ KvRows(const cmf_attention_args& a, const Keys& ks, int g) {
+        n0 = ks.npos0;
+        rs = nrs = (uint32_t)a.row_stride * sizeof(T);
+        const uintptr_t o = (uintptr_t)g * a.head_stride * sizeof(T);
+        k = (uintptr_t)a.k + o;
+        v = (uintptr_t)a.v + o;
+        kn = k + (uintptr_t)n0 * rs;
+        vn = v + (uintptr_t)n0 * rs;
+        if (a.k_new) {
+            const uintptr_t p = (uintptr_t)g * a.new_head_stride * sizeof(T);
+            kn = (uintptr_t)a.k_new + p;
+            vn = (uintptr_t)a.v_new + p;
+            nrs = (uint32_t)a.new_row_stride * sizeof(T);
+        }
+        asm("" : "+s"(k), "+s"(v), "+s"(kn), "+s"(vn), "+s"(rs), "+s"(nrs));
     }
-}
+    // (device memory: the global address space lets the loads be global ones)
+    static __device__ __forceinline__ const T* ptr(uintptr_t u) {
+        return (const T*)(const __attribute__((address_space(1))) T*)u;
+    }
+    __device__ __forceinline__ uintptr_t offset(int pos) const {
+        const bool old = pos < n0;
+        return (uintptr_t)(uint32_t)(old ? pos : pos - n0) * (old ? rs : nrs);
+    }
+    __device__ __forceinline__ const T* key(int pos) const { return ptr((pos < n0 ? k : kn) + offset(pos)); }
+    __device__ __forceinline__ const T* value(int pos) const { return ptr((pos < n0 ? v : vn) + offset(pos)); }
+};
 
 // N elements as they lie in memory, and as f32
 template <class T, int N>
@@ -203,7 +239,7 @@ struct Part<_Float16> {
 template <>
 struct Part<bf16_t> {
     static constexpr int N = 3;
-    static constexpr float SHIFT = 0.f, LAZY = 12.f;
+    static constexpr float SHIFT = -12.f, LAZY = 12.f;  // weights of at most 1
     static constexpr bool SCALED = false;
     static constexpr uint32_t INF = 0x7f80;
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -221,7 +257,7 @@ struct Part<bf16_t> {
 template <>
 struct Part<float> {
     static constexpr int N = 1;
-    static constexpr float SHIFT = 0.f, LAZY = 12.f;
+    static constexpr float SHIFT = -12.f, LAZY = 12.f;  // weights of at most 1
     static constexpr bool SCALED = false;
 };
 // x as the parts p[0 .. N) of two values
@@ -267,6 +303,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + QN, nq) - 1);
     const Keys ks = keys_of(a, r0, r1);
 
+    const KvRows<T> kv(a, ks, g);
     // this split's keys, whole tiles
     const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + 15) / 16 * 16;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
@@ -278,40 +315,41 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     Raw<T, 8> kn[4];
     Raw<T, 16 / sizeof(T)> vn[4][VP];
     auto load = [&](int v0) {
-        const T *kp, *vp;
-        key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+        const T* kp = kv.key(ks.pos(min(v0 + n, ks.nv - 1)));
 #pragma unroll
         for (int j = 0; j < 4; j++) kn[j].load(kp, 32 * j + 8 * kq);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const T *kp2, *vp2;
-            key_row(a, ks, ks.pos(min(v0 + 4 * kq + e, ks.nv - 1)), g, kp2, vp2);
+            const T* vp = kv.value(ks.pos(min(v0 + 4 * kq + e, ks.nv - 1)));
 #pragma unroll
-            for (int u = 0; u < VP; u++) vn[e][u].load(vp2, 64 * u + (VP == 2 ? 4 : 8) * n);
+            for (int u = 0; u < VP; u++) vn[e][u].load(vp, 64 * u + (VP == 2 ? 4 : 8) * n);
         }
     };
-    if (v_lo + 16 * wave < v_hi) load(v_lo + 16 * wave);
-
-    // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n
+    // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n (read
+    // before the keys: loads are waited for in order)
     constexpr int QF = F32 ? 32 : 1, QP = F32 ? 1 : 4;
     float qf[QB][QF], cq[QB];  // cq: what the scores are multiplied by, positive
     uint4v qp[QB][QP][Part<T>::N];
     Sight see[QB];
+    Raw<float, 8> xq[QB][4];
+    SightIn in[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
         const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
-        see[qb] = sight_of(a, ks, r);
-        const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 8 * kq;
+        in[qb] = sight_in(a, r);
+        const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD;
+#pragma unroll
+        for (int j = 0; j < 4; j++) xq[qb][j].load(q, 32 * j + 8 * kq);
+    }
+    load(v_lo + 16 * wave);  // (there is a key at least; a wave without a tile reads it in vain)
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+        see[qb] = sight_of(a, ks, row_of(c, min(q0 + 16 * qb + n, nq - 1)), in[qb]);
         float x[32];
         float f = c.qscale < 0.f ? -1.f : 1.f;
         int eq = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float t[8];
-            load8(q + 32 * j, t);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[8 * j + i] = t[i];
-        }
+        for (int i = 0; i < 32; i++) x[i] = xq[qb][i >> 3].get(i & 7);
         if constexpr (Part<T>::SCALED) {
             float mx = 0.f;
 #pragma unroll
@@ -476,8 +514,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
         for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
             bool bad = false;
             {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + n, ks.nv - 1)), g, kp, vp);
+                const T* vp = kv.value(ks.pos(min(v0 + n, ks.nv - 1)));
 #pragma unroll 1
                 for (int u = 0; u < 32; u++) bad |= !(fabsf(to_f32(vp[32 * kq + u])) < INFINITY);
             }
@@ -485,8 +522,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 #pragma unroll 1
             for (int k = 0; k < 16; k++) {
                 const int v = v0 + k, pos = ks.pos(min(v, ks.nv - 1));
-                const T *kp, *vp;
-                key_row(a, ks, pos, g, kp, vp);
+                const T *kp = kv.key(pos), *vp = kv.value(pos);
 #pragma unroll
                 for (int qb = 0; qb < QB; qb++) {
                     const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
@@ -666,6 +702,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     const Keys ks = keys_of(a, r0, r1);
     const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + KT - 1) / KT * KT;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
+    const KvRows<T> kv(a, ks, g);
     const int qg = wave & 3, kb = wave >> 2;  // the wave's queries and 32-key block
 
     // what thread t stages of a tile: dims 8 kd .. of keys kk and kk + 32, and
@@ -688,9 +725,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         } else {
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + kk + 32 * r, ks.nv - 1)), g, kp, vp);
-                kx[r].load(kp, 8 * kd);
+                kx[r].load(kv.key(ks.pos(min(v0 + kk + 32 * r, ks.nv - 1))), 8 * kd);
             }
         }
     };
@@ -702,9 +737,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1)), g, kp, vp);
-                vx[i].load(vp, 2 * lane);
+                vx[i].load(kv.value(ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1))), 2 * lane);
             }
         }
     };
@@ -1006,8 +1039,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             float mv = 0.f;    // the largest of value row n of the block
 #pragma unroll 1
             for (int r = 0; r < 2; r++) {
-                const T *kp, *vp;
-                key_row(a, ks, ks.pos(min(v0 + 32 * r + n1, ks.nv - 1)), g, kp, vp);
+                const int pos = ks.pos(min(v0 + 32 * r + n1, ks.nv - 1));
+                const T *kp = kv.key(pos), *vp = kv.value(pos);
 #pragma unroll 1
                 for (int u = 0; u < HD; u++) {
                     bad |= !(fabsf(to_f32(kp[u])) < INFINITY);
@@ -1033,8 +1066,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             for (int kn = 0; kn < 32; kn++) {
                 const int v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));
                 const bool vis = sees(a, ks, see, pos) & (v < v_hi);
-                const T *kp, *vp;
-                key_row(a, ks, pos, g, kp, vp);
+                const T *kp = kv.key(pos), *vp = kv.value(pos);
                 float d = 0.f;
 #pragma unroll 4
                 for (int u = 0; u < 64; u++) d = fmaf(q[u], to_f32(kp[64 * h1 + u]), d);
