@@ -76,15 +76,18 @@ __device__ __forceinline__ int exponent_of(float x) {
 // 2^n for any n (what f32 cannot hold ends at its largest power)
 __device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, max(-300, min(n, 127))); }
 
-// A call as the kernels take it.
+// A call as the kernels take it.  An item is a block of queries of a kv head
+// (the blocks of a head in turn); items from `whole` on are split over their
+// keys, and their queries' partial results lie in the items' order.
 struct AttnCall {
     cmf_attention_args a;
     int hpk;         // query heads per kv head
     uint32_t inv;    // ceil(2^32 / hpk): query / hpk = high word of query * inv
-    int nsplit;      // key splits per query block; 1: the output itself
+    int groups, per;  // items of a kv head, queries of an item
+    int whole, nsplit;
     float qscale;    // scale * log2(e)
-    float *pm, *pl;  // [b * nh][nsplit] partial maxima (log2 units) and sums
-    float* po;       // [b * nh][nsplit][128], relative to the maximum
+    float *pm, *pl;  // [split items' queries][nsplit] partial maxima (log2 units) and sums
+    float* po;       // [split items' queries][nsplit][128], relative to the maximum
 };
 
 // row of query qi (exact: queries and hpk multiply to less than 2^32)
@@ -573,11 +576,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             const float inv = L == 0.f ? 0.f : 1.0f / L;
             *(float4v*)(a.out + (size_t)r * a.ldo + (size_t)h * HD + d) = o * inv;
         } else {
-            const size_t rh = (size_t)r * a.nh + h;
-            *(float4v*)(c.po + (rh * c.nsplit + split) * HD + d) = o;
+            const size_t at = ((size_t)(g * c.groups + blockIdx.z) * QN + qq) * c.nsplit + split;
+            *(float4v*)(c.po + at * HD + d) = o;
             if (d == 0) {
-                c.pm[rh * c.nsplit + split] = M;
-                c.pl[rh * c.nsplit + split] = L;
+                c.pm[at] = M;
+                c.pl[at] = L;
             }
         }
     }
@@ -614,8 +617,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // (only block 1's waves stage and read its values, a tile later).
 //
 // Bound by the MFMAs: 1536 cycles per tile and wave at f32.
-// grid nsplit ceil(b hpk / 128) nkv, block 512, LDS Tile<T>::LDS: the items
-// (split fastest, then query block, then kv head) in eight runs, one to an
+// grid whole + nsplit (items - whole), block 512, LDS Tile<T>::LDS: the items
+// (those in one piece, then the splits of the others) in eight runs, one to an
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
 // same keys.
 // ---------------------------------------------------------------------------
@@ -695,12 +698,14 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     int* texp = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: 4 of K, 2 of V
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 31, h = lane >> 5, nq = a.b * c.hpk;
-    const uint32_t item = xcd_run(blockIdx.x, gridDim.x), groups = (nq + TQ - 1) / TQ;
-    const int split = item % c.nsplit, g = item / c.nsplit / groups;
-    const int q0 = (item / c.nsplit - g * groups) * TQ;
+    const bool part = (int)blockIdx.x >= c.whole;
+    const int nsplit = part ? c.nsplit : 1;
+    const uint32_t id = part ? xcd_run(blockIdx.x - c.whole, gridDim.x - c.whole) : xcd_run(blockIdx.x, c.whole);
+    const int own = id / (uint32_t)nsplit, split = id - own * nsplit, item = part ? c.whole + own : own;
+    const int g = (uint32_t)item / (uint32_t)c.groups, q0 = (item - g * c.groups) * TQ;
     const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + TQ, nq) - 1);
     const Keys ks = keys_of(a, r0, r1);
-    const int per = ((ks.nv + c.nsplit - 1) / c.nsplit + KT - 1) / KT * KT;
+    const int per = ((ks.nv + nsplit - 1) / nsplit + KT - 1) / KT * KT;
     const int v_lo = min(split * per, ks.nv), v_hi = min(v_lo + per, ks.nv);
     const KvRows<T> kv(a, ks, g);
     const int qg = wave & 3, kb = wave >> 2;  // the wave's queries and 32-key block
@@ -1093,11 +1098,11 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         const float2 e1 = e[0], e2 = e[TQ];
         const float mx = fmaxf(e1.x, e2.x);
         const float f1 = e1.x == -INFINITY ? 0.f : exp2f(e1.x - mx), f2 = e2.x == -INFINITY ? 0.f : exp2f(e2.x - mx);
-        const float lt = e1.y * f1 + e2.y * f2, f = c.nsplit > 1 ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
+        const float lt = e1.y * f1 + e2.y * f2, f = part ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
         const float4v y = (*(const float4v*)x * f1 + *(const float4v*)(x + TQ * OROW) * f2) * f;
         const int row = row_of(c, qi), head = g * c.hpk + qi - row * c.hpk;
-        if (c.nsplit > 1) {
-            const size_t at = ((size_t)row * a.nh + head) * c.nsplit + split;
+        if (part) {
+            const size_t at = ((size_t)own * TQ + k) * nsplit + split;
             *(float4v*)(c.po + at * HD + 4 * (t1 & 31)) = y;
             if ((t1 & 31) == 0) {
                 c.pm[at] = mx;
@@ -1109,18 +1114,20 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     }
 }
 
-// The splits of one (row, head) by one wave: out = sum w_c o_c / sum w_c l_c,
+// The splits of one query by one wave: out = sum w_c o_c / sum w_c l_c,
 // w_c = 2^(m_c - M); lane = dim pair.  The maxima, the sums and CB splits'
 // outputs are requested together, so that up to CB splits take one memory
-// round trip.  Bound by latency.  grid (b nh), block 64.
+// round trip.  Bound by latency.  grid (per, split items), block 64.
 template <int CB>
 __global__ __launch_bounds__(64) void k_attn_join(AttnCall c) {
     const cmf_attention_args& a = c.a;
-    const int lane = threadIdx.x, ns = c.nsplit;
-    const size_t rh = blockIdx.x;
-    const float* pm = c.pm + rh * ns;
-    const float* pl = c.pl + rh * ns;
-    const float2* po = (const float2*)(c.po + rh * ns * HD) + lane;
+    const int lane = threadIdx.x, ns = c.nsplit, item = c.whole + blockIdx.y;
+    const int g = (uint32_t)item / (uint32_t)c.groups, qi = (item - g * c.groups) * c.per + blockIdx.x;
+    if (qi >= a.b * c.hpk) return;
+    const size_t at = (size_t)blockIdx.y * c.per + blockIdx.x;
+    const float* pm = c.pm + at * ns;
+    const float* pl = c.pl + at * ns;
+    const float2* po = (const float2*)(c.po + at * ns * HD) + lane;
     float M = -INFINITY, L = 0.f;
     float2 o = make_float2(0.f, 0.f);
     for (int j0 = 0; j0 < ns; j0 += CB) {
@@ -1144,8 +1151,8 @@ __global__ __launch_bounds__(64) void k_attn_join(AttnCall c) {
         }
     }
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    const size_t r = rh / a.nh, h = rh - r * a.nh;
-    ((float2*)(a.out + r * a.ldo + h * HD))[lane] = make_float2(o.x * inv, o.y * inv);
+    const int r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
+    ((float2*)(a.out + (size_t)r * a.ldo + (size_t)h * HD))[lane] = make_float2(o.x * inv, o.y * inv);
 }
 
 // the most keys that a block of rows may have to read
@@ -1160,8 +1167,9 @@ long long keys_bound(const cmf_attention_args& a, int rows) {
 struct Plan {
     bool tiles = false;  // k_attn_tiles, else k_attn_rows
     int nb = 1;          // k_attn_rows: 16-query columns of a wave
-    int groups = 1, nsplit = 1;
+    int groups = 1, per = 1, items = 1, whole = 1, nsplit = 1;  // as AttnCall's
     size_t bytes = 0;
+    size_t partial() const { return (size_t)(items - whole) * per * nsplit; }
 };
 
 Plan plan_of(const cmf_attention_args& a) {
@@ -1170,17 +1178,24 @@ Plan plan_of(const cmf_attention_args& a) {
     const long long nq = (long long)a.b * hpk;
     p.tiles = nq > 32;
     p.nb = nq <= 16 ? 1 : 2;
-    const int per_wg = p.tiles ? TQ : 16 * p.nb;
-    p.groups = (int)((nq + per_wg - 1) / per_wg);
-    const int rows = (int)std::min<long long>(a.b, per_wg / hpk + 2);
-    const long long nv = keys_bound(a, rows);
-    // one workgroup a CU of the tiles, two of the rows; a split of at least 64 keys
-    long long ns = (p.tiles ? 256 : 512) / std::max(1ll, (long long)a.nkv * p.groups);
-    ns = std::max(1ll, std::min(ns, (nv + 63) / 64));
-    const size_t per = (size_t)a.b * a.nh * (HD + 2) * sizeof(float);
-    while (ns > 1 && per * ns > OP_WS_MAX) ns--;
+    p.per = p.tiles ? TQ : 16 * p.nb;
+    p.groups = (int)((nq + p.per - 1) / p.per);
+    p.items = p.groups * a.nkv;
+    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, p.per / hpk + 2));
+    // One workgroup a CU of the tiles, two of the rows.  The items that fill
+    // the card's CUs whole times stay in one piece, the rest is split to fill
+    // them once more, a split of at least 64 keys (256 behind whole items,
+    // which would wait for the join alone).
+    const int room = p.tiles ? 256 : 512;
+    p.whole = p.items / room * room;
+    const int rest = p.items - p.whole;
+    const long long least = p.whole ? 256 : 64;
+    long long ns = rest ? std::max(1ll, std::min<long long>(room / rest, (nv + least - 1) / least)) : 1;
+    const size_t one = (size_t)rest * p.per * (HD + 2) * sizeof(float);
+    while (ns > 1 && one * ns > OP_WS_MAX) ns--;
     p.nsplit = (int)ns;
-    p.bytes = ns > 1 ? per * ns : 0;
+    if (ns == 1) p.whole = p.items;
+    p.bytes = ns > 1 ? one * ns : 0;
     return p;
 }
 
@@ -1208,7 +1223,7 @@ int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
     if (allow_lds(f, Tile<T>::LDS) != CMF_OK) return CMF_ERR;
     AttnCall arg = c;
     void* args[] = {&arg};
-    CMF_HIP(hipLaunchKernel(f, dim3((unsigned)c.nsplit * p.groups * c.a.nkv), dim3(512), args, Tile<T>::LDS, s));
+    CMF_HIP(hipLaunchKernel(f, dim3((unsigned)(p.whole + p.nsplit * (p.items - p.whole))), dim3(512), args, Tile<T>::LDS, s));
     return CMF_OK;
 }
 
@@ -1220,18 +1235,25 @@ int launch_cache_attention(const cmf_attention_args& a, hipStream_t s) {
     const Plan p = plan_of(a);
     if (p.bytes > a.ws_bytes || (p.bytes && !a.ws)) return fail("attention: the workspace is too small (cmf_attention_workspace)");
     const uint32_t hpk = a.nh / a.nkv;
-    AttnCall c{a, (int)hpk, (uint32_t)(((1ull << 32) + hpk - 1) / hpk), p.nsplit, (a.scale == 0.f ? 0.08838834764831845f : a.scale) * LOG2E, nullptr, nullptr, nullptr};
+    AttnCall c{};
+    c.a = a;
+    c.hpk = (int)hpk;
+    c.inv = (uint32_t)(((1ull << 32) + hpk - 1) / hpk);
+    c.groups = p.groups;
+    c.per = p.per;
+    c.whole = p.whole;
+    c.nsplit = p.nsplit;
+    c.qscale = (a.scale == 0.f ? 0.08838834764831845f : a.scale) * LOG2E;
     if (p.nsplit > 1) {
-        const size_t rh = (size_t)a.b * a.nh * p.nsplit;
         c.po = (float*)a.ws;
-        c.pm = c.po + rh * HD;
-        c.pl = c.pm + rh;
+        c.pm = c.po + p.partial() * HD;
+        c.pl = c.pm + p.partial();
     }
     const int rc = a.kv_dtype == CMF_DT_F32   ? launch_t<float>(c, p, s)
                    : a.kv_dtype == CMF_DT_F16 ? launch_t<_Float16>(c, p, s)
                                               : launch_t<bf16_t>(c, p, s);
     if (rc != CMF_OK) return rc;
-    const dim3 rows((unsigned)(a.b * a.nh));
+    const dim3 rows(p.per, p.items - p.whole);
     if (p.nsplit > 16) hipLaunchKernelGGL(k_attn_join<32>, rows, dim3(64), 0, s, c);
     else if (p.nsplit > 1) hipLaunchKernelGGL(k_attn_join<16>, rows, dim3(64), 0, s, c);
     return CMF_OK;

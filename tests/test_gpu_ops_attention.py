@@ -329,3 +329,30 @@ def test_a_scratch_too_small_is_refused(ops):
     assert (out.numpy() == 2.0).all()
     ops.attention(q, k, v, out, T.empty(need, "uint8"), pos0=5000)
     assert not (out.numpy() == 2.0).any()
+
+
+@pytest.mark.parametrize("b,ctx,window,sinks,nh,nkv,dtype", [
+    (1030, 500, 0, 0, 32, 16, "float32"), (2060, 40, 600, 4, 16, 16, "float16"), (2060, 900, 0, 0, 16, 16, "bfloat16")])
+def test_blocks_that_do_not_fill_the_card(ops, ws, b, ctx, window, sinks, nh, nkv, dtype):
+    """272 blocks of 128 queries: 256 in one piece, the rest split over their keys."""
+    T = ops.DevTensor
+    r = np.random.default_rng(b + ctx)
+    q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=b)
+    out = filled(ops, q.shape)
+    dq, dk, dv = T.of(q), T.of(k, dtype), T.of(v, dtype)
+    assert ops.attention_workspace(dq, dk, dv, pos0=ctx, window=window, sinks=sinks) > 0
+    ops.attention(dq, dk, dv, out, ws, pos0=ctx, window=window, sinks=sinks)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, window, sinks)))
+
+
+@pytest.mark.parametrize("b", [1, 9, 80])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_values_of_1e36(ops, ws, b, dtype):
+    """weights are summed without leaving f32's range"""
+    T = ops.DevTensor
+    r = np.random.default_rng(b)
+    q, k, v = tensors(r, b, 700, 4, 2, dtype, extra=b, std=4.0)
+    v = rounded(v * np.float32(1e36), dtype)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=700)
+    check(out.numpy(), *reference(q, k, v, visible(b, 700, 0, 0)))
