@@ -148,7 +148,7 @@ __device__ __forceinline__ Sight sight_of(const cmf_attention_args& a, const Key
     return Sight{k.tree ? -1 : row, a.window ? P - a.window : -1, k.tree ? 0 : 0x7fffffff, k.tree ? in.mask : 0};
 }
 __device__ __forceinline__ Sight sight_of(const cmf_attention_args& a, const Keys& k, int row) {
-    return sight_of(a, k, row, sight_in(a, row));
+    return sight_of(a, k, row, a.d_mask ? sight_in(a, row) : SightIn{});  // (a depth goes with a mask)
 }
 __device__ __forceinline__ bool sees(const cmf_attention_args& a, const Keys& k, const Sight& s, int pos) {
     const int j = pos - k.npos0;
@@ -716,34 +716,33 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     const int kd = t & 15, kk = t >> 4, vk = 32 * (wave >> 2) + 16 * (wave >> 1 & 1) + 4 * (wave & 1);
     Raw<T, 8> kx[2];
     Raw<T, 2> vx[8];
-    auto one_run = [&](int v0) {  // of the cache
-        return v0 >= ks.s && v0 + KT <= ks.nv && (ks.pos(v0) + KT <= ks.npos0 || !a.k_new);
-    };
+    // A tile that is one run of the cache needs one address, and a sum a row.
+    auto one_run = [&](int v0) { return v0 >= ks.s && v0 + KT <= ks.nv && (ks.pos(v0) + KT <= ks.npos0 || !a.k_new); };
     auto load_k = [&](int v0) {
         if (one_run(v0)) {
-            const T* kp = (const T*)a.k + (size_t)g * a.head_stride + (size_t)ks.pos(v0) * a.row_stride;
-            uint32_t rs = (uint32_t)a.row_stride;
+            uint32_t rs = kv.rs;
             asm("" : "+s"(rs));  // (the offset is not kept over the loop)
-            const uint32_t ko = kk * rs + 8 * kd;
+            const uintptr_t k = kv.k + (uintptr_t)(uint32_t)ks.pos(v0) * rs;
+            const uint32_t ko = kk * (rs / sizeof(T)) + 8 * kd;
 #pragma unroll
-            for (int r = 0; r < 2; r++) kx[r].load(kp + (size_t)(32 * r) * a.row_stride, ko);
+            for (int r = 0; r < 2; r++) kx[r].load(kv.ptr(k + 32 * r * rs), ko);
         } else {
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                kx[r].load(kv.key(ks.pos(min(v0 + kk + 32 * r, ks.nv - 1))), 8 * kd);
-            }
+            for (int r = 0; r < 2; r++) kx[r].load(kv.key(ks.pos(min(v0 + kk + 32 * r, ks.nv - 1))), 8 * kd);
         }
     };
     auto load_v = [&](int v0) {
         if (one_run(v0)) {
-            const T* vp = (const T*)a.v + (size_t)g * a.head_stride + (size_t)(ks.pos(v0) + vk) * a.row_stride;
-#pragma unroll
-            for (int i = 0; i < 8; i++) vx[i].load(vp + (size_t)(8 * (i >> 2) + (i & 3)) * a.row_stride, 2 * lane);
-        } else {
+            uintptr_t v = kv.v + (uintptr_t)(uint32_t)(ks.pos(v0) + vk) * kv.rs;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                vx[i].load(kv.value(ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1))), 2 * lane);
+                vx[i].load(kv.ptr(v), 2 * lane);
+                v += i == 3 ? 5 * kv.rs : kv.rs;
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                vx[i].load(kv.value(ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1))), 2 * lane);
         }
     };
     if (v_lo < v_hi) {  // under way while the queries are split
