@@ -1181,11 +1181,13 @@ Plan plan_of(const cmf_attention_args& a) {
     p.groups = (int)((nq + p.per - 1) / p.per);
     p.items = p.groups * a.nkv;
     const long long nv = keys_bound(a, (int)std::min<long long>(a.b, p.per / hpk + 2));
-    // One workgroup a CU of the tiles, two of the rows.  The items that fill
+    // One workgroup a CU of the tiles, two of the rows where one would have more
+    // than two tiles for each of its waves (9 rows of 16 heads: at 2048 keys 15.5
+    // us with one, 17.0 with two; at 12000 36.9 and 31.6).  The items that fill
     // the card's CUs whole times stay in one piece, the rest is split to fill
     // them once more, a split of at least 64 keys (256 behind whole items,
     // which would wait for the join alone).
-    const int room = p.tiles ? 256 : 512;
+    const int room = p.tiles || nv * p.items <= 256 * 128 ? 256 : 512;
     p.whole = p.items / room * room;
     const int rest = p.items - p.whole;
     const long long least = p.whole ? 256 : 64;

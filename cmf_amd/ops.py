@@ -15,6 +15,7 @@ stream.cuda_stream; 0 is the null stream).  Raises CmfError when the library
 refuses the arguments.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -117,11 +118,41 @@ def _dt(t):
 
 
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _stream(s):
-    return None if s is None else (s or STREAM_NULL)
+    return 0 if s is None else (s or STREAM_NULL)
+
+
+class _Call:
+    """A library function of one argument struct, called with the struct's
+    fields: packed in one go, which a ctypes struct takes 1 us longer for."""
+    CODES = {C.c_void_p: "P", C.c_size_t: "N", C.c_longlong: "q", C.c_int: "i", C.c_double: "d", C.c_float: "f"}
+
+    def __init__(self, name, args, result=C.c_int):
+        self.name, self.result, self.fn = name, result, None
+        layout = struct.Struct("".join(self.CODES[t] for _, t in args._fields_))
+        assert layout.size == C.sizeof(args), name
+        self.pack = layout.pack
+
+    def __call__(self, fields):
+        if self.fn is None:
+            at = C.cast(getattr(lib(), self.name), C.c_void_p).value
+            self.fn = C.CFUNCTYPE(self.result, C.c_char_p)(at)
+        try:
+            a = self.pack(*fields)
+        except (struct.error, OverflowError) as e:
+            raise CmfError(f"{self.name}: {e}") from None
+        return self.fn(a)
+
+
+_qk_rope = _Call("cmf_qk_rope_dev", QkRopeArgs)
+_attention = _Call("cmf_attention_dev", AttentionArgs)
+_attention_ws = _Call("cmf_attention_workspace", AttentionArgs, C.c_size_t)
+_kv_copy = _Call("cmf_kv_copy_dev", KvCopyArgs)
+_logprobs = _Call("cmf_logprobs_dev", LogprobsArgs)
+_logprobs_ws = _Call("cmf_logprobs_workspace", LogprobsArgs, C.c_size_t)
 
 
 def _want(ok, what):
@@ -177,9 +208,8 @@ def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=
     _want(tuple(rope.shape[1:]) == (64, 2) and tuple(rope.stride()) == (128, 2, 1), "rope must be [positions][64][2], contiguous")
     _i32(depth, b, "depth")
     _i32(pos0_dev, 1, "pos0_dev")
-    a = QkRopeArgs(_p(qkv), _p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(rope), _p(pos0_dev), _p(depth), eps, hst, rst,
-                   b, nh, nkv, ldq, ldo, _dt(k), rope.shape[0], pos0, slots, 1 if at_pos else 0, _stream(stream))
-    check(lib().cmf_qk_rope_dev(C.byref(a)))
+    check(_qk_rope((_p(qkv), _p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(rope), _p(pos0_dev), _p(depth), eps, hst, rst,
+                    b, nh, nkv, ldq, ldo, _dt(k), rope.shape[0], pos0, slots, 1 if at_pos else 0, _stream(stream))))
 
 
 def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream):
@@ -202,17 +232,16 @@ def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, s
     _i32(depth, b, "depth")
     _i32(pos0_dev, 1, "pos0_dev")
     nb = 0 if ws is None else ws.shape[0] * ws.element_size()
-    return AttentionArgs(_p(q), _p(out), _p(k), _p(v), _p(k_new), _p(v_new), _p(mask), _p(pos0_dev), _p(depth), _p(ws), nb,
-                         hst, rst, nhst, nrst, b, nh, nkv, ldq, ldo, _dt(k), pos0, slots, len_bound, window, sinks, scale,
-                         _stream(stream))
+    return (_p(q), _p(out), _p(k), _p(v), _p(k_new), _p(v_new), _p(mask), _p(pos0_dev), _p(depth), _p(ws), nb, hst, rst, nhst,
+            nrst, b, nh, nkv, ldq, ldo, _dt(k), pos0, slots, len_bound, window, sinks, scale, _stream(stream))
 
 
 def attention_workspace(q, k, v, *, pos0=0, k_new=None, v_new=None, mask=None, depth=None, window=0, sinks=0,
                         pos0_dev=None, len_bound=0):
     """cmf_attention_workspace: bytes of scratch the call of these arguments
     needs (never more than WORKSPACE_MAX)."""
-    a = _attention_args(q, k, v, None, None, pos0, k_new, v_new, mask, depth, window, sinks, 0.0, pos0_dev, len_bound, None)
-    return lib().cmf_attention_workspace(C.byref(a))
+    return _attention_ws(_attention_args(q, k, v, None, None, pos0, k_new, v_new, mask, depth, window, sinks, 0.0, pos0_dev,
+                                         len_bound, None))
 
 
 def attention(q, k, v, out, ws, *, pos0=0, k_new=None, v_new=None, mask=None, depth=None, window=0, sinks=0, scale=0.0,
@@ -224,8 +253,8 @@ def attention(q, k, v, out, ws, *, pos0=0, k_new=None, v_new=None, mask=None, de
     it row i sees the rows up to its own.  window, sinks: only the last window
     positions and the first sinks are seen (window 0: all).  ws: 1-d scratch
     tensor of attention_workspace bytes (None: nothing)."""
-    a = _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream)
-    check(lib().cmf_attention_dev(C.byref(a)))
+    check(_attention(_attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev,
+                                     len_bound, stream)))
 
 
 def tree_masks(parents, pos0=0, window=0, sinks=0):
@@ -251,9 +280,8 @@ def kv_copy(dst_ptrs, src_ptrs, dst, src, *, n, pos0=0, idx=None, n_dev=None, po
     _i32(idx, n, "idx")
     _i32(n_dev, 1, "n_dev")
     _i32(pos0_dev, 1, "pos0_dev")
-    a = KvCopyArgs(_p(dst_ptrs), _p(src_ptrs), _p(idx), _p(n_dev), _p(pos0_dev), dh, dr, sh, sr, dst_ptrs.shape[0], nkv,
-                   _dt(dst), n, pos0, ds, ss, _stream(stream))
-    check(lib().cmf_kv_copy_dev(C.byref(a)))
+    check(_kv_copy((_p(dst_ptrs), _p(src_ptrs), _p(idx), _p(n_dev), _p(pos0_dev), dh, dr, sh, sr, dst_ptrs.shape[0], nkv,
+                    _dt(dst), n, pos0, ds, ss, _stream(stream))))
 
 
 def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws, stream):
@@ -273,15 +301,13 @@ def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws,
     if top_lp is not None:
         _f32(top_lp, "top_lp")
     nb = 0 if ws is None else ws.shape[0] * ws.element_size()
-    return LogprobsArgs(_p(logits), _p(target), _p(logprob), _p(entropy), _p(top_ids), _p(top_lp), _p(ws), nb,
-                        logits.stride()[0] if rows > 1 else max(logits.stride()[0], V), rows, V, _dt(logits), top_k,
-                        _stream(stream))
+    return (_p(logits), _p(target), _p(logprob), _p(entropy), _p(top_ids), _p(top_lp), _p(ws), nb,
+            logits.stride()[0] if rows > 1 else max(logits.stride()[0], V), rows, V, _dt(logits), top_k, _stream(stream))
 
 
 def logprobs_workspace(logits, top_k=0):
     """cmf_logprobs_workspace: bytes of scratch for these logits."""
-    a = _logprobs_args(logits, None, None, None, None, None, top_k, None, None)
-    return lib().cmf_logprobs_workspace(C.byref(a))
+    return _logprobs_ws(_logprobs_args(logits, None, None, None, None, None, top_k, None, None))
 
 
 def logprobs(logits, target=None, logprob=None, entropy=None, top_ids=None, top_lp=None, ws=None, *, stream=None):
@@ -290,5 +316,5 @@ def logprobs(logits, target=None, logprob=None, entropy=None, top_ids=None, top_
     k most likely tokens (equal logits: the lowest id first).  Any output may be
     None.  ws: 1-d scratch tensor of logprobs_workspace bytes."""
     top = top_ids if top_ids is not None else top_lp
-    a = _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, 0 if top is None else top.shape[1], ws, stream)
-    check(lib().cmf_logprobs_dev(C.byref(a)))
+    check(_logprobs(_logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, 0 if top is None else top.shape[1], ws,
+                                   stream)))
