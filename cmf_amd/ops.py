@@ -155,18 +155,13 @@ _logprobs = _Call("cmf_logprobs_dev", LogprobsArgs)
 _logprobs_ws = _Call("cmf_logprobs_workspace", LogprobsArgs, C.c_size_t)
 
 
-def _want(ok, what):
-    if not ok:
-        raise CmfError(what)
-
-
 def _f32(t, what):
     if _name(t) != "float32":
         raise CmfError(f"{what} must be f32")
 
 
 def _i32(t, n, what):
-    if t is not None and not (_name(t) == "int32" and t.stride()[-1] == 1 and t.shape[0] >= n):
+    if not (_name(t) == "int32" and t.stride()[-1] == 1 and t.shape[0] >= n):
         raise CmfError(f"{what} must be int32, contiguous, of at least {n}")
 
 
@@ -198,39 +193,47 @@ def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=
     b, hs, ldq = _rows(qkv, "qkv")
     nkv, slots, hst, rst = _cache(k, v, "k / v")
     bq, nh, ldo = _rows(q, "q")
-    _want(bq == b and hs == nh + 2 * nkv, "qkv must hold nh + 2 nkv heads of every row of q")
-    for t, w in ((qkv, "qkv"), (q, "q"), (rope, "rope")):
-        _f32(t, w)
+    if not (bq == b and hs == nh + 2 * nkv):
+        raise CmfError("qkv must hold nh + 2 nkv heads of every row of q")
+    f32 = qkv.dtype
+    if _name(qkv) != "float32" or q.dtype != f32 or rope.dtype != f32:
+        raise CmfError("qkv, q and rope must be f32")
     for t in (q_norm, k_norm):
-        if t is not None:
-            _f32(t, "the norms")
-            _want(tuple(t.shape) == (128,) and t.stride()[0] == 1, "the norms must be [128]")
-    _want(tuple(rope.shape[1:]) == (64, 2) and tuple(rope.stride()) == (128, 2, 1), "rope must be [positions][64][2], contiguous")
-    _i32(depth, b, "depth")
-    _i32(pos0_dev, 1, "pos0_dev")
+        if t is not None and not (t.dtype == f32 and t.shape == (128,) and t.stride()[0] == 1):
+            raise CmfError("the norms must be f32, [128]")
+    positions, *pairs = rope.shape
+    if pairs != [64, 2] or rope.stride() != (128, 2, 1):
+        raise CmfError("rope must be [positions][64][2], contiguous")
+    if depth is not None:
+        _i32(depth, b, "depth")
+    if pos0_dev is not None:
+        _i32(pos0_dev, 1, "pos0_dev")
     check(_qk_rope((_p(qkv), _p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(rope), _p(pos0_dev), _p(depth), eps, hst, rst,
-                    b, nh, nkv, ldq, ldo, _dt(k), rope.shape[0], pos0, slots, 1 if at_pos else 0, _stream(stream))))
+                    b, nh, nkv, ldq, ldo, _dt(k), positions, pos0, slots, 1 if at_pos else 0, _stream(stream))))
 
 
 def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream):
     b, nh, ldq = _rows(q, "q")
     nkv, slots, hst, rst = _cache(k, v, "k / v")
-    _want(nkv >= 1 and nh % nkv == 0, "the query heads must be a multiple of the kv heads")
+    if nkv < 1 or nh % nkv:
+        raise CmfError("the query heads must be a multiple of the kv heads")
     _f32(q, "q")
     ldo = nh * 128
     if out is not None:
-        _f32(out, "out")
         bo, ho, ldo = _rows(out, "out")
-        _want((bo, ho) == (b, nh), "out must be shaped as q")
+        if bo != b or ho != nh or out.dtype != q.dtype:
+            raise CmfError("out must be shaped as q, f32")
     nhst = nrst = 0
     if k_new is not None:
         nk, rows, nhst, nrst = _cache(k_new, v_new, "k_new / v_new")
-        _want(nk == nkv and rows >= b and k_new.dtype == k.dtype, "k_new / v_new must hold b rows of k's type")
-    if mask is not None:
-        _want(_name(mask) in ("int64", "uint64") and mask.shape[0] >= b and
-              mask.stride()[0] == 1, "mask must be [b] of 64 bits")
-    _i32(depth, b, "depth")
-    _i32(pos0_dev, 1, "pos0_dev")
+        if nk != nkv or rows < b or k_new.dtype != k.dtype:
+            raise CmfError("k_new / v_new must hold b rows of k's type")
+    if mask is not None and not (_name(mask) in ("int64", "uint64") and mask.shape[0] >= b and mask.stride()[0] == 1):
+        raise CmfError("mask must be [b] of 64 bits")
+    if depth is not None:
+        _i32(depth, b, "depth")
+    if pos0_dev is not None:
+        _i32(pos0_dev, 1, "pos0_dev")
     nb = 0 if ws is None else ws.shape[0] * ws.element_size()
     return (_p(q), _p(out), _p(k), _p(v), _p(k_new), _p(v_new), _p(mask), _p(pos0_dev), _p(depth), _p(ws), nb, hst, rst, nhst,
             nrst, b, nh, nkv, ldq, ldo, _dt(k), pos0, slots, len_bound, window, sinks, scale, _stream(stream))
@@ -273,36 +276,40 @@ def kv_copy(dst_ptrs, src_ptrs, dst, src, *, n, pos0=0, idx=None, n_dev=None, po
     of the buffers of each side, [nkv][slots][128], for the layout."""
     nkv, ds, dh, dr = _cache(dst, dst, "dst")
     nk, ss, sh, sr = _cache(src, src, "src")
-    _want(nk == nkv and src.dtype == dst.dtype, "dst and src must have the same heads and type")
-    for t in (dst_ptrs, src_ptrs):
-        _want(_name(t) == "int64" and t.stride()[0] == 1, "pointers must be int64, contiguous")
-    _want(dst_ptrs.shape[0] == src_ptrs.shape[0], "as many buffers on both sides")
-    _i32(idx, n, "idx")
-    _i32(n_dev, 1, "n_dev")
-    _i32(pos0_dev, 1, "pos0_dev")
-    check(_kv_copy((_p(dst_ptrs), _p(src_ptrs), _p(idx), _p(n_dev), _p(pos0_dev), dh, dr, sh, sr, dst_ptrs.shape[0], nkv,
+    if nk != nkv or src.dtype != dst.dtype:
+        raise CmfError("dst and src must have the same heads and type")
+    if _name(dst_ptrs) != "int64" or src_ptrs.dtype != dst_ptrs.dtype or dst_ptrs.stride() != (1,) or src_ptrs.stride() != (1,):
+        raise CmfError("pointers must be int64, [buffers], contiguous")
+    nbuf = dst_ptrs.shape[0]
+    if src_ptrs.shape[0] != nbuf:
+        raise CmfError("as many buffers on both sides")
+    if idx is not None:
+        _i32(idx, n, "idx")
+    if n_dev is not None:
+        _i32(n_dev, 1, "n_dev")
+    if pos0_dev is not None:
+        _i32(pos0_dev, 1, "pos0_dev")
+    check(_kv_copy((_p(dst_ptrs), _p(src_ptrs), _p(idx), _p(n_dev), _p(pos0_dev), dh, dr, sh, sr, nbuf, nkv,
                     _dt(dst), n, pos0, ds, ss, _stream(stream))))
 
 
 def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws, stream):
-    _want(len(logits.shape) == 2 and logits.stride()[1] == 1, "logits must be [rows][V]")
-    rows, V = logits.shape
-    _i32(target, rows, "target")
+    shape, st = logits.shape, logits.stride()
+    if len(shape) != 2 or st[1] != 1:
+        raise CmfError("logits must be [rows][V]")
+    rows, V = shape
+    if target is not None:
+        _i32(target, rows, "target")
     for t, w in ((logprob, "logprob"), (entropy, "entropy")):
-        if t is not None:
-            _f32(t, w)
-            _want(t.shape[0] >= rows and t.stride()[0] == 1, f"{w} must be [rows]")
-    for t, w in ((top_ids, "top_ids"), (top_lp, "top_lp")):
-        if t is not None:
-            _want(len(t.shape) == 2 and t.shape[0] >= rows and t.shape[1] == top_k and tuple(t.stride()) == (top_k, 1),
-                  f"{w} must be [rows][top_k], contiguous")
-    if top_ids is not None:
-        _want(_name(top_ids) == "int32", "top_ids must be int32")
-    if top_lp is not None:
-        _f32(top_lp, "top_lp")
+        if t is not None and not (_name(t) == "float32" and t.shape[0] >= rows and t.stride()[0] == 1):
+            raise CmfError(f"{w} must be f32, [rows]")
+    for t, w, d in ((top_ids, "top_ids", "int32"), (top_lp, "top_lp", "float32")):
+        if t is not None and not (_name(t) == d and len(t.shape) == 2 and t.shape[0] >= rows and t.shape[1] == top_k and
+                                  t.stride() == (top_k, 1)):
+            raise CmfError(f"{w} must be {d}, [rows][top_k], contiguous")
     nb = 0 if ws is None else ws.shape[0] * ws.element_size()
     return (_p(logits), _p(target), _p(logprob), _p(entropy), _p(top_ids), _p(top_lp), _p(ws), nb,
-            logits.stride()[0] if rows > 1 else max(logits.stride()[0], V), rows, V, _dt(logits), top_k, _stream(stream))
+            st[0] if rows > 1 else max(st[0], V), rows, V, _dt(logits), top_k, _stream(stream))
 
 
 def logprobs_workspace(logits, top_k=0):
