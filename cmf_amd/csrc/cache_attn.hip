@@ -292,7 +292,7 @@ __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::
 //
 // Bound by the cache's bytes: 16 KiB of f32 K/V per tile against 64 MFMAs of
 // 32 cycles per 16 queries, 8 KiB of f16 against 24 of 16.
-// grid (nsplit, nkv, ceil(b hpk / 16 QB) <= 2), block 256.
+// grid (nsplit, nkv, ceil(b hpk / 16 QB)), block 256.
 // ---------------------------------------------------------------------------
 template <class T, int QB>
 __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
@@ -650,10 +650,12 @@ __device__ __forceinline__ int exponent_class(uint32_t u) {  // of a magnitude's
     return u >= 0x7f800000u ? BAD_EXP : u == 0 ? NO_EXP : e >= -2 && e < 6 ? PLAIN : e;
 }
 __device__ __forceinline__ int group_exponent(float mx) {
+    // (the ordinary case by two comparisons)
+    if (!__builtin_amdgcn_ballot_w64(!(mx < 64.f)) && __builtin_amdgcn_ballot_w64(mx >= 0.25f)) return PLAIN;
     return exponent_class(__builtin_amdgcn_readfirstlane(wave_max_u32(__float_as_uint(mx))));
 }
 __device__ __forceinline__ bool scaled(int e) { return e != PLAIN && e != NO_EXP; }
-__device__ __forceinline__ float group_scale(int e) { return scaled(e) ? pow2(PLAIN - e) : 1.0f; }
+__device__ __forceinline__ float group_scale(int e) { return pow2(PLAIN - e); }  // of a scaled one
 
 struct Split8 {
     half8 hi, lo;
@@ -806,15 +808,19 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll
             for (int i = 0; i < 8; i++) mx = mag(mx, kx[r].get(i));
         const int e = group_exponent(mx);
-        const float f = group_scale(e);
+        float x[2][8];
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[r][i] = kx[r].get(i);
+        if (scaled(e)) {
+            const float f = group_scale(e);
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i >> 3][i & 7] *= f;
+        }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = kx[r].get(i);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= f;
-            const Split8 s = split8<LO>(x);
+            const Split8 s = split8<LO>(x[r]);
             const int o = (r * 16 + kd) * KFRAG + kk * 16;
             *(half8*)(buf + o) = s.hi;
             if (LO) *(half8*)(buf + KL + o) = s.lo;
@@ -828,15 +834,19 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll
         for (int i = 0; i < 8; i++) mx = mag(mag(mx, vx[i].get(0)), vx[i].get(1));
         const int e = group_exponent(mx);
-        const float f = group_scale(e);
+        float x[2][8];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[j][i] = vx[i].get(j);
+        if (scaled(e)) {
+            const float f = group_scale(e);
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i >> 3][i & 7] *= f;
+        }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = vx[i].get(j);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= f;
-            const Split8 s = split8<LO>(x);
+            const Split8 s = split8<LO>(x[j]);
             const int o = wave * VGROUP + j * 1024 + lane * 16;
             *(half8*)(buf + VH + o) = s.hi;
             if (LO) *(half8*)(buf + VL + o) = s.lo;
@@ -1168,36 +1178,79 @@ struct Plan {
     int nb = 1;          // k_attn_rows: 16-query columns of a wave
     int groups = 1, per = 1, items = 1, whole = 1, nsplit = 1;  // as AttnCall's
     size_t bytes = 0;
+    double cost = 0;  // in us, roughly: what the two kernels are chosen by
     size_t partial() const { return (size_t)(items - whole) * per * nsplit; }
 };
 
-Plan plan_of(const cmf_attention_args& a) {
-    Plan p;
-    const int hpk = a.nh / a.nkv;
-    const long long nq = (long long)a.b * hpk;
-    p.tiles = nq > 32;
-    p.nb = nq <= 16 ? 1 : 2;
-    p.per = p.tiles ? TQ : 16 * p.nb;
-    p.groups = (int)((nq + p.per - 1) / p.per);
-    p.items = p.groups * a.nkv;
-    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, p.per / hpk + 2));
-    // One workgroup a CU of the tiles, two of the rows where one would have more
-    // than two tiles for each of its waves (9 rows of 16 heads: at 2048 keys 15.5
-    // us with one, 17.0 with two; at 12000 36.9 and 31.6).  The items that fill
-    // the card's CUs whole times stay in one piece, the rest is split to fill
-    // them once more, a split of at least 64 keys (256 behind whole items,
-    // which would wait for the join alone).
-    const int room = p.tiles || nv * p.items <= 256 * 128 ? 256 : 512;
-    p.whole = p.items / room * room;
-    const int rest = p.items - p.whole;
-    const long long least = p.whole ? 256 : 64;
+// The items' blocks of `per` queries and the splits over their keys that fill
+// `room` workgroups; where whole items may stay (whole), those that fill it
+// whole times do, and the rest is split to fill it once more.
+void lay_out(const cmf_attention_args& a, long long nq, long long nv, int per, int room, bool whole, long long least, Plan* p) {
+    p->per = per;
+    p->groups = (int)((nq + per - 1) / per);
+    p->items = p->groups * a.nkv;
+    p->whole = whole ? p->items / room * room : 0;
+    const int rest = p->items - p->whole;
     long long ns = rest ? std::max(1ll, std::min<long long>(room / rest, (nv + least - 1) / least)) : 1;
-    const size_t one = (size_t)rest * p.per * (HD + 2) * sizeof(float);
+    const size_t one = (size_t)rest * per * (HD + 2) * sizeof(float);
     while (ns > 1 && one * ns > OP_WS_MAX) ns--;
-    p.nsplit = (int)ns;
-    if (ns == 1) p.whole = p.items;
-    p.bytes = ns > 1 ? one * ns : 0;
+    p->nsplit = (int)ns;
+    if (ns == 1) p->whole = p->items;
+    p->bytes = ns > 1 ? one * ns : 0;
+}
+
+// Keys a workgroup of the rows takes alone: more are split, which costs the
+// join (3 us, and another launch).  8 rows of 16 heads, f32, 108 keys 8.1 us in
+// one piece and 8.5 in two, 158 keys 9.9 and 8.7; f16, 158 keys 6.7 and 7.4,
+// 258 keys 8.3 and 7.5 (a call 8.6 and 10.0).
+long long alone(const cmf_attention_args& a, int nb) { return 256 / nb / (a.kv_dtype == CMF_DT_F32 ? 2 : 1); }
+
+Plan plan_rows(const cmf_attention_args& a, long long nq) {
+    Plan p;
+    p.nb = nq <= 16 ? 1 : 2;
+    const int per = 16 * p.nb;
+    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, per / (a.nh / a.nkv) + 2));
+    // Two workgroups a CU, or one where that gives each wave two tiles at most
+    // (9 rows of 16 heads: at 2048 keys 15.5 us with one, 17.0 with two; at 12000
+    // 36.9 and 31.6).
+    const long long items = (nq + per - 1) / per * a.nkv;
+    const int room = nv * items <= 256 * 128 ? 256 : 512;
+    lay_out(a, nq, nv, per, room, false, nv <= alone(a, p.nb) ? nv : 64, &p);
+    const double wgs = (double)p.items * p.nsplit, tiles = std::ceil((double)nv / p.nsplit / 64);
+    const bool f32 = a.kv_dtype == CMF_DT_F32;
+    p.cost = wgs <= 256 ? 7 + (f32 ? 3 : 1.2) * tiles : std::max(1.0, wgs / 512) * (f32 ? 9 + 6 * tiles : 8 + 2.1 * tiles);
+    if (p.nsplit > 1) p.cost += 3;
     return p;
+}
+
+Plan plan_tiles(const cmf_attention_args& a, long long nq) {
+    Plan p;
+    p.tiles = true;
+    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, TQ / (a.nh / a.nkv) + 2));
+    // One workgroup a CU; a split of 64 keys or more, two tiles stay together
+    // (the join costs more than a tile), behind whole items 256 or more.
+    const bool fills = (nq + TQ - 1) / TQ * a.nkv >= 256;
+    lay_out(a, nq, nv, TQ, 256, true, fills ? 256 : nv <= 128 ? nv : 64, &p);
+    const auto time = [&](double wgs, int ns) {
+        return std::ceil(wgs / 256) * (11 + (a.kv_dtype == CMF_DT_F32 ? 4 : 3) * std::ceil((double)nv / ns / KT));
+    };
+    p.cost = time(p.whole, 1);
+    if (p.nsplit > 1) p.cost += time((double)(p.items - p.whole) * p.nsplit, p.nsplit) + 5;
+    return p;
+}
+
+// Up to 32 queries a kv head are one item of the rows.  Above, the kernel with
+// the lower cost, in us, as both measure: the tiles take longer to begin (11 us)
+// and less a key.  us of the rows and the tiles, 16 heads on 8: trees of 30 rows
+// over 2000 keys f32 17 20, f16 13 18; over 12000 f32 49 41, f16 25 31; 63 rows
+// over 2000 f32 27 25, f16 18 23; over 40000 f16 93 78; windows of 100, 800 rows
+// f32 20 31, f16 14 29; of 1000, 1600 rows f32 127 73, f16 58 61.
+Plan plan_of(const cmf_attention_args& a) {
+    const long long nq = (long long)a.b * (a.nh / a.nkv);
+    const Plan r = plan_rows(a, nq);
+    if (nq <= 32) return r;
+    const Plan t = plan_tiles(a, nq);
+    return r.cost <= t.cost && r.groups <= 65535 ? r : t;
 }
 
 // Allows kernel f its dynamic LDS (once a kernel).

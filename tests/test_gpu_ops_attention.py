@@ -105,7 +105,8 @@ def run_tree(ops, ws, q, k, v, kn, vn, dtype, ctx, mask, depth, window=0, sinks=
     (1, 0, 2, 2, "float32"), (1, 1, 16, 8, "float32"), (2, 0, 4, 1, "bfloat16"), (5, 63, 16, 8, "float32"),
     (9, 64, 12, 4, "float16"), (9, 2048, 16, 8, "float32"), (17, 65, 8, 8, "bfloat16"), (29, 1201, 16, 8, "float32"),
     (33, 500, 32, 2, "float16"), (64, 3001, 32, 8, "bfloat16"), (64, 0, 8, 1, "float32"), (64, 129, 3, 1, "float32"),
-    (64, 4099, 64, 1, "float32"), (7, 20011, 5, 5, "float16"),
+    (64, 4099, 64, 1, "float32"), (7, 20011, 5, 5, "float16"), (64, 5001, 64, 2, "bfloat16"), (64, 5001, 64, 1, "float16"),
+    (29, 12001, 16, 8, "float32"), (3, 300, 600, 600, "float32"), (1, 4001, 300, 300, "bfloat16"),
 ])
 def test_tree(ops, ws, b, ctx, nh, nkv, dtype):
     r = np.random.default_rng(b * 1000 + ctx)
@@ -123,6 +124,7 @@ def test_tree(ops, ws, b, ctx, nh, nkv, dtype):
     (16, 1000, 17, 1000, 16, 4, "float16"), (200, 0, 0, 0, 16, 8, "float32"), (130, 70, 33, 5, 16, 8, "float32"),
     (257, 1000, 128, 4, 12, 4, "bfloat16"), (512, 31, 100, 128, 16, 8, "float32"), (300, 200, 16, 0, 2, 1, "float16"),
     (65, 0, 1, 0, 4, 2, "float32"), (700, 3, 64, 1, 8, 8, "float32"), (90, 4000, 0, 0, 12, 4, "float32"),
+    (900, 2500, 0, 0, 16, 8, "float32"), (1000, 3001, 1500, 70, 12, 4, "bfloat16"), (900, 1000, 1700, 130, 16, 4, "float16"),
 ])
 def test_window(ops, ws, b, ctx, window, sinks, nh, nkv, dtype):
     T = ops.DevTensor
@@ -133,7 +135,8 @@ def test_window(ops, ws, b, ctx, window, sinks, nh, nkv, dtype):
     check(out.numpy(), *reference(q, k, v, visible(b, ctx, window, sinks)))
 
 
-@pytest.mark.parametrize("b,ctx,window,sinks", [(40, 50, 6, 3), (64, 300, 64, 0), (9, 4, 3, 7), (24, 2000, 1, 0)])
+@pytest.mark.parametrize("b,ctx,window,sinks", [(40, 50, 6, 3), (64, 300, 64, 0), (9, 4, 3, 7), (24, 2000, 1, 0),
+                                                (64, 2000, 1500, 40)])
 def test_tree_under_a_window(ops, ws, b, ctx, window, sinks):
     r = np.random.default_rng(b)
     q, k, v = tensors(r, b, ctx, 16, 8, "float32")
@@ -156,13 +159,30 @@ def test_rows_that_see_nothing(ops, ws, b, nh, nkv):
     assert (out[::3] == 0).all()
 
 
+def test_rows_past_every_key_of_their_window(ops, ws):
+    """Rows of a large tree so deep that nothing of a long cache is near, with
+    an empty mask: zeros; the others see the cache."""
+    b, ctx, window, nh = 64, 1000, 900, 64
+    r = np.random.default_rng(15)
+    q, k, v = tensors(r, b, ctx, nh, 1, "float32")
+    _, kn, vn = tensors(r, b, b, nh, 1, "float32")
+    mask = np.array([0 if i % 5 == 2 else 1 << i for i in range(b)], np.uint64)
+    depth = np.array([5000 if i % 5 == 2 else i for i in range(b)], np.int32)
+    out = run_tree(ops, ws, q, k, v, kn, vn, "float32", ctx, mask, depth, window)
+    see = visible(b, ctx, window, 0, mask, depth)
+    check(out, *reference(q, np.concatenate([k, kn], 1), np.concatenate([v, vn], 1), see))
+    assert (out[2::5] == 0).all()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-@pytest.mark.parametrize("b,nh,nkv,dtype", [(5, 16, 8, "float32"), (9, 4, 2, "float16"), (64, 16, 4, "float32"),
-                                            (64, 16, 4, "bfloat16")])
-def test_garbage_where_a_row_does_not_look(ops, ws, b, nh, nkv, dtype, bad):
+@pytest.mark.parametrize("b,nh,nkv,dtype,ctx,window", [
+    (5, 16, 8, "float32", 200, 90), (9, 4, 2, "float16", 200, 90), (64, 16, 4, "float32", 200, 90),
+    (64, 16, 4, "bfloat16", 200, 90), (64, 64, 1, "float32", 1400, 1200), (64, 64, 1, "bfloat16", 3400, 3100),
+    (64, 64, 1, "float16", 3400, 3100)])
+def test_garbage_where_a_row_does_not_look(ops, ws, b, nh, nkv, dtype, ctx, window, bad):
     """A tree row that other rows do not see, cache rows behind the window and
     past the end hold NaN or infinities: only the row that sees them feels it."""
-    ctx, window, sinks = 200, 90, 3
+    sinks = 3
     r = np.random.default_rng(5)
     q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=60)
     _, kn, vn = tensors(r, b, b, nh, nkv, dtype)
@@ -184,33 +204,33 @@ def test_garbage_where_a_row_does_not_look(ops, ws, b, nh, nkv, dtype, bad):
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("what", ["k", "v"])
-def test_garbage_seen_by_some_rows_of_a_chunk(ops, ws, bad, what):
-    """Row 40 of a chunk holds garbage: rows 40 .. 59 see it through a window
-    of 20, the others do not."""
+@pytest.mark.parametrize("b,window", [(160, 20), (1600, 1000)])
+def test_garbage_seen_by_some_rows_of_a_chunk(ops, ws, b, window, bad, what):
+    """Row 40 of a chunk holds garbage: the rows from it see it through their
+    window, the others do not."""
     T = ops.DevTensor
     r = np.random.default_rng(6)
-    b, ctx = 160, 10
+    ctx, last = 10, 40 + window
     q, k, v = tensors(r, b, ctx, 16, 8, "float32", extra=b)
-    want, tol = reference(q, k, v, visible(b, ctx, 20, 0))
+    want, tol = reference(q, k, v, visible(b, ctx, window, 0))
     (k if what == "k" else v)[:, ctx + 40] = bad
     out = filled(ops, q.shape)
-    ops.attention(T.of(q), T.of(k), T.of(v), out, ws, pos0=ctx, window=20)
+    ops.attention(T.of(q), T.of(k), T.of(v), out, ws, pos0=ctx, window=window)
     out = out.numpy()
-    rows = [i for i in range(b) if not 40 <= i < 60]
+    rows = [i for i in range(b) if not 40 <= i < last]
     check(out[rows], want[rows], tol[rows])
-    assert not np.isfinite(out[40:60]).any()
+    assert not np.isfinite(out[40:last]).any()
 
 
 @pytest.mark.parametrize("big", [1e4, 1e10, 1e30])
-@pytest.mark.parametrize("b", [5, 64])
-def test_values_of_another_size_seen_by_some_rows(ops, ws, b, big):
+@pytest.mark.parametrize("b,nh,nkv,ctx,window", [(5, 16, 4, 300, 280), (64, 16, 4, 300, 280), (64, 64, 1, 1300, 1280)])
+def test_values_of_another_size_seen_by_some_rows(ops, ws, b, nh, nkv, ctx, window, big):
     """A leaf of a tree, and a cached position that only the first rows see
     through their window, hold values `big` times the others': the rows that do
     not see them keep their accuracy."""
-    ctx, window = 300, 280
     r = np.random.default_rng(13)
-    q, k, v = tensors(r, b, ctx, 16, 4, "float32")
-    _, kn, vn = tensors(r, b, b, 16, 4, "float32")
+    q, k, v = tensors(r, b, ctx, nh, nkv, "float32")
+    _, kn, vn = tensors(r, b, b, nh, nkv, "float32")
     mask, depth = ops.tree_masks([-1] + [max(0, i - 2) for i in range(1, b)], pos0=ctx, window=window)
     v[:, ctx - window + 1] *= np.float32(big)  # seen at depth 0 alone
     vn[:, b - 1] *= np.float32(big)
@@ -221,12 +241,11 @@ def test_values_of_another_size_seen_by_some_rows(ops, ws, b, big):
 
 
 @pytest.mark.parametrize("size", [1e-18, 1e18])
-@pytest.mark.parametrize("b", [4, 64])
-def test_far_ranges(ops, ws, b, size):
+@pytest.mark.parametrize("b,ctx", [(4, 300), (64, 300), (1000, 1500)])
+def test_far_ranges(ops, ws, b, ctx, size):
     """Keys and values of 1e18 (1e-18) against queries of 1e-18 (1e18)."""
     T = ops.DevTensor
     r = np.random.default_rng(8)
-    ctx = 300
     q, k, v = tensors(r, b, ctx, 8, 2, "float32", extra=b)
     q, k, v = q / np.float32(size), k * np.float32(size), v * np.float32(size)
     out = filled(ops, q.shape)
@@ -234,7 +253,7 @@ def test_far_ranges(ops, ws, b, size):
     check(out.numpy(), *reference(q, k, v, visible(b, ctx, 0, 0)))
 
 
-@pytest.mark.parametrize("b,ctx", [(1, 777), (40, 777), (150, 333)])
+@pytest.mark.parametrize("b,ctx", [(1, 777), (40, 777), (150, 333), (1500, 333)])
 @pytest.mark.parametrize("stream", [None, 0])
 def test_strides_scale_and_a_position_on_the_device(ops, ws, b, ctx, stream):
     """A cache whose positions are interleaved with other data, padded query and
@@ -281,13 +300,13 @@ def test_offsets_past_32_bits(ops, ws):
     check(out.numpy(), *reference(q, tail[0], tail[1], see))
 
 
-@pytest.mark.parametrize("b,tree", [(1, False), (12, True), (64, True), (200, False)])
+@pytest.mark.parametrize("b,tree", [(1, False), (12, True), (64, True), (200, False), (700, False)])
 def test_captured_calls(ops, b, tree):
     """Two captured calls with a scratch each, replayed with other positions and
     eager calls between: every replay equals the eager call, bit for bit."""
     T = ops.DevTensor
     r = np.random.default_rng(11)
-    q, k, v = (T.of(t) for t in tensors(r, b, 1500, 16, 8, "float32"))
+    q, k, v = (T.of(t) for t in tensors(r, b, 1200 + b, 16, 8, "float32"))
     _, kn, vn = (T.of(t) for t in tensors(r, b, b, 16, 8, "float32"))
     at = T.of(np.array([100], np.int32))
     kw = dict(pos0_dev=at, len_bound=1200)
@@ -334,18 +353,18 @@ def test_a_scratch_too_small_is_refused(ops):
 @pytest.mark.parametrize("b,ctx,window,sinks,nh,nkv,dtype", [
     (1030, 500, 0, 0, 32, 16, "float32"), (2060, 40, 600, 4, 16, 16, "float16"), (2060, 900, 0, 0, 16, 16, "bfloat16")])
 def test_blocks_that_do_not_fill_the_card(ops, ws, b, ctx, window, sinks, nh, nkv, dtype):
-    """272 blocks of 128 queries: 256 in one piece, the rest split over their keys."""
+    """272 blocks of 128 queries: as tiles, 256 in one piece and the rest split over
+    their keys."""
     T = ops.DevTensor
     r = np.random.default_rng(b + ctx)
     q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=b)
     out = filled(ops, q.shape)
     dq, dk, dv = T.of(q), T.of(k, dtype), T.of(v, dtype)
-    assert ops.attention_workspace(dq, dk, dv, pos0=ctx, window=window, sinks=sinks) > 0
     ops.attention(dq, dk, dv, out, ws, pos0=ctx, window=window, sinks=sinks)
     check(out.numpy(), *reference(q, k, v, visible(b, ctx, window, sinks)))
 
 
-@pytest.mark.parametrize("b", [1, 9, 80])
+@pytest.mark.parametrize("b", [1, 9, 80, 900])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_values_of_1e36(ops, ws, b, dtype):
     """weights are summed without leaving f32's range"""
