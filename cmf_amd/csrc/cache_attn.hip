@@ -300,6 +300,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     constexpr int NW = 4, QN = 16 * QB, OROW = HD + 4;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr float SHIFT = Part<T>::SHIFT, LAZY = Part<T>::LAZY;
+    constexpr float up = SHIFT < 0 ? 1.f / (1 << (int)-SHIFT) : 1 << (int)SHIFT;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, kq = lane >> 4, split = blockIdx.x, g = blockIdx.y, q0 = blockIdx.z * QN;
     const int nq = a.b * c.hpk;
@@ -433,9 +434,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int v = v0 + 4 * kq + e;
-                    s[qb][e] = (sees(a, ks, see[qb], ks.pos(v)) & (inside | (v < v_hi))) ? s[qb][e] * cq[qb] : -INFINITY;
+                    s[qb][e] = (sees(a, ks, see[qb], ks.pos(v)) & (inside | (v < v_hi))) ? s[qb][e] : -INFINITY;
                 }
-                mx[qb] = lanes4_max(fmaxf(fmaxf(s[qb][0], s[qb][1]), fmaxf(s[qb][2], s[qb][3])));
+                mx[qb] = lanes4_max(fmaxf(fmaxf(s[qb][0], s[qb][1]), fmaxf(s[qb][2], s[qb][3]))) * cq[qb];
                 grow |= mx[qb] > m[qb] + LAZY;
             }
             if (__builtin_amdgcn_ballot_w64(grow)) {
@@ -450,10 +451,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             }
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) {
-                const float ref = (m[qb] == -INFINITY ? 0.f : m[qb]) - SHIFT;
+                // (2^SHIFT as a factor: in the exponent it would cost bits of the score)
+                const float ref = m[qb] == -INFINITY ? 0.f : m[qb];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    s[qb][e] = __builtin_amdgcn_exp2f(s[qb][e] - ref);
+                    s[qb][e] = __builtin_amdgcn_exp2f(fmaf(s[qb][e], cq[qb], -ref)) * up;
                     l[qb] += s[qb][e];
                 }
             }
@@ -1331,7 +1333,8 @@ static int check_attention(const cmf_attention_args* p) {
     if (a.row_stride < HD || a.row_stride % 8 || a.head_stride < 0 || a.head_stride % 8 ||
         (a.k_new && (a.new_row_stride < HD || a.new_row_stride % 8 || a.new_head_stride < 0 || a.new_head_stride % 8)))
         return fail("attention: strides must be multiples of 8 elements, rows of 128");
-    if (a.row_stride > MAX_ROW_STRIDE) return fail("attention: row_stride of at most 2^22 elements");
+    if (a.row_stride > MAX_ROW_STRIDE || (a.k_new && a.new_row_stride > MAX_ROW_STRIDE))
+        return fail("attention: row strides of at most 2^22 elements");
     const long long need = (long long)a.pos0 + (a.k_new ? 0 : a.b);
     if (!a.d_pos0 && need > a.slots) return fail("attention: positions past the cache's slots");
     if (a.d_pos0 && (a.len_bound < 0 || (long long)a.len_bound + (a.k_new ? 0 : a.b) > a.slots))

@@ -467,7 +467,9 @@ int cmf_qk_rope_dev(const cmf_qk_rope_args* a);
  *   the new rows j by bit j of d_mask[i] (b <= 64: cmf_tree_masks), or without
  *   d_mask the rows j <= i under the same window (positions pos0 + j).
  * A row that sees nothing gets zeros.  What a row does not see may hold
- * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  ws: scratch of
+ * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  At most 2^19
+ * rows, 4096 query heads, 64 of them on a kv head, 2^30 positions, row strides
+ * of 2^22 elements; more is refused.  out may be q.  ws: scratch of
  * at least cmf_attention_workspace bytes (at most 64 MiB) that no other call
  * uses meanwhile; captured graphs that may run at the same time need one
  * each. */
@@ -488,8 +490,8 @@ size_t cmf_attention_workspace(const cmf_attention_args* a);
 int cmf_attention_dev(const cmf_attention_args* a);
 /* The masks and depths of a tree of b <= 64 rows given by parents (parent[i] <
  * i; -1: a root), host arrays: bit j of mask[i] for row i itself and its
- * ancestors, those nearer than window rows up where window > 0, and
- * sinks - pos0 rows from the root where sinks reach past pos0. */
+ * ancestors; where window > 0, of these only the ones less than window
+ * generations up or at a position pos0 + depth[j] below sinks. */
 int cmf_tree_masks(const int32_t* parent, int b, int pos0, int window, int sinks, uint64_t* mask, int32_t* depth);
 
 /* Rows copied between caches, all buffers in one launch: for every buffer j <

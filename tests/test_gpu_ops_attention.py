@@ -375,3 +375,14 @@ def test_values_of_1e36(ops, ws, b, dtype):
     out = filled(ops, q.shape)
     ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=700)
     check(out.numpy(), *reference(q, k, v, visible(b, 700, 0, 0)))
+
+
+@pytest.mark.parametrize("b,ctx", [(1, 100), (5, 3000), (1000, 1500)])
+def test_output_over_the_queries(ops, ws, b, ctx):
+    T = ops.DevTensor
+    r = np.random.default_rng(b)
+    q, k, v = (T.of(t) for t in tensors(r, b, ctx, 16, 8, "float32", extra=b))
+    out = filled(ops, q.shape)
+    ops.attention(q, k, v, out, ws, pos0=ctx)
+    ops.attention(q, k, v, q, ws, pos0=ctx)
+    assert np.array_equal(q.numpy(), out.numpy())

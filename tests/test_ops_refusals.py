@@ -49,7 +49,8 @@ def attn(**kw):
     (dict(b=0), "at least 1"), (dict(nh=3), "multiple"), (dict(b=65, d_mask=X, slots=300), "64 rows"),
     (dict(d_depth=X), "d_mask"), (dict(d_mask=X, window=5), "d_depth"), (dict(kv_dtype=15), "kv_dtype"),
     (dict(ldq=510), "ldq"), (dict(ldo=256), "ldo"), (dict(row_stride=64), "strides"), (dict(head_stride=4), "strides"),
-    (dict(k_new=X, v_new=X, new_row_stride=4), "strides"), (dict(pos0=-1), "at least 0"), (dict(window=-1), "at least 0"),
+    (dict(k_new=X, v_new=X, new_row_stride=4), "strides"), (dict(row_stride=(1 << 22) + 8), "strides"),
+    (dict(k_new=X, v_new=X, new_row_stride=1 << 33, new_head_stride=1 << 40), "strides"), (dict(pos0=-1), "at least 0"), (dict(window=-1), "at least 0"),
     (dict(sinks=-2), "at least 0"), (dict(pos0=255), "slots"), (dict(d_pos0=X, len_bound=255), "len_bound"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=X + 8), "aligned"),
     (dict(b=1 << 20, slots=1 << 30), "2^19"), (dict(nh=130, nkv=2, ldq=130 * 128, ldo=130 * 128), "64 query heads"), (dict(slots=(1 << 30) + 1), "2^30"),
