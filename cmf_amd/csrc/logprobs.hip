@@ -9,7 +9,9 @@
 // with the k-th of them and only the few that pass are looked at further.  In
 // the first round the k-th of the lanes' own maxima bounds them.
 // The waves and then the slices of a row meet in a fixed order.
-// Bound by the logits' bytes for many rows, by latency for few.
+// Bound by the logits' bytes for many rows (400 of 151936, f32, 5 alternatives:
+// 57 us, 4.3 TB/s, and 4.9 for the join), by latency for few (5 rows, 8
+// alternatives: 8.4 and 4.7 us).
 #include <math.h>
 
 #include <algorithm>
@@ -43,8 +45,29 @@ __device__ __forceinline__ float key_val(uint64_t k) {  // (what is below -inf's
     const uint32_t u = (uint32_t)(k >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
-    return (uint64_t)(uint32_t)__shfl((int)(v >> 32), src) << 32 | (uint32_t)__shfl((int)(uint32_t)v, src);
+// Lanes' values from the lane ^ O, the lane 63 - lane, or the lane below (lane
+// 0: its own), without a trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lanes_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int O>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
+    if constexpr (O == 1) return lanes_dpp<0xb1>(v);                    // quad_perm [1,0,3,2]
+    else if constexpr (O == 2) return lanes_dpp<0x4e>(v);               // quad_perm [2,3,0,1]
+    else if constexpr (O == 4) return lanes_dpp<0x1b>(lanes_dpp<0x141>(v));  // half-row and quad mirrored
+    else if constexpr (O == 8) return lanes_dpp<0x128>(v);              // row_ror 8
+    else {
+        auto s = O == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false)
+                         : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return lane & O ? s[0] : s[1];
+    }
+}
+__device__ __forceinline__ uint32_t lane_mirror(uint32_t v, int lane) {
+    return lane_xor<32>(lane_xor<16>(lanes_dpp<0x140>(v), lane), lane);  // (rows mirrored first)
+}
+__device__ __forceinline__ uint64_t lane_below(uint64_t v) {  // wave_shr 1
+    return (uint64_t)lanes_dpp<0x138>((uint32_t)(v >> 32)) << 32 | lanes_dpp<0x138>((uint32_t)v);
 }
 __device__ __forceinline__ uint64_t lane64(uint64_t v, int src) {  // src wave-uniform
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), src) << 32 |
@@ -52,26 +75,34 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int src) {  // src wave-u
 }
 
 // one compare-exchange step of a descending bitonic network
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, int o, bool keep_max) {
-    const uint64_t w = shfl64(v, lane ^ o);
+template <int O>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, bool keep_max) {
+    const uint64_t w = (uint64_t)lane_xor<O>((uint32_t)(v >> 32), lane) << 32 | lane_xor<O>((uint32_t)v, lane);
     return (v > w) == keep_max ? v : w;
 }
-// lanes hold a bitonic sequence: sorted, descending
-__device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, int lane) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = exchange(v, lane, o, !(lane & o));
+// blocks of 2 O lanes hold bitonic sequences: sorted, descending in the even
+// blocks, ascending in the odd ones
+template <int O>
+__device__ __forceinline__ uint64_t merge_step(uint64_t v, int lane, bool down) {
+    v = exchange<O>(v, lane, !(lane & O) == down);
+    if constexpr (O > 1) v = merge_step<O / 2>(v, lane, down);
     return v;
 }
+__device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, int lane) { return merge_step<32>(v, lane, true); }
 // Lanes hold sorted lists of n lanes (a power of two), the even ones descending
 // and the odd ones ascending: the wave sorted, descending.
 __device__ __forceinline__ uint64_t merge_lists(uint64_t v, int n, int lane) {
-    for (int m = 2 * n; m <= 64; m <<= 1)
-        for (int o = m >> 1; o; o >>= 1) v = exchange(v, lane, o, !(lane & o) == !(lane & m));
+    if (n <= 1) v = merge_step<1>(v, lane, !(lane & 2));
+    if (n <= 2) v = merge_step<2>(v, lane, !(lane & 4));
+    if (n <= 4) v = merge_step<4>(v, lane, !(lane & 8));
+    if (n <= 8) v = merge_step<8>(v, lane, !(lane & 16));
+    if (n <= 16) v = merge_step<16>(v, lane, !(lane & 32));
+    if (n <= 32) v = merge_step<32>(v, lane, true);
     return v;
 }
 // the 64 largest of two descending lists
 __device__ __forceinline__ uint64_t top_join(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = shfl64(b, 63 - lane);
+    const uint64_t r = (uint64_t)lane_mirror((uint32_t)(b >> 32), lane) << 32 | lane_mirror((uint32_t)b, lane);
     return bitonic_merge(a > r ? a : r, lane);
 }
 // The 64 keys `key` (0: none) taken into the list: one at a time, or sorted
@@ -85,7 +116,7 @@ __device__ __forceinline__ uint64_t top_take(uint64_t best, uint64_t key, uint64
         pass &= pass - 1;
         if (x <= lane64(best, k - 1)) continue;
         const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(best > x));
-        const uint64_t up = shfl64(best, max(lane - 1, 0));
+        const uint64_t up = lane_below(best);
         best = lane < at ? best : lane == at ? x : up;
     }
     return best;
@@ -267,7 +298,8 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
 }
 
 // The slices of a row: every wave joins a quarter of them, then the waves
-// meet.  grid (rows), block 256.
+// meet.  Bound by latency (the slices' states, then their lists by ten to twenty
+// exchanges of a wave).  grid (rows), block 256.
 template <class T, bool TOP>
 __global__ __launch_bounds__(LT) void k_logprobs_join(LpCall c) {
     const cmf_logprobs_args& a = c.a;
