@@ -290,8 +290,12 @@ __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::
 // 16-bit caches: K (16x16x32) and V (16x16x16, its four keys per lane packed by
 // dim) are operands as they lie in memory, the queries and weights in parts.
 //
-// Bound by the cache's bytes: 16 KiB of f32 K/V per tile against 64 MFMAs of
-// 32 cycles per 16 queries, 8 KiB of f16 against 24 of 16.
+// Bound by the cache's bytes where that is long (16 KiB of f32 K/V per tile
+// against 64 MFMAs of 32 cycles per 16 queries, 8 KiB of f16 against 24 of 16),
+// by the chain of round trips where it is short: 5 rows of 32 heads on 8
+// through a window of 16000 in f16, 66 MB, 18.1 us (3.6 TB/s); 9 rows of 16 heads
+// on 8 over 2048 f32 keys 13 us, of which about 4 are the first loads and 3
+// the tile; one row through a window of 1024, 6.3 us.
 // grid (nsplit, nkv, ceil(b hpk / 16 QB)), block 256.
 // ---------------------------------------------------------------------------
 template <class T, int QB>
@@ -618,7 +622,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 //   block 1: weights t - 1 | values t - 1 | stage K t + 1, V t | scores t
 // (only block 1's waves stage and read its values, a tile later).
 //
-// Bound by the MFMAs: 1536 cycles per tile and wave at f32.
+// A tile takes a SIMD about 8000 cycles at f32 and 6700 at 16 bits, of which
+// the MFMAs of its two waves are 3072 and 2048: bound by what each wave does
+// one after the other (scores 1550, weights and values 2300, splitting 1850,
+// loads 1280, the barrier), and by 28000 cycles a workgroup to read and split
+// the queries and to join and write the outputs.  4100 rows of 16 heads on 8
+// behind 4000 through a window of 1024, f32: 186 us, 186 TFLOP/s of the formula
+// (558 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 186 us, 369
+// TFLOP/s (740 of products).
 // grid whole + nsplit (items - whole), block 512, LDS Tile<T>::LDS: the items
 // (those in one piece, then the splits of the others) in eight runs, one to an
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
@@ -1128,7 +1139,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 // The splits of one query by one wave: out = sum w_c o_c / sum w_c l_c,
 // w_c = 2^(m_c - M); lane = dim pair.  The maxima, the sums and CB splits'
 // outputs are requested together, so that up to CB splits take one memory
-// round trip.  Bound by latency.  grid (per, split items), block 64.
+// round trip.  Bound by latency: 2.8 us for 16 queries of 16 splits, 4.8 for
+// 1024 of 32.  grid (per, split items), block 64.
 template <int CB>
 __global__ __launch_bounds__(64) void k_attn_join(AttnCall c) {
     const cmf_attention_args& a = c.a;

@@ -40,7 +40,9 @@ namespace {
 // up (the rotation pairs), so that every access is 16 bytes a lane and a wave
 // serves four heads.  The mean of squares is summed in f64 as the decode
 // layers do (norm_rope); its 16 partials meet by four xor shuffles.  Bound by
-// memory: a head is read once and written once.
+// memory: a head is read once and written once (2001 rows of 32 + 16 heads into
+// a bf16 cache, 91 MB: 16.3 us, 5.6 TB/s, part of it from and to the caches); one
+// row by latency, 2.8 us.
 // grid (ceil(b (nh + 2 nkv) / 16)), block 256: 16 heads a workgroup.
 template <class T>
 __global__ __launch_bounds__(256) void k_qk_rope(cmf_qk_rope_args a) {
@@ -102,7 +104,9 @@ __global__ __launch_bounds__(256) void k_qk_rope(cmf_qk_rope_args a) {
 }
 
 // Rows of 16 C bytes (C = 32: f32, 16: 16-bit caches) by 16-byte pieces, U
-// pieces a thread, all loads before the first store.  Bound by memory.
+// pieces a thread, all loads before the first store.  Bound by memory: 4001
+// rows of 16 caches of 8 heads in f32, 524 MB read and written, 107 us (4.9 TB/s);
+// 5 rows of 56 caches by latency, 2.6 us.
 // grid (ceil(n C / (256 U)), nbuf * nkv), block 256.
 template <int C, int U>
 __global__ __launch_bounds__(256) void k_kv_copy(cmf_kv_copy_args a) {
