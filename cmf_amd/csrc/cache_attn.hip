@@ -616,20 +616,18 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // of a tile on different waves, joined at the end.  Two tile buffers: while one
 // is multiplied, the next tile, in registers since the tile before, is split
 // into the other, and the one after is loaded; one barrier a tile.  The two
-// waves of a SIMD (block 0 and 1) go through a tile half a turn apart, so that
-// the vector work of one runs beside the products of the other:
-//   block 0: scores t | weights t       | values t           | stage t + 1
-//   block 1: weights t - 1 | values t - 1 | stage K t + 1, V t | scores t
-// (only block 1's waves stage and read its values, a tile later).
+// waves of a SIMD (block 0 and 1) go through a tile half a turn apart, one
+// multiplies before it splits and loads, the other after, so that the vector
+// work of one runs beside the products of the other.
 //
-// A tile takes a SIMD about 8000 cycles at f32 and 6700 at 16 bits, of which
+// A tile takes a SIMD about 7800 cycles at f32 and 6600 at 16 bits, of which
 // the MFMAs of its two waves are 3072 and 2048: bound by what each wave does
 // one after the other (scores 1550, weights and values 2300, splitting 1850,
 // loads 1280, the barrier), and by 28000 cycles a workgroup to read and split
 // the queries and to join and write the outputs.  4100 rows of 16 heads on 8
-// behind 4000 through a window of 1024, f32: 186 us, 186 TFLOP/s of the formula
-// (558 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 186 us, 369
-// TFLOP/s (740 of products).
+// behind 4000 through a window of 1024, f32: 181 us, 191 TFLOP/s of the formula
+// (572 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 184 us, 373
+// TFLOP/s (747 of products).
 // grid whole + nsplit (items - whole), block 512, LDS Tile<T>::LDS: the items
 // (those in one piece, then the splits of the others) in eight runs, one to an
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
@@ -995,42 +993,37 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 
     if (v_lo < v_hi) {
         stage_k(0);
-        if (kb == 0) stage_v(0);
+        stage_v(0);
         if (v_lo + KT < v_hi) {
             load_k(v_lo + KT);
-            if (kb == 0) load_v(v_lo + KT);
+            load_v(v_lo + KT);
         }
     }
+    // the tile after v0 into the other buffer, the one after that under way
+    auto next = [&](int v0, int at) {
+        if (v0 + KT < v_hi) {
+            stage_k(at ^ 1);
+            stage_v(at ^ 1);
+            if (v0 + 2 * KT < v_hi) {
+                load_k(v0 + 2 * KT);
+                load_v(v0 + 2 * KT);
+            }
+        }
+    };
     if (kb == 0) {
         for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
             __syncthreads();  // this tile is whole, the other buffer free
             scores(v0, at);
             values(at);
-            if (v0 + KT < v_hi) {
-                stage_k(at ^ 1);
-                stage_v(at ^ 1);
-                if (v0 + 2 * KT < v_hi) {
-                    load_k(v0 + 2 * KT);
-                    load_v(v0 + 2 * KT);
-                }
-            }
+            next(v0, at);
         }
-        __syncthreads();
     } else {
-        int at = 0;
-        for (int v0 = v_lo; v0 < v_hi; v0 += KT, at ^= 1) {
+        for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
             __syncthreads();
-            if (v0 > v_lo) values(at ^ 1);
-            stage_v(at);
-            if (v0 + KT < v_hi) {
-                stage_k(at ^ 1);
-                load_v(v0 + KT);
-                if (v0 + 2 * KT < v_hi) load_k(v0 + 2 * KT);
-            }
+            next(v0, at);
             scores(v0, at);
+            values(at);
         }
-        __syncthreads();
-        if (v_lo < v_hi) values(at ^ 1);
     }
 
     // The wave's state into LDS, in the values' own units (row r = 8 a + 4 h + b
