@@ -278,7 +278,7 @@ __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::
 // Few queries per kv head (decode rows, small trees): the scores and values
 // in f32 on the 16x16x4 MFMA, K and V straight from memory into its operands.
 //
-// A wave takes 16 keys at a time for up to 16 QB queries, transposed so that
+// A wave takes 16 keys at a time for up to 16 queries, transposed so that
 // nothing goes through LDS: S^T = K Q^T (rows keys, columns queries), and the
 // weights come out in the lanes and registers that O^T = V^T P^T wants them
 // in (lane (n, kq) = query n, keys 4 kq + e in register e; the MFMA's k order
@@ -296,19 +296,21 @@ __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::
 // through a window of 16000 in f16, 66 MB, 18.1 us (3.6 TB/s); 9 rows of 16 heads
 // on 8 over 2048 f32 keys 13 us, of which about 4 are the first loads and 3
 // the tile; one row through a window of 1024, 6.3 us.
-// grid (nsplit, nkv, ceil(b hpk / 16 QB)), block 256.
+// grid (nsplit, nkv, ceil(b hpk / 16)), block 256.
 // ---------------------------------------------------------------------------
-template <class T, int QB>
+constexpr int RQ = 16;  // queries of a workgroup
+
+template <class T>
 __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     const cmf_attention_args& a = c.a;
-    constexpr int NW = 4, QN = 16 * QB, OROW = HD + 4;
+    constexpr int NW = 4, OROW = HD + 4;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr float SHIFT = Part<T>::SHIFT, LAZY = Part<T>::LAZY;
     constexpr float up = SHIFT < 0 ? 1.f / (1 << (int)-SHIFT) : 1 << (int)SHIFT;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 15, kq = lane >> 4, split = blockIdx.x, g = blockIdx.y, q0 = blockIdx.z * QN;
+    const int n = lane & 15, kq = lane >> 4, split = blockIdx.x, g = blockIdx.y, q0 = blockIdx.z * RQ;
     const int nq = a.b * c.hpk;
-    const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + QN, nq) - 1);
+    const int r0 = row_of(c, q0), r1 = row_of(c, min(q0 + RQ, nq) - 1);
     const Keys ks = keys_of(a, r0, r1);
 
     const KvRows<T> kv(a, ks, g);
@@ -336,60 +338,47 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     // the queries: lane (n, kq) holds dims 32 j + 8 kq + c of query n (read
     // before the keys: loads are waited for in order)
     constexpr int QF = F32 ? 32 : 1, QP = F32 ? 1 : 4;
-    float qf[QB][QF], cq[QB];  // cq: what the scores are multiplied by, positive
-    uint4v qp[QB][QP][Part<T>::N];
-    Sight see[QB];
-    Raw<float, 8> xq[QB][4];
-    SightIn in[QB];
+    float qf[QF], cq;  // cq: what the scores are multiplied by, positive
+    uint4v qp[QP][Part<T>::N];
+    const int qi = min(q0 + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
+    const SightIn in = sight_in(a, r);
+    const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD;
+    Raw<float, 8> xq[4];
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-        const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
-        in[qb] = sight_in(a, r);
-        const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD;
-#pragma unroll
-        for (int j = 0; j < 4; j++) xq[qb][j].load(q, 32 * j + 8 * kq);
-    }
+    for (int j = 0; j < 4; j++) xq[j].load(q, 32 * j + 8 * kq);
     load(v_lo + 16 * wave);  // (there is a key at least; a wave without a tile reads it in vain)
+    const Sight see = sight_of(a, ks, r, in);
+    float x[32];
+    float f = c.qscale < 0.f ? -1.f : 1.f;
+    int eq = 0;
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-        see[qb] = sight_of(a, ks, row_of(c, min(q0 + 16 * qb + n, nq - 1)), in[qb]);
-        float x[32];
-        float f = c.qscale < 0.f ? -1.f : 1.f;
-        int eq = 0;
+    for (int i = 0; i < 32; i++) x[i] = xq[i >> 3].get(i & 7);
+    if constexpr (Part<T>::SCALED) {
+        float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; i++) x[i] = xq[qb][i >> 3].get(i & 7);
-        if constexpr (Part<T>::SCALED) {
-            float mx = 0.f;
+        for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(x[i]));
+        eq = exponent_of(lanes4_max(mx)) - 14;
+        f *= pow2(-eq);
+    }
+    cq = fmaxf(fabsf(ldexpf(c.qscale, eq)), 1e-37f);  // (not 0: a score that is not seen is -inf)
+    if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(x[i]));
-            eq = exponent_of(lanes4_max(mx)) - 14;
-            f *= pow2(-eq);
-        }
-        cq[qb] = fmaxf(fabsf(ldexpf(c.qscale, eq)), 1e-37f);  // (not 0: a score that is not seen is -inf)
-        if constexpr (F32) {
+        for (int i = 0; i < 32; i++) qf[i] = x[i] * f;
+    } else {
 #pragma unroll
-            for (int i = 0; i < 32; i++) qf[qb][i] = x[i] * f;
-        } else {
+        for (int i = 0; i < 32; i += 2) {
+            uint32_t p[Part<T>::N];
+            parts2<T>(x[i] * f, x[i + 1] * f, p);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                uint32_t p[Part<T>::N];
-                parts2<T>(x[i] * f, x[i + 1] * f, p);
-#pragma unroll
-                for (int k = 0; k < Part<T>::N; k++) qp[qb][i >> 3][k][(i & 7) >> 1] = p[k];
-            }
+            for (int k = 0; k < Part<T>::N; k++) qp[i >> 3][k][(i & 7) >> 1] = p[k];
         }
     }
 
-    float4v acc[QB][8];
-    float m[QB], l[QB];
+    float4v acc[8];
+    float m = -INFINITY, l = 0.f;
     bool odd = false;
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-        m[qb] = -INFINITY;
-        l[qb] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) acc[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int i = 0; i < 8; i++) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
 
     for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
         // a tile with infinities or NaN in V (0 * v is NaN then) is left for the
@@ -412,77 +401,54 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             bad = max((int)x[0], (int)x[1]) >= (int)Part<std::conditional_t<F32, bf16_t, T>>::INF;
         }
         if (__builtin_amdgcn_ballot_w64(bad) == 0) {
-            float4v s[QB];
-#pragma unroll
-            for (int qb = 0; qb < QB; qb++) s[qb] = float4v{0.f, 0.f, 0.f, 0.f};
+            float4v s = {0.f, 0.f, 0.f, 0.f};
             if constexpr (F32) {
 #pragma unroll
                 for (int i = 0; i < 32; i++)
-#pragma unroll
-                    for (int qb = 0; qb < QB; qb++)
-                        s[qb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kn[i >> 3].get(i & 7), qf[qb][i], s[qb], 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(kn[i >> 3].get(i & 7), qf[i], s, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int k = Part<T>::N - 1; k >= 0; k--)  // the small parts first
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int qb = 0; qb < QB; qb++)
-                            s[qb] = Part<T>::mm32(__builtin_bit_cast(uint4v, kn[j].v), qp[qb][j][k], s[qb]);
+                        s = Part<T>::mm32(__builtin_bit_cast(uint4v, kn[j].v), qp[j][k], s);
             }
             const bool inside = v0 + 16 <= v_hi;
-            bool grow = false;
-            float mx[QB];
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int v = v0 + 4 * kq + e;
-                    s[qb][e] = (sees(a, ks, see[qb], ks.pos(v)) & (inside | (v < v_hi))) ? s[qb][e] : -INFINITY;
-                }
-                mx[qb] = lanes4_max(fmaxf(fmaxf(s[qb][0], s[qb][1]), fmaxf(s[qb][2], s[qb][3]))) * cq[qb];
-                grow |= mx[qb] > m[qb] + LAZY;
+            for (int e = 0; e < 4; e++) {
+                const int v = v0 + 4 * kq + e;
+                s[e] = (sees(a, ks, see, ks.pos(v)) & (inside | (v < v_hi))) ? s[e] : -INFINITY;
             }
-            if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float mx = lanes4_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * cq;
+            if (__builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
+                const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1));
+                m = m1;
+                l *= al;
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++) {
-                    const float m1 = fmaxf(m[qb], mx[qb]), al = exp2f(m[qb] - (m1 == -INFINITY ? 0.f : m1));
-                    m[qb] = m1;
-                    l[qb] *= al;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[qb][i] *= al;
-                }
+                for (int i = 0; i < 8; i++) acc[i] *= al;
             }
+            // (2^SHIFT as a factor: in the exponent it would cost bits of the score)
+            const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int qb = 0; qb < QB; qb++) {
-                // (2^SHIFT as a factor: in the exponent it would cost bits of the score)
-                const float ref = m[qb] == -INFINITY ? 0.f : m[qb];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s[qb][e] = __builtin_amdgcn_exp2f(fmaf(s[qb][e], cq[qb], -ref)) * up;
-                    l[qb] += s[qb][e];
-                }
+            for (int e = 0; e < 4; e++) {
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cq, -ref)) * up;
+                l += s[e];
             }
             if constexpr (F32) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-#pragma unroll
-                        for (int qb = 0; qb < QB; qb++)
-                            acc[qb][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vn[e][i / (8 / VP)].get(i % (8 / VP)), s[qb][e],
-                                                                             acc[qb][i], 0, 0, 0);
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vn[e][i / (8 / VP)].get(i % (8 / VP)), s[e], acc[i], 0, 0, 0);
             } else {
-                uint2v w[QB][Part<T>::N];
+                uint2v w[Part<T>::N];
 #pragma unroll
-                for (int qb = 0; qb < QB; qb++)
+                for (int e = 0; e < 4; e += 2) {
+                    uint32_t p[Part<T>::N];
+                    parts2<T>(s[e], s[e + 1], p);
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        uint32_t p[Part<T>::N];
-                        parts2<T>(s[qb][e], s[qb][e + 1], p);
-#pragma unroll
-                        for (int k = 0; k < Part<T>::N; k++) w[qb][k][e >> 1] = p[k];
-                    }
+                    for (int k = 0; k < Part<T>::N; k++) w[k][e >> 1] = p[k];
+                }
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     // dim 8 n + i of the lane's four keys
@@ -490,9 +456,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
                     const uint2v x = {__builtin_amdgcn_perm(vn[1][0].v[i >> 1], vn[0][0].v[i >> 1], sel),
                                       __builtin_amdgcn_perm(vn[3][0].v[i >> 1], vn[2][0].v[i >> 1], sel)};
 #pragma unroll
-                    for (int k = Part<T>::N - 1; k >= 0; k--)
-#pragma unroll
-                        for (int qb = 0; qb < QB; qb++) acc[qb][i] = Part<T>::mm16(x, w[qb][k], acc[qb][i]);
+                    for (int k = Part<T>::N - 1; k >= 0; k--) acc[i] = Part<T>::mm16(x, w[k], acc[i]);
                 }
             }
         } else {
@@ -502,20 +466,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     }
 
     // the wave's state into LDS
-    __shared__ float2 sml[NW][QN];
-    __shared__ __align__(16) float so[NW][QN][OROW];
+    __shared__ float2 sml[NW][RQ];
+    __shared__ __align__(16) float so[NW][RQ][OROW];
     const float un = pow2(-(int)(SHIFT + LAZY));  // (sums of large values stay finite)
+    l = lanes4_sum(l) * un;
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-        l[qb] = lanes4_sum(l[qb]) * un;
+    for (int i = 0; i < 8; i++)
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int r = 4 * kq + e;
-                so[wave][16 * qb + n][VP == 2 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[qb][i][e] * un;
-            }
-    }
+        for (int e = 0; e < 4; e++) {
+            const int r = 4 * kq + e;
+            so[wave][n][VP == 2 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[i][e] * un;
+        }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (odd) {
         // the tiles left out, key by key; lane (n, kq) has 32 dims of its query
@@ -532,33 +493,26 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             for (int k = 0; k < 16; k++) {
                 const int v = v0 + k, pos = ks.pos(min(v, ks.nv - 1));
                 const T *kp = kv.key(pos), *vp = kv.value(pos);
-#pragma unroll
-                for (int qb = 0; qb < QB; qb++) {
-                    const int qi = min(q0 + 16 * qb + n, nq - 1), r = row_of(c, qi), h = g * c.hpk + qi - r * c.hpk;
-                    const float* q = a.q + (size_t)r * a.ldq + (size_t)h * HD + 32 * kq;
-                    float d = 0.f;
+                float d = 0.f;
 #pragma unroll 4
-                    for (int u = 0; u < 32; u++) d = fmaf(q[u], to_f32(kp[32 * kq + u]), d);
-                    d = lanes4_sum(d) * c.qscale;
-                    if (!(sees(a, ks, see[qb], pos) & (v < v_hi))) continue;
-                    float* o = &so[wave][16 * qb + n][32 * kq];
-                    const float m1 = fmaxf(m[qb], d), ref = m1 == -INFINITY ? 0.f : m1;
-                    const float al = exp2f(m[qb] - ref), wt = exp2f(d - ref - LAZY);
+                for (int u = 0; u < 32; u++) d = fmaf(q[32 * kq + u], to_f32(kp[32 * kq + u]), d);
+                d = lanes4_sum(d) * c.qscale;
+                if (!(sees(a, ks, see, pos) & (v < v_hi))) continue;
+                float* o = &so[wave][n][32 * kq];
+                const float m1 = fmaxf(m, d), ref = m1 == -INFINITY ? 0.f : m1;
+                const float al = exp2f(m - ref), wt = exp2f(d - ref - LAZY);
 #pragma unroll 4
-                    for (int u = 0; u < 32; u++) o[u] = o[u] * al + wt * to_f32(vp[32 * kq + u]);
-                    l[qb] = l[qb] * al + wt;
-                    m[qb] = m1;
-                }
+                for (int u = 0; u < 32; u++) o[u] = o[u] * al + wt * to_f32(vp[32 * kq + u]);
+                l = l * al + wt;
+                m = m1;
             }
         }
     }
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++)
-        if (kq == 0) sml[wave][16 * qb + n] = make_float2(m[qb], l[qb]);
+    if (kq == 0) sml[wave][n] = make_float2(m, l);
     __syncthreads();
     // the four waves meet, in wave order; whole rows out
 #pragma unroll
-    for (int t = threadIdx.x; t < QN * 32; t += 256) {
+    for (int t = threadIdx.x; t < RQ * 32; t += 256) {
         const int qq = t >> 5, d = (t & 31) * 4, qi = q0 + qq;
         if (qi >= nq) continue;
         float2 e[NW];
@@ -582,7 +536,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             const float inv = L == 0.f ? 0.f : 1.0f / L;
             *(float4v*)(a.out + (size_t)r * a.ldo + (size_t)h * HD + d) = o * inv;
         } else {
-            const size_t at = ((size_t)(g * c.groups + blockIdx.z) * QN + qq) * c.nsplit + split;
+            const size_t at = ((size_t)(g * c.groups + blockIdx.z) * RQ + qq) * c.nsplit + split;
             *(float4v*)(c.po + at * HD + d) = o;
             if (d == 0) {
                 c.pm[at] = M;
@@ -1182,7 +1136,6 @@ long long keys_bound(const cmf_attention_args& a, int rows) {
 
 struct Plan {
     bool tiles = false;  // k_attn_tiles, else k_attn_rows
-    int nb = 1;          // k_attn_rows: 16-query columns of a wave
     int groups = 1, per = 1, items = 1, whole = 1, nsplit = 1;  // as AttnCall's
     size_t bytes = 0;
     double cost = 0;  // in us, roughly: what the two kernels are chosen by
@@ -1206,27 +1159,22 @@ void lay_out(const cmf_attention_args& a, long long nq, long long nv, int per, i
     p->bytes = ns > 1 ? one * ns : 0;
 }
 
-// Keys a workgroup of the rows takes alone: more are split, which costs the
-// join (3 us, and another launch).  8 rows of 16 heads, f32, 108 keys 8.1 us in
-// one piece and 8.5 in two, 158 keys 9.9 and 8.7; f16, 158 keys 6.7 and 7.4,
-// 258 keys 8.3 and 7.5 (a call 8.6 and 10.0).
-long long alone(const cmf_attention_args& a, int nb) { return 256 / nb / (a.kv_dtype == CMF_DT_F32 ? 2 : 1); }
-
 Plan plan_rows(const cmf_attention_args& a, long long nq) {
     Plan p;
-    p.nb = nq <= 16 ? 1 : 2;
-    const int per = 16 * p.nb;
-    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, per / (a.nh / a.nkv) + 2));
-    // Two workgroups a CU, or one where that gives each wave two tiles at most
-    // (9 rows of 16 heads: at 2048 keys 15.5 us with one, 17.0 with two; at 12000
-    // 36.9 and 31.6).
-    const long long items = (nq + per - 1) / per * a.nkv;
-    const int room = nv * items <= 256 * 128 ? 256 : 512;
-    lay_out(a, nq, nv, per, room, false, nv <= alone(a, p.nb) ? nv : 64, &p);
-    const double wgs = (double)p.items * p.nsplit, tiles = std::ceil((double)nv / p.nsplit / 64);
+    const long long nv = keys_bound(a, (int)std::min<long long>(a.b, RQ / (a.nh / a.nkv) + 2));
     const bool f32 = a.kv_dtype == CMF_DT_F32;
-    p.cost = wgs <= 256 ? 7 + (f32 ? 3 : 1.2) * tiles : std::max(1.0, wgs / 512) * (f32 ? 9 + 6 * tiles : 8 + 2.1 * tiles);
-    if (p.nsplit > 1) p.cost += 3;
+    // Workgroups a CU: one up to 256 keys each (220 keys f32: 20.5 us, with two
+    // 21.7), then two (580 keys f32: 31.8 us with one, 28.4), three for long
+    // 16-bit caches (5800 keys f16: 161 with one, 92 with two, 76; f32 of 4600 127
+    // with two, 150).  Few keys are not split: a join is 3 us, and another launch
+    // (8 rows of 16 heads, f32, 108 keys 8.1 us in one piece and 8.5 in two, 158
+    // keys 9.9 and 8.7; f16, 258 keys 8.3 and 7.5, a call 8.6 and 10.0).
+    const long long load = nv * ((nq + RQ - 1) / RQ * a.nkv);
+    const int room = load <= 256 * 256 ? 256 : !f32 && load > 256 * 4096 ? 768 : 512;
+    lay_out(a, nq, nv, RQ, room, false, nv <= (f32 ? 128 : 256) ? nv : 64, &p);
+    const double wgs = (double)p.items * p.nsplit, tiles = std::ceil((double)nv / p.nsplit / 64);  // of a wave
+    if (wgs <= 256) p.cost = (f32 ? 2.6 + 2.6 * tiles : 3.3 + 1.4 * tiles) + (p.nsplit > 1 ? 3.6 : 0);
+    else p.cost = std::max(1.0, wgs / 512) * (f32 ? 5.5 + 3.1 * tiles : 5.5 + 1.5 * tiles) + (p.nsplit > 1 ? f32 ? 6.5 : 4 : 0);
     return p;
 }
 
@@ -1234,28 +1182,31 @@ Plan plan_tiles(const cmf_attention_args& a, long long nq) {
     Plan p;
     p.tiles = true;
     const long long nv = keys_bound(a, (int)std::min<long long>(a.b, TQ / (a.nh / a.nkv) + 2));
+    const bool f32 = a.kv_dtype == CMF_DT_F32;
     // One workgroup a CU; a split of 64 keys or more, two tiles stay together
     // (the join costs more than a tile), behind whole items 256 or more.
     const bool fills = (nq + TQ - 1) / TQ * a.nkv >= 256;
     lay_out(a, nq, nv, TQ, 256, true, fills ? 256 : nv <= 128 ? nv : 64, &p);
     const auto time = [&](double wgs, int ns) {
-        return std::ceil(wgs / 256) * (11 + (a.kv_dtype == CMF_DT_F32 ? 4 : 3) * std::ceil((double)nv / ns / KT));
+        const double tiles = std::ceil((double)nv / ns / KT);
+        return std::ceil(wgs / 256) * (f32 ? 7.8 + 4.3 * tiles : 8.6 + 2.8 * tiles);
     };
     p.cost = time(p.whole, 1);
-    if (p.nsplit > 1) p.cost += time((double)(p.items - p.whole) * p.nsplit, p.nsplit) + 5;
+    if (p.nsplit > 1) p.cost += time((double)(p.items - p.whole) * p.nsplit, p.nsplit) + (f32 ? 3.4 : 4.4);
     return p;
 }
 
-// Up to 32 queries a kv head are one item of the rows.  Above, the kernel with
-// the lower cost, in us, as both measure: the tiles take longer to begin (11 us)
-// and less a key.  us of the rows and the tiles, 16 heads on 8: trees of 30 rows
-// over 2000 keys f32 17 20, f16 13 18; over 12000 f32 49 41, f16 25 31; 63 rows
-// over 2000 f32 27 25, f16 18 23; over 40000 f16 93 78; windows of 100, 800 rows
-// f32 20 31, f16 14 29; of 1000, 1600 rows f32 127 73, f16 58 61.
+// Up to 16 queries a kv head are one item of the rows.  Above, the kernel with
+// the lower cost, in us, as fitted to 130 random sizes (mean error 8 %; the
+// choice loses 0.4 % to the better one): the tiles take longer to begin, the
+// rows longer a key and query.  us of the rows and the tiles:
+// trees of 30 rows of 32 heads on 8 over 81 keys f32 8.3 16.5; 22 over 26238 f32
+// 144 68; 39 of 16 on 4 over 49610 bf16 98 79; windows of 31, 146 rows bf16 5.0
+// 16.4; of 107, 1241 rows f16 12.2 24.7; of 165, 985 rows f32 41 36.
 Plan plan_of(const cmf_attention_args& a) {
     const long long nq = (long long)a.b * (a.nh / a.nkv);
     const Plan r = plan_rows(a, nq);
-    if (nq <= 32) return r;
+    if (nq <= RQ) return r;
     const Plan t = plan_tiles(a, nq);
     return r.cost <= t.cost && r.groups <= 65535 ? r : t;
 }
@@ -1276,8 +1227,7 @@ template <class T>
 int launch_t(const AttnCall& c, const Plan& p, hipStream_t s) {
     if (!p.tiles) {
         const dim3 grid(c.nsplit, c.a.nkv, p.groups);
-        if (p.nb == 1) hipLaunchKernelGGL((k_attn_rows<T, 1>), grid, dim3(256), 0, s, c);
-        else hipLaunchKernelGGL((k_attn_rows<T, 2>), grid, dim3(256), 0, s, c);
+        hipLaunchKernelGGL(k_attn_rows<T>, grid, dim3(256), 0, s, c);
         return CMF_OK;
     }
     const void* f = (const void*)k_attn_tiles<T>;
