@@ -293,9 +293,12 @@ __device__ __forceinline__ void parts2(float x, float y, uint32_t (&p)[Part<T>::
 // Bound by the cache's bytes where that is long (16 KiB of f32 K/V per tile
 // against 64 MFMAs of 32 cycles per 16 queries, 8 KiB of f16 against 24 of 16),
 // by the chain of round trips where it is short: 5 rows of 32 heads on 8
-// through a window of 16000 in f16, 66 MB, 18.1 us (3.6 TB/s); 9 rows of 16 heads
-// on 8 over 2048 f32 keys 13 us, of which about 4 are the first loads and 3
-// the tile; one row through a window of 1024, 6.3 us.
+// through a window of 16000 in f16, 66 MB, 19 us (3.5 TB/s); 9 rows of 16 heads on
+// 8 over 2048 f32 keys 11 us, of which about 3 are the first loads and 3 two
+// tiles; one row through a window of 1024, 6.2 us.  32 queries a wave read the
+// keys half as often, but begin later and take turns at the MFMAs (9 rows of 16
+// heads: over 100 keys 10.3 us instead of 8.0, over 2048 15.5 instead of 14.2, over
+// 16000 39.9 instead of 42.0).
 // grid (nsplit, nkv, ceil(b hpk / 16)), block 256.
 // ---------------------------------------------------------------------------
 constexpr int RQ = 16;  // queries of a workgroup
