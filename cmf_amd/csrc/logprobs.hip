@@ -6,12 +6,14 @@
 // one is worked on.  Every lane keeps a softmax state of its own (running
 // maximum, sum of weights, sum of weighted differences), every wave the 64
 // largest of its logits, one a lane, in order: a round's logits are compared
-// with the k-th of them and only the few that pass are looked at further.  In
-// the first round the k-th of the lanes' own maxima bounds them.
+// with the k-th of them and only the few that pass wait in LDS to be sorted and
+// joined, 64 at a time.  In the first round the k-th of the lanes' own maxima
+// bounds them.
 // The waves and then the slices of a row meet in a fixed order.
 // Bound by the logits' bytes for many rows (400 of 151936, f32, 5 alternatives:
-// 57 us, 4.3 TB/s, and 4.9 for the join), by latency for few (5 rows, 8
-// alternatives: 8.4 and 4.7 us).
+// 51 us, 4.8 TB/s, and 4.8 for the join), by latency for few (5 rows, 8
+// alternatives: 6.5 and 5.0 us), by the lists for many alternatives (600 rows of
+// 50000: none 26 us in all, 5 alternatives 36, 20 44, 64 62).
 #include <math.h>
 
 #include <algorithm>
@@ -45,8 +47,8 @@ __device__ __forceinline__ float key_val(uint64_t k) {  // (what is below -inf's
     const uint32_t u = (uint32_t)(k >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-// Lanes' values from the lane ^ O, the lane 63 - lane, or the lane below (lane
-// 0: its own), without a trip through LDS.
+// Lanes' values from the lane ^ O or the lane 63 - lane, without a trip through
+// LDS.
 template <int CTRL>
 __device__ __forceinline__ uint32_t lanes_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
@@ -65,9 +67,6 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t v, int lane) {
 }
 __device__ __forceinline__ uint32_t lane_mirror(uint32_t v, int lane) {
     return lane_xor<32>(lane_xor<16>(lanes_dpp<0x140>(v), lane), lane);  // (rows mirrored first)
-}
-__device__ __forceinline__ uint64_t lane_below(uint64_t v) {  // wave_shr 1
-    return (uint64_t)lanes_dpp<0x138>((uint32_t)(v >> 32)) << 32 | lanes_dpp<0x138>((uint32_t)v);
 }
 __device__ __forceinline__ uint64_t lane64(uint64_t v, int src) {  // src wave-uniform
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), src) << 32 |
@@ -90,14 +89,15 @@ __device__ __forceinline__ uint64_t merge_step(uint64_t v, int lane, bool down) 
 }
 __device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, int lane) { return merge_step<32>(v, lane, true); }
 // Lanes hold sorted lists of n lanes (a power of two), the even ones descending
-// and the odd ones ascending: the wave sorted, descending.
-__device__ __forceinline__ uint64_t merge_lists(uint64_t v, int n, int lane) {
-    if (n <= 1) v = merge_step<1>(v, lane, !(lane & 2));
-    if (n <= 2) v = merge_step<2>(v, lane, !(lane & 4));
-    if (n <= 4) v = merge_step<4>(v, lane, !(lane & 8));
-    if (n <= 8) v = merge_step<8>(v, lane, !(lane & 16));
-    if (n <= 16) v = merge_step<16>(v, lane, !(lane & 32));
-    if (n <= 32) v = merge_step<32>(v, lane, true);
+// and the odd ones ascending, zeros from lane `used` on: the wave sorted,
+// descending.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t v, int n, int used, int lane) {
+    if (n <= 1 && used > 1) v = merge_step<1>(v, lane, !(lane & 2));
+    if (n <= 2 && used > 2) v = merge_step<2>(v, lane, !(lane & 4));
+    if (n <= 4 && used > 4) v = merge_step<4>(v, lane, !(lane & 8));
+    if (n <= 8 && used > 8) v = merge_step<8>(v, lane, !(lane & 16));
+    if (n <= 16 && used > 16) v = merge_step<16>(v, lane, !(lane & 32));
+    if (n <= 32 && used > 32) v = merge_step<32>(v, lane, true);
     return v;
 }
 // the 64 largest of two descending lists
@@ -105,23 +105,6 @@ __device__ __forceinline__ uint64_t top_join(uint64_t a, uint64_t b, int lane) {
     const uint64_t r = (uint64_t)lane_mirror((uint32_t)(b >> 32), lane) << 32 | lane_mirror((uint32_t)b, lane);
     return bitonic_merge(a > r ? a : r, lane);
 }
-// The 64 keys `key` (0: none) taken into the list: one at a time, or sorted
-// and joined where many pass (an insertion is about 15 instructions, a sort
-// and join about 250).
-__device__ __forceinline__ uint64_t top_take(uint64_t best, uint64_t key, uint64_t bound, int k, int lane) {
-    uint64_t pass = __builtin_amdgcn_ballot_w64(key > bound);
-    if (__builtin_popcountll(pass) > 12) return top_join(best, merge_lists(key, 1, lane), lane);
-    while (pass) {
-        const uint64_t x = lane64(key, __builtin_ctzll(pass));
-        pass &= pass - 1;
-        if (x <= lane64(best, k - 1)) continue;
-        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(best > x));
-        const uint64_t up = lane_below(best);
-        best = lane < at ? best : lane == at ? x : up;
-    }
-    return best;
-}
-
 // Sums relative to the maximum m: z = sum e^(x - m), h = sum e^(x - m) (x - m)
 // log2(e); nothing yet: m = -inf, z = h = 0.
 struct Soft {
@@ -148,6 +131,7 @@ struct LpCall {
     uint64_t* top;    // [rows][nslice][top_k]
 };
 
+constexpr int LQ = 4 * 64 + 64;  // a wave's queue: what four logits a lane may add to less than 64
 struct LpShared {
     Soft soft[LT / 64];
     uint64_t top[LT / 64][64];
@@ -165,7 +149,7 @@ __device__ __forceinline__ uint64_t top_lists(const uint64_t* src, int ld, int l
     for (int g = from; g < groups; g += step) {
         uint64_t v = next;
         if (g + step < groups) next = load(g + step);
-        v = merge_lists(v, n, lane);
+        v = merge_lists(v, n, min(lists - g * each, each) * n, lane);
         best = g == from ? v : top_join(best, v, lane);
     }
     return best;
@@ -204,7 +188,26 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
     __shared__ LpShared sh;
     const float xt = lp_target<T>(a, row);
     Soft s{-INFINITY, 0.f, 0.f};
-    uint64_t best = 0;
+    // The wave's list, the key that a logit has to pass, and the keys that did
+    // since the list was last brought up to date.
+    uint64_t best = 0, bound = 0;
+    float bv = NAN;
+    int waiting = 0;
+    bool listed = false;
+    __shared__ uint64_t queue[TOP ? LT / 64 : 1][TOP ? LQ : 1];
+    auto take = [&]() {  // the last 64 of them into the list
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int from = max(waiting - 64, 0);
+        const uint64_t key = lane < waiting - from ? queue[wave][from + lane] : 0;
+        const uint64_t v = merge_lists(key, 1, waiting - from, lane);
+        best = listed ? top_join(best, v, lane) : v;
+        listed = true;
+        waiting = from;
+        const uint64_t last = lane64(best, a.top_k - 1);
+        bound = last > bound ? last : bound;
+        bv = key_val(bound);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
 
     auto load = [&](long long r0, float (&v)[LV]) {
 #pragma unroll
@@ -248,7 +251,6 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
             s.h = fmaf(p, fmaxf(d, -1000.f), s.h);
         }
         if constexpr (TOP) {
-            uint64_t bound = lane64(best, a.top_k - 1);
             if (r0 == lo) {
                 // top_k lanes' maxima are at or above this: the upper half of its bits, one by one
                 // (a lane whose maximum is -inf may hold no logit, or NaN: not counted)
@@ -260,25 +262,29 @@ __global__ __launch_bounds__(LT) void k_logprobs(LpCall c) {
                     if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(u >= up)) >= a.top_k) b = up;
                 }
                 bound = (uint64_t)b << 32;
+                bv = key_val(bound);
             }
-            float bv = key_val(bound);
 #pragma unroll
             for (int i = 0; i < LV; i++) {
-                const int id = id_of(r0, i);
                 // (the bound's own value may tie: the keys decide; NaN pass)
-                const bool may = !(v[i] < bv) && id >= 0 && id < a.V && r0 + (long long)(i / VE * LT + t) * VE < hi;
-                if (__builtin_amdgcn_ballot_w64(may)) {
-                    best = top_take(best, may ? key_of(v[i], id) : 0, bound, a.top_k, lane);
-                    const uint64_t last = lane64(best, a.top_k - 1);
-                    bound = last > bound ? last : bound;
-                    bv = key_val(bound);
+                if (__builtin_amdgcn_ballot_w64(!(v[i] < bv))) {
+                    const int id = id_of(r0, i);
+                    const bool is = id >= 0 && id < a.V && r0 + (long long)(i / VE * LT + t) * VE < hi;
+                    const uint64_t key = is ? key_of(v[i], id) : 0, pass = __builtin_amdgcn_ballot_w64(key > bound);
+                    if (key > bound)
+                        queue[wave][waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32),
+                                                                        __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] = key;
+                    waiting += __builtin_popcountll(pass);
                 }
+                if (i % 4 == 3)
+                    while (waiting >= 64) take();
             }
         }
 #pragma unroll
         for (int i = 0; i < LV; i++) v[i] = nx[i];
     }
 
+    if (TOP && waiting) take();
     s = soft_wave(s);
     if (lane == 0) sh.soft[wave] = s;
     if (TOP) sh.top[wave][lane] = best;
