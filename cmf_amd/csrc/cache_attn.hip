@@ -580,11 +580,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // A tile takes a SIMD about 7800 cycles at f32 and 6600 at 16 bits, of which
 // the MFMAs of its two waves are 3072 and 2048: bound by what each wave does
 // one after the other (scores 1550, weights and values 2300, splitting 1850,
-// loads 1280, the barrier), and by 28000 cycles a workgroup to read and split
+// loads 1280, the barrier), and by 26000 cycles a workgroup to read and split
 // the queries and to join and write the outputs.  4100 rows of 16 heads on 8
-// behind 4000 through a window of 1024, f32: 181 us, 191 TFLOP/s of the formula
-// (572 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 184 us, 373
-// TFLOP/s (747 of products).
+// behind 4000 through a window of 1024, f32: 176 us, 196 TFLOP/s of the formula
+// (588 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 185 us, 371
+// TFLOP/s (743 of products).
 // grid whole + nsplit (items - whole), block 512, LDS Tile<T>::LDS: the items
 // (those in one piece, then the splits of the others) in eight runs, one to an
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the
@@ -715,7 +715,15 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
                 vx[i].load(kv.value(ks.pos(min(v0 + vk + 8 * (i >> 2) + (i & 3), ks.nv - 1))), 2 * lane);
         }
     };
-    if (v_lo < v_hi) {  // under way while the queries are split
+    // The queries' rows, whole, on their way to LDS, and behind them the first
+    // tile (loads are waited for in order).
+    float4v qx[TQ / 16];
+#pragma unroll
+    for (int k = 0; k < TQ / 16; k++) {
+        const int qi = min(q0 + 16 * k + (t >> 5), nq - 1), row = row_of(c, qi), head = g * c.hpk + qi - row * c.hpk;
+        qx[k] = *(const float4v*)(a.q + (size_t)row * a.ldq + (size_t)head * HD + 4 * (t & 31));
+    }
+    if (v_lo < v_hi) {
         load_k(v_lo);
         load_v(v_lo);
     }
@@ -734,14 +742,9 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     half8 qh[8], ql[8];
     float cq;  // the scores' factor: |scale| * log2(e) * 2^(eq - 14)
     {
-        // whole rows through LDS
         float* sq = (float*)sm;
 #pragma unroll
-        for (int k = 0; k < TQ / 16; k++) {
-            const int i = 16 * k + (t >> 5), qi = min(q0 + i, nq - 1), row = row_of(c, qi), head = g * c.hpk + qi - row * c.hpk;
-            *(float4*)(sq + i * OROW + 4 * (t & 31)) =
-                *(const float4*)(a.q + (size_t)row * a.ldq + (size_t)head * HD + 4 * (t & 31));
-        }
+        for (int k = 0; k < TQ / 16; k++) *(float4v*)(sq + (16 * k + (t >> 5)) * OROW + 4 * (t & 31)) = qx[k];
         __syncthreads();
         const float* q = sq + (32 * qg + n) * OROW + 8 * h;
         float x[8][8], mx = 0.f;
