@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // work of one runs beside the products of the other.
 //
 // A tile takes a SIMD about 7800 cycles at f32 and 6600 at 16 bits, of which
-// the MFMAs of its two waves are 3072 and 2048: bound by what each wave does
+// the MFMAs of its two waves take 96 and 64 times 32: bound by what each wave does
 // one after the other (scores 1550, weights and values 2300, splitting 1850,
 // loads 1280, the barrier), and by 26000 cycles a workgroup to read and split
 // the queries and to join and write the outputs.  4100 rows of 16 heads on 8
