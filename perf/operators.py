@@ -26,7 +26,7 @@ HD = 128
 EPS = 1e-6
 THETA = 1e6
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
-WS_BYTES = 64 << 20  # the scratch a program keeps for the attention and the log probabilities
+WS_BYTES = 64 << 20  # the scratch a program keeps for the attention
 
 
 def listed():
@@ -161,8 +161,7 @@ def prepare(case, seed):
     x.scatter_add_(1, tgt[:, None], r.normal(rows, 1, std=4.0).abs())
     s.update(x=x.to(DTYPES[c["dtype"]]), tgt=tgt.to(torch.int32), lp=torch.empty(rows, device="cuda"),
              ent=torch.empty(rows, device="cuda"), ids=torch.empty(rows, c["k"], dtype=torch.int32, device="cuda"),
-             top=torch.empty(rows, c["k"], device="cuda"),
-             ws=torch.empty(WS_BYTES, dtype=torch.uint8, device="cuda"))
+             top=torch.empty(rows, c["k"], device="cuda"))
     return s
 
 
@@ -263,6 +262,8 @@ def _run_own(s):
         ops.kv_copy(s["dst_ptrs"], s["src_ptrs"], s["dst"][0], s["src"][0], n=c["n"], pos0=c["pos0"], idx=s["idx"],
                     stream=s["stream"])
         return s["dst"]
+    if "ws" not in s:  # the scratch, made once and kept as the attention's
+        s["ws"] = torch.empty(WS_BYTES, dtype=torch.uint8, device="cuda")
     ops.logprobs(s["x"], s["tgt"], s["lp"], s["ent"], s["ids"] if c["k"] else None, s["top"] if c["k"] else None, s["ws"],
                  stream=s["stream"])
     return dict(lp=s["lp"], ent=s["ent"], **(dict(ids=s["ids"], top=s["top"]) if c["k"] else {}))
