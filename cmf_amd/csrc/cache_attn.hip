@@ -422,9 +422,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
                 const int v = v0 + 4 * kq + e;
                 s[e] = (sees(a, ks, see, ks.pos(v)) & (inside | (v < v_hi))) ? s[e] : -INFINITY;
             }
-            const float mx = lanes4_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * cq;
-            if (__builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
-                const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1));
+            // (maximum and differences before the factor: exact near the maximum,
+            // however large the scores; 0 for the largest one)
+            const float mx = lanes4_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+            if (__builtin_amdgcn_ballot_w64((mx - m) * cq > LAZY)) {
+                const float m1 = fmaxf(m, mx), al = exp2f((m - (m1 == -INFINITY ? 0.f : m1)) * cq);
                 m = m1;
                 l *= al;
 #pragma unroll
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cq, -ref)) * up;
+                s[e] = __builtin_amdgcn_exp2f((s[e] - ref) * cq) * up;
                 l += s[e];
             }
             if constexpr (F32) {
@@ -473,6 +475,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
     __shared__ __align__(16) float so[NW][RQ][OROW];
     const float un = pow2(-(int)(SHIFT + LAZY));  // (sums of large values stay finite)
     l = lanes4_sum(l) * un;
+    m *= cq;  // in log2 units from here on
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -593,6 +596,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 
 constexpr int KT = 64, TQ = 128;     // keys of a tile, queries of a workgroup
 constexpr float SHIFT = 6.f, LAZY = 8.f;  // weights are 2^(s - m + SHIFT) <= 2^(SHIFT + LAZY)
+constexpr float FAR_SCORE = 4096.f;  // (log2 units: a product's rounding moves a weight by 2^-12 of itself here)
 constexpr int KFRAG = 528;           // 32 keys x 8 dims (512 B), padded against bank conflicts
 constexpr int K_BYTES = 32 * KFRAG;  // one half (hi or lo) of the keys
 constexpr int VGROUP = 2048;         // 8 keys x 128 dims: [dim % 2][dim / 2][8 keys]
@@ -916,7 +920,20 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             for (int d = 0; d < 4; d++) acc[d] *= f;
             m = m1;
         }
-        const float ref = (m == -INFINITY ? 0.f : m) - SHIFT;
+        const float m0 = m == -INFINITY ? 0.f : m;
+        float f = cq, ref = m0 - SHIFT;
+        if (__builtin_amdgcn_ballot_w64(fabsf(m0) > FAR_SCORE)) {
+            // Far from 0 a score is rounded as the maximum was before that is taken
+            // off: the largest is then 0, and not what the product's rounding left.
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float p = s[i] * cq;
+                asm("" : "+v"(p));  // (no fma)
+                s[i] = p - m0;
+            }
+            f = 1.f;
+            ref = -SHIFT;
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             // the weights in units of the values' scale, their sum in its own
@@ -925,7 +942,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             float x[8], lu = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], cq, -ru));
+                x[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], f, -ru));
                 lu += x[i];
             }
             l = fmaf(lu, ldexpf(1.0f, -de), l);

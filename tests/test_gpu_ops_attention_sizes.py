@@ -1,0 +1,47 @@
+"""cmf_attention_dev where the sizes of queries, keys, values and scores differ
+within a call: what a row does not see may be of any size, and neither kernel
+may lose what it does see.  Sizes take the kernel of few queries and the one of
+tiles, whole and split over the keys.
+
+Tolerances are those of test_gpu_ops_attention.py: by the largest key and value
+that a row sees, so that they stay tight for the rows that see ordinary ones."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from conftest import ROOT
+from ops_util import rounded
+from test_gpu_ops_attention import HD, U, check, filled, ops, reference, run_tree, tensors, visible, ws  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- scores ---------------------------------------------------------------
+@pytest.mark.parametrize("power", [3, 8, 12, 20, 30])
+@pytest.mark.parametrize("b,ctx,nh,nkv,dtype", [
+    (5, 300, 16, 8, "float32"), (9, 3000, 16, 8, "float16"), (3, 500, 4, 2, "bfloat16"), (64, 300, 16, 4, "float32"),
+    (64, 3000, 64, 1, "bfloat16"), (1000, 1500, 16, 8, "float32"), (1000, 1500, 16, 8, "float16")])
+def test_large_scores(ops, ws, b, ctx, nh, nkv, dtype, power):
+    """Queries and keys of 1 and -1 in their first 6 dims times 2^power: scores
+    are exact in f32, distinct ones lie at least 2^(2 power - 2) apart.  For the
+    larger powers the weights are 1 for the keys that share a row's largest
+    score and 0 for all others: the output is those values' mean, rounded like
+    any sum (2^-24 of the largest value for each of its sqrt(n) independent
+    roundings, 8 fold, and a few for the operands in parts)."""
+    T = ops.DevTensor
+    r = np.random.default_rng(b + ctx + power)
+    q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=b)
+    most = 12 if dtype == "float16" else 60
+    for t, p in ((q, 2 * power - min(power, most)), (k, min(power, most))):
+        t[...] = np.where(t < 0, -1, 1)
+        t[..., 6:] = 0
+        t *= np.float32(2.0 ** p)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx, scale=0.125)
+    want, tol = reference(q, k, v, visible(b, ctx, 0, 0), 0.125)
+    if power > 3:  # (one step between scores is 2^14 at least: e^-2^14 is 0)
+        tol = np.abs(v).max() * U * (8 * np.sqrt(ctx + b) + 16) + 0 * tol
+    check(out.numpy(), want, tol)
