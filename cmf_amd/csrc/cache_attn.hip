@@ -503,6 +503,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 #pragma unroll 4
                 for (int u = 0; u < 32; u++) d = fmaf(q[32 * kq + u], to_f32(kp[32 * kq + u]), d);
                 d = lanes4_sum(d) * c.qscale;
+                asm("" : "+v"(d));  // (rounded before the maximum comes off: no fma)
                 if (!(sees(a, ks, see, pos) & (v < v_hi))) continue;
                 float* o = &so[wave][n][32 * kq];
                 const float m1 = fmaxf(m, d), ref = m1 == -INFINITY ? 0.f : m1;
@@ -1068,6 +1069,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll 4
                 for (int u = 0; u < 64; u++) d = fmaf(q[u], to_f32(kp[64 * h1 + u]), d);
                 d = lanes2_sum(d) * c.qscale;
+                asm("" : "+v"(d));  // (rounded before the maximum comes off: no fma)
                 if (!vis) continue;
                 const float m1 = fmaxf(m, d), ref = m1 == -INFINITY ? 0.f : m1, al = exp2f(m - ref), wt = ldexpf(exp2f(d - ref), -(int)LAZY);
 #pragma unroll 4

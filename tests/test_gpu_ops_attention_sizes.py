@@ -45,3 +45,24 @@ def test_large_scores(ops, ws, b, ctx, nh, nkv, dtype, power):
     if power > 3:  # (one step between scores is 2^14 at least: e^-2^14 is 0)
         tol = np.abs(v).max() * U * (8 * np.sqrt(ctx + b) + 16) + 0 * tol
     check(out.numpy(), want, tol)
+
+
+@pytest.mark.parametrize("power", [12, 20, 30])
+@pytest.mark.parametrize("b,ctx,nh,nkv,dtype", [(5, 300, 16, 8, "float32"), (9, 300, 16, 8, "bfloat16"),
+                                                (700, 900, 16, 4, "float32"), (700, 900, 16, 4, "bfloat16")])
+def test_large_scores_beside_garbage(ops, ws, b, ctx, nh, nkv, dtype, power):
+    """The same, where the last row's value is infinite: keys beside it are gone
+    through one by one."""
+    T = ops.DevTensor
+    r = np.random.default_rng(b + ctx + power)
+    q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=b)
+    for t in (q, k):
+        t[...] = np.where(t < 0, -1, 1)
+        t[..., 6:] = 0
+        t *= np.float32(2.0 ** power)
+    want, tol = reference(q, k, v, visible(b, ctx, 0, 0), 0.125)
+    tol = np.abs(v).max() * U * (8 * np.sqrt(ctx + b) + 16) + 0 * tol
+    v[:, ctx + b - 1] = np.inf
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx, scale=0.125)
+    check(out.numpy()[:-1], want[:-1], tol[:-1])
