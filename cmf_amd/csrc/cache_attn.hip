@@ -38,8 +38,8 @@ constexpr int HD = CACHE_HD;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr long long MAX_ROW_STRIDE = 1 << 22;  // a tile's offsets stay in 32 bits
 
-// the largest of the wave (the same in every lane)
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+// the largest of each 16 lanes
+__device__ __forceinline__ uint32_t lanes16_max_u32(uint32_t v) {
     auto step = [&](auto ctrl) {
         v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true));
     };
@@ -47,6 +47,11 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     step(std::integral_constant<int, 0x4e>{});   // quad_perm [2,3,0,1]
     step(std::integral_constant<int, 0x141>{});  // row_half_mirror
     step(std::integral_constant<int, 0x140>{});  // row_mirror
+    return v;
+}
+// the largest of the wave (the same in every lane)
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = lanes16_max_u32(v);
     auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = max(a[0], a[1]);
     auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
@@ -560,15 +565,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // no kl and vl), three products at 16 times the f32 MFMA's rate.
 //
 // f16 has 5 exponent bits, so operands of an unusual size are scaled by a power
-// of two first (exact): 4 keys or 8 keys' values at a time whose largest
+// of two first (exact): a key row or 8 keys' values at a time whose largest
 // magnitude is not in [2^-2, 2^6) to [2^2, 2^3), a query row always, to [2^14,
 // 2^15).  The keys' factor is undone in the scores, the values' in the weights
 // (2^(s - m + 6), m at most 8 below the maximum), relative to the largest
 // factor so far (the accumulated output follows when that grows).  What the
-// halves drop is then 2^-23 of an element or of its group's largest.
-// A block of 32 keys that holds infinities, NaN or values 2^12 from the others'
-// (anything in a row that some query does not see) is left for a second walk
-// without MFMAs, so that it reaches only the queries that see it.
+// halves drop is then 2^-23 of an element or of its row's or group's largest:
+// a key's score depends on no other key.
+// A block of 32 keys that holds infinities, NaN, keys from 2^101 or below
+// 2^-100, or values 2^12 from the others' (anything in a row that some query
+// does not see) is left for a second walk without MFMAs, so that it reaches only
+// the queries that see it.
 //
 // S^T = K Q^T: a lane (query n = lane % 32, h = lane / 32) ends up with the
 // keys 8 a + 4 h + b of a 32-key block in register 4 a + b, which is the B
@@ -608,7 +615,9 @@ template <class T>
 struct Tile {
     static constexpr bool LO = sizeof(T) == 4;
     static constexpr int HALVES = LO ? 2 : 1, BUF = HALVES * (K_BYTES + V_BYTES);
-    static constexpr int USE = 2 * (BUF + 128);  // and the exponents of their groups: a block's 8 of K, 4 of V, in 64 bytes
+    // and of a block's groups: 8 codes of K and 4 exponents of V in 64 bytes, the
+    // key rows' factors
+    static constexpr int USE = 2 * (BUF + 128 + 4 * KT);
     static constexpr int LDS = USE > END_BYTES ? USE : END_BYTES;
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
@@ -617,6 +626,10 @@ constexpr int SCHED_MFMA = 8, SCHED_LDS = 0x100;  // of sched_group_barrier: MFM
 // A group's scale 2^(PLAIN - e) by the largest magnitude of the wave's elements:
 // e = PLAIN where f16 halves take them as they are; all zeros; infinities, NaN
 constexpr int PLAIN = 2, NO_EXP = -1000, BAD_EXP = 1000;
+// What a group of four key rows is: as it stands; rows with factors of their own;
+// something that halves and f32 scores between them cannot hold
+enum { ROWS_PLAIN = 0, ROWS_SCALED = 1, ROWS_ODD = 2 };
+constexpr int KEY_RANGE = 100;  // exponents: scores by 2^-14 of a query's stay below 2^25+100, queries' factors normal
 constexpr int FAR = 12;  // values 2^FAR apart are not summed with each other's halves
 __device__ __forceinline__ int exponent_class(uint32_t u) {  // of a magnitude's bits
     const int e = (int)(u >> 23) - 127;
@@ -627,6 +640,21 @@ __device__ __forceinline__ int group_exponent(float mx) {
     if (!__builtin_amdgcn_ballot_w64(!(mx < 64.f)) && __builtin_amdgcn_ballot_w64(mx >= 0.25f)) return PLAIN;
     return exponent_class(__builtin_amdgcn_readfirstlane(wave_max_u32(__float_as_uint(mx))));
 }
+// Whether all lanes' magnitudes are below 2^6 and each 16 lanes hold one of
+// 2^-2 or more in a and in b.
+__device__ __forceinline__ bool each16(uint64_t m) {
+    m |= m >> 8;
+    m |= m >> 4;
+    m |= m >> 2;
+    m |= m >> 1;
+    return (~m & 0x0001000100010001ull) == 0;
+}
+__device__ __forceinline__ bool rows16_plain(float a, float b) {
+    return !__builtin_amdgcn_ballot_w64(!(mag(a, b) < 64.f)) && each16(__builtin_amdgcn_ballot_w64(a >= 0.25f)) &&
+           each16(__builtin_amdgcn_ballot_w64(b >= 0.25f));
+}
+// whether the tiles cannot take a key row whose largest magnitude has class e
+__device__ __forceinline__ bool odd_key(int e) { return e == BAD_EXP || (e != NO_EXP && (e > KEY_RANGE || e < -KEY_RANGE)); }
 __device__ __forceinline__ bool scaled(int e) { return e != PLAIN && e != NO_EXP; }
 __device__ __forceinline__ float group_scale(int e) { return pow2(PLAIN - e); }  // of a scaled one
 
@@ -670,7 +698,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     constexpr bool LO = Tile<T>::LO;
     constexpr int BUF = Tile<T>::BUF, KL = K_BYTES, VH = Tile<T>::HALVES * K_BYTES, VL = VH + V_BYTES;
     extern __shared__ __align__(16) uint8_t sm[];
-    int* texp = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: 4 of K, 2 of V
+    int* texp = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: codes of 4 groups of K, exponents of 2 of V
+    float* kfac = (float*)(texp + 64);  // [buffer][key]: factors of the rows of groups with ROWS_SCALED
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 31, h = lane >> 5, nq = a.b * c.hpk;
     const bool part = (int)blockIdx.x >= c.whole;
@@ -774,25 +803,30 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     }
 
     // The tile in registers into buffer `at`.  This wave stages keys 4 wave ..
-    // 4 wave + 3 of both blocks (with one scale) and the values of group `wave`.
+    // 4 wave + 3 of both blocks (16 lanes a row) and the values of group `wave`.
     auto stage_k = [&](int at) {
         uint8_t* buf = sm + at * BUF;
-        int* te = texp + at * 32;
-        float mx = 0.f;
+        int* te = texp + at * 32 + 8 * (wave & 1) + (wave >> 1);
+        float x[2][8], mx[2] = {0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 2; r++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) mx = mag(mx, kx[r].get(i));
-        const int e = group_exponent(mx);
-        float x[2][8];
+            for (int i = 0; i < 8; i++) {
+                x[r][i] = kx[r].get(i);
+                mx[r] = mag(mx[r], x[r][i]);
+            }
+        int code[2] = {ROWS_PLAIN, ROWS_PLAIN};
+        if (!rows16_plain(mx[0], mx[1])) {
 #pragma unroll
-        for (int r = 0; r < 2; r++)
+            for (int r = 0; r < 2; r++) {
+                const int e = exponent_class(lanes16_max_u32(__float_as_uint(mx[r])));
+                const bool sc = scaled(e) && !odd_key(e);
+                code[r] = __builtin_amdgcn_ballot_w64(odd_key(e)) ? ROWS_ODD : ROWS_SCALED;
+                const float f = sc ? pow2(PLAIN - e) : 1.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[r][i] = kx[r].get(i);
-        if (scaled(e)) {
-            const float f = group_scale(e);
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i >> 3][i & 7] *= f;
+                for (int i = 0; i < 8; i++) x[r][i] *= f;
+                if (kd == 0) kfac[at * KT + 32 * r + kk] = sc ? pow2(e - PLAIN) : 1.f;
+            }
         }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
@@ -800,7 +834,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             const int o = (r * 16 + kd) * KFRAG + kk * 16;
             *(half8*)(buf + o) = s.hi;
             if (LO) *(half8*)(buf + KL + o) = s.lo;
-            te[16 * r + 8 * (wave & 1) + (wave >> 1)] = e;  // (all lanes the same)
+            te[16 * r] = code[r];  // (all lanes the same)
         }
     };
     auto stage_v = [&](int at) {
@@ -841,7 +875,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 
     constexpr int RD = LO ? 2 : 1, MM = LO ? 3 : 2;  // fragments read and products of a step
     float16v s;         // the block's scores, by 1 / cq
-    bool kbad = false;  // its keys hold infinities or NaN
+    bool kbad = false;  // one of its keys is odd
     // the scores of the wave's block of the tile at v0, in buffer `at`
     auto scores = [&](int v0, int at) {
         const uint8_t* buf = sm + at * BUF;
@@ -868,14 +902,14 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         }
         __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 3 * MM, 0);
         kbad = false;
-        if (__builtin_amdgcn_ballot_w64((int)scaled(ek.x) | (int)scaled(ek.y) | (int)scaled(ek.z) | (int)scaled(ek.w))) {
-            kbad = __builtin_amdgcn_ballot_w64(max(max(ek.x, ek.y), max(ek.z, ek.w)) == BAD_EXP) != 0;
+        if (__builtin_amdgcn_ballot_w64((ek.x | ek.y | ek.z | ek.w) != ROWS_PLAIN)) {
+            kbad = __builtin_amdgcn_ballot_w64(max(max(ek.x, ek.y), max(ek.z, ek.w)) == ROWS_ODD) != 0;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int e = i == 0 ? ek.x : i == 4 ? ek.y : i == 8 ? ek.z : ek.w;
-                const float f = scaled(e) ? ldexpf(1.0f, e - PLAIN) : 1.0f;
+                const float4v f = *(const float4v*)(kfac + at * KT + 32 * kb + 2 * i + 4 * h);
 #pragma unroll
-                for (int b = 0; b < 4; b++) s[i + b] *= f;
+                for (int b = 0; b < 4; b++) s[i + b] *= e == ROWS_SCALED ? f[b] : 1.f;
             }
         }
         // whether every query of the workgroup sees the whole tile
@@ -1033,18 +1067,17 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         int es = NO_EXP;
 #pragma unroll 1
         for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
-            bool bad = false;  // infinities or NaN among the tile's keys
-            float mv = 0.f;    // the largest of value row n of the block
-#pragma unroll 1
-            for (int r = 0; r < 2; r++) {
-                const int pos = ks.pos(min(v0 + 32 * r + n1, ks.nv - 1));
+            float mk = 0.f, mv = 0.f;  // the largest of key and value row n of the block
+            {
+                const int pos = ks.pos(min(v0 + 32 * kb + n1, ks.nv - 1));
                 const T *kp = kv.key(pos), *vp = kv.value(pos);
 #pragma unroll 1
                 for (int u = 0; u < HD; u++) {
-                    bad |= !(fabsf(to_f32(kp[u])) < INFINITY);
-                    if (r == kb) mv = mag(mv, to_f32(vp[u]));
+                    mk = mag(mk, to_f32(kp[u]));
+                    mv = mag(mv, to_f32(vp[u]));
                 }
             }
+            const bool bad = odd_key(exponent_class(__float_as_uint(mk)));
             uint32_t um = __float_as_uint(mv);  // of its group: keys 16 u + 4 h1 + {0 .. 3, 8 .. 11}
             um = max(um, (uint32_t)__shfl_xor((int)um, 1));
             um = max(um, (uint32_t)__shfl_xor((int)um, 2));

@@ -66,3 +66,53 @@ def test_large_scores_beside_garbage(ops, ws, b, ctx, nh, nkv, dtype, power):
     out = filled(ops, q.shape)
     ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx, scale=0.125)
     check(out.numpy()[:-1], want[:-1], tol[:-1])
+
+
+# ---- keys -----------------------------------------------------------------
+@pytest.mark.parametrize("dtype,big", [("float32", 1e4), ("float32", 1e6), ("float32", 1e10), ("float32", 1e30),
+                                       ("float16", 1e4), ("bfloat16", 1e6), ("bfloat16", 1e30)])
+@pytest.mark.parametrize("b,nh,nkv,ctx,window", [(5, 16, 4, 300, 280), (64, 16, 4, 300, 280), (64, 64, 1, 1300, 1280)])
+def test_keys_of_another_size_seen_by_some_rows(ops, ws, b, nh, nkv, ctx, window, dtype, big):
+    """A leaf of a tree, and a cached position that only the first rows see
+    through their window, hold keys `big` times the others."""
+    r = np.random.default_rng(21)
+    q, k, v = tensors(r, b, ctx, nh, nkv, dtype)
+    _, kn, vn = tensors(r, b, b, nh, nkv, dtype)
+    mask, depth = ops.tree_masks([-1] + [max(0, i - 2) for i in range(1, b)], pos0=ctx, window=window)
+    near = np.float32(1 if dtype == "float16" else 4)  # (f16 ends at 65504)
+    for t, at in ((k, ctx - window + 1), (kn, b - 1)):
+        t[:, at] = rounded(np.clip(t[:, at], -near, near) * np.float32(big), dtype)
+    see = visible(b, ctx, window, 0, mask, depth)
+    want, tol = reference(q, np.concatenate([k, kn], 1), np.concatenate([v, vn], 1), see)
+    check(run_tree(ops, ws, q, k, v, kn, vn, dtype, ctx, mask, depth, window), want, tol)
+
+
+@pytest.mark.parametrize("small", [1e-4, 1e-12])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("b", [100, 2000])
+def test_small_keys_between_ordinary_ones(ops, ws, b, small, dtype):
+    """Through a window of two, half the rows see keys `small` times the ordinary
+    ones beside them, with queries as much larger: scores of the usual size."""
+    T = ops.DevTensor
+    r = np.random.default_rng(22)
+    q, k, v = tensors(r, b, 0, 16, 8, dtype, extra=b)
+    at = np.arange(b) % 4
+    k[:, at != 1] = rounded(k[:, at != 1] * np.float32(small), dtype)
+    q[(at == 0) | (at == 3)] /= np.float32(small)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, window=2)
+    check(out.numpy(), *reference(q, k, v, visible(b, 0, 2, 0)))
+
+
+@pytest.mark.parametrize("dtype,big", [("float32", 1e4), ("float32", 1e6), ("float32", 1e12), ("float16", 1e4),
+                                       ("bfloat16", 1e6)])
+@pytest.mark.parametrize("b,window", [(200, 30), (1600, 1000)])
+def test_large_keys_in_a_chunk(ops, ws, b, window, dtype, big):
+    """The rows before the middle of a chunk do not see its far larger key."""
+    T = ops.DevTensor
+    r = np.random.default_rng(23)
+    q, k, v = tensors(r, b, 0, 16, 8, dtype, extra=b)
+    k[:, b // 2] = rounded(np.clip(k[:, b // 2], -4, 4) * np.float32(big), dtype)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, window=window)
+    check(out.numpy(), *reference(q, k, v, visible(b, 0, window, 0)))
