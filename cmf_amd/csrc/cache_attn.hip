@@ -565,17 +565,18 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // no kl and vl), three products at 16 times the f32 MFMA's rate.
 //
 // f16 has 5 exponent bits, so operands of an unusual size are scaled by a power
-// of two first (exact): a key row or 8 keys' values at a time whose largest
-// magnitude is not in [2^-2, 2^6) to [2^2, 2^3), a query row always, to [2^14,
-// 2^15).  The keys' factor is undone in the scores, the values' in the weights
-// (2^(s - m + 6), m at most 8 below the maximum), relative to the largest
-// factor so far (the accumulated output follows when that grows).  What the
-// halves drop is then 2^-23 of an element or of its row's or group's largest:
-// a key's score depends on no other key.
-// A block of 32 keys that holds infinities, NaN, keys from 2^101 or below
-// 2^-100, or values 2^12 from the others' (anything in a row that some query
-// does not see) is left for a second walk without MFMAs, so that it reaches only
-// the queries that see it.
+// of two first (exact): a key row whose largest magnitude is not in [2^-2, 2^6)
+// to [2^2, 2^3), a query row always, to [2^14, 2^15), and the values of 8 keys by
+// one factor where their rows are alike (within 2^4), else by one a row.  A key's
+// factor is undone in its scores, a value's in its weights: they are 2^(s + f - m
+// + 6), f the factor's exponent and m, kept per query, at most 8 below the
+// largest s + f that the query sees.  What the halves drop is then 2^-23 of an
+// element or of its row's largest, and of a query's largest weighted value:
+// nothing that a query does not see takes part.
+// A block of 32 keys that holds infinities, NaN, keys outside [2^-100, 2^101) or
+// values outside [2^-50, 2^61) by their rows' largest (0 is none of these) is
+// left for a second walk without MFMAs, so that it reaches only the queries
+// that see it.
 //
 // S^T = K Q^T: a lane (query n = lane % 32, h = lane / 32) ends up with the
 // keys 8 a + 4 h + b of a 32-key block in register 4 a + b, which is the B
@@ -615,33 +616,32 @@ template <class T>
 struct Tile {
     static constexpr bool LO = sizeof(T) == 4;
     static constexpr int HALVES = LO ? 2 : 1, BUF = HALVES * (K_BYTES + V_BYTES);
-    // and of a block's groups: 8 codes of K and 4 exponents of V in 64 bytes, the
-    // key rows' factors
-    static constexpr int USE = 2 * (BUF + 128 + 4 * KT);
+    // and the codes of a block's groups (8 of K, 4 of V in 64 bytes), the key and
+    // value rows' factors
+    static constexpr int USE = 2 * (BUF + 128 + 8 * KT);
     static constexpr int LDS = USE > END_BYTES ? USE : END_BYTES;
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
 
 constexpr int SCHED_MFMA = 8, SCHED_LDS = 0x100;  // of sched_group_barrier: MFMAs, LDS reads
-// A group's scale 2^(PLAIN - e) by the largest magnitude of the wave's elements:
-// e = PLAIN where f16 halves take them as they are; all zeros; infinities, NaN
+// The scale of a row or group is 2^(PLAIN - e) by its largest magnitude: e =
+// PLAIN where f16 halves take it as it is; all zeros; infinities, NaN
 constexpr int PLAIN = 2, NO_EXP = -1000, BAD_EXP = 1000;
 // What a group of four key rows is: as it stands; rows with factors of their own;
-// something that halves and f32 scores between them cannot hold
-enum { ROWS_PLAIN = 0, ROWS_SCALED = 1, ROWS_ODD = 2 };
+// something that halves and f32 sums cannot hold.  One of eight value rows: its
+// exponent, or one of these
+enum { ROWS_PLAIN = 0, ROWS_SCALED = 500, ROWS_ODD = BAD_EXP };
+constexpr int ALIKE = 4;  // value rows within 2^ALIKE share a factor
 constexpr int KEY_RANGE = 100;  // exponents: scores by 2^-14 of a query's stay below 2^25+100, queries' factors normal
-constexpr int FAR = 12;  // values 2^FAR apart are not summed with each other's halves
+// value rows: a sum of weights and the weighted values by one maximum stay within
+// f32's range, and so do those of splits by the others' (2^(61 + 50) apart)
+constexpr int VALUE_MIN = -50, VALUE_MAX = 60;
 __device__ __forceinline__ int exponent_class(uint32_t u) {  // of a magnitude's bits
     const int e = (int)(u >> 23) - 127;
     return u >= 0x7f800000u ? BAD_EXP : u == 0 ? NO_EXP : e >= -2 && e < 6 ? PLAIN : e;
 }
-__device__ __forceinline__ int group_exponent(float mx) {
-    // (the ordinary case by two comparisons)
-    if (!__builtin_amdgcn_ballot_w64(!(mx < 64.f)) && __builtin_amdgcn_ballot_w64(mx >= 0.25f)) return PLAIN;
-    return exponent_class(__builtin_amdgcn_readfirstlane(wave_max_u32(__float_as_uint(mx))));
-}
 // Whether all lanes' magnitudes are below 2^6 and each 16 lanes hold one of
-// 2^-2 or more in a and in b.
+// 2^-2 or more in a and in b (most often all do, which is one comparison).
 __device__ __forceinline__ bool each16(uint64_t m) {
     m |= m >> 8;
     m |= m >> 4;
@@ -650,13 +650,38 @@ __device__ __forceinline__ bool each16(uint64_t m) {
     return (~m & 0x0001000100010001ull) == 0;
 }
 __device__ __forceinline__ bool rows16_plain(float a, float b) {
-    return !__builtin_amdgcn_ballot_w64(!(mag(a, b) < 64.f)) && each16(__builtin_amdgcn_ballot_w64(a >= 0.25f)) &&
+    const bool low = mag(a, b) < 64.f;
+    if (!__builtin_amdgcn_ballot_w64(!(low & (fminf(a, b) >= 0.25f)))) return true;
+    return !__builtin_amdgcn_ballot_w64(!low) && each16(__builtin_amdgcn_ballot_w64(a >= 0.25f)) &&
            each16(__builtin_amdgcn_ballot_w64(b >= 0.25f));
 }
 // whether the tiles cannot take a key row whose largest magnitude has class e
 __device__ __forceinline__ bool odd_key(int e) { return e == BAD_EXP || (e != NO_EXP && (e > KEY_RANGE || e < -KEY_RANGE)); }
+__device__ __forceinline__ bool odd_value(int e) { return e == BAD_EXP || (e != NO_EXP && (e > VALUE_MAX || e < VALUE_MIN)); }
+// The largest of each of eight registers over the wave, that of v[lane / 8] in
+// every lane.
+__device__ __forceinline__ uint32_t rows8_max(const float (&v)[8], int lane) {
+    uint32_t a[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), false, false);
+        a[i] = max(s[0], s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const auto s = __builtin_amdgcn_permlane16_swap(a[i], a[i + 2], false, false);
+        a[i] = max(s[0], s[1]);
+    }
+    auto step = [&](uint32_t x, auto ctrl) {
+        return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    const std::integral_constant<int, 0x128> ror8;
+    uint32_t r = lane & 8 ? step(a[1], ror8) : step(a[0], ror8);
+    r = step(r, std::integral_constant<int, 0xb1>{});      // quad_perm [1,0,3,2]
+    r = step(r, std::integral_constant<int, 0x4e>{});      // quad_perm [2,3,0,1]
+    return step(r, std::integral_constant<int, 0x141>{});  // row_half_mirror
+}
 __device__ __forceinline__ bool scaled(int e) { return e != PLAIN && e != NO_EXP; }
-__device__ __forceinline__ float group_scale(int e) { return pow2(PLAIN - e); }  // of a scaled one
 
 struct Split8 {
     half8 hi, lo;
@@ -698,8 +723,9 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     constexpr bool LO = Tile<T>::LO;
     constexpr int BUF = Tile<T>::BUF, KL = K_BYTES, VH = Tile<T>::HALVES * K_BYTES, VL = VH + V_BYTES;
     extern __shared__ __align__(16) uint8_t sm[];
-    int* texp = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: codes of 4 groups of K, exponents of 2 of V
-    float* kfac = (float*)(texp + 64);  // [buffer][key]: factors of the rows of groups with ROWS_SCALED
+    int* code_at = (int*)(sm + 2 * BUF);  // [buffer][block][h][8]: codes of 4 groups of K, 2 of V
+    // factors of the rows of groups with ROWS_SCALED: [buffer][key], and [buffer][group][8 values]
+    float *kfac = (float*)(code_at + 64), *vfac = kfac + 2 * KT;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 31, h = lane >> 5, nq = a.b * c.hpk;
     const bool part = (int)blockIdx.x >= c.whole;
@@ -714,6 +740,13 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     const KvRows<T> kv(a, ks, g);
     const int qg = wave & 3, kb = wave >> 2;  // the wave's queries and 32-key block
 
+    // the lane, where it is needed: addresses of what is seldom done are not worked
+    // out before the loop, which has no registers left for them
+    auto lane_here = []() {
+        int x;
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+        return x;
+    };
     // what thread t stages of a tile: dims 8 kd .. of keys kk and kk + 32, and
     // dims 2 lane, 2 lane + 1 of the keys vk + {0 .. 3, 8 .. 11} (the slots of
     // group (block, 16-key half, h) = wave)
@@ -806,7 +839,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     // 4 wave + 3 of both blocks (16 lanes a row) and the values of group `wave`.
     auto stage_k = [&](int at) {
         uint8_t* buf = sm + at * BUF;
-        int* te = texp + at * 32 + 8 * (wave & 1) + (wave >> 1);
+        int* te = code_at + at * 32 + 8 * (wave & 1) + (wave >> 1);
         float x[2][8], mx[2] = {0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 2; r++)
@@ -825,7 +858,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
                 const float f = sc ? pow2(PLAIN - e) : 1.f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[r][i] *= f;
-                if (kd == 0) kfac[at * KT + 32 * r + kk] = sc ? pow2(e - PLAIN) : 1.f;
+                const int lane1 = lane_here();
+                if (!(lane1 & 15)) kfac[at * KT + 32 * r + 4 * wave + (lane1 >> 4)] = sc ? pow2(e - PLAIN) : 1.f;
             }
         }
 #pragma unroll
@@ -839,20 +873,51 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     };
     auto stage_v = [&](int at) {
         uint8_t* buf = sm + at * BUF;
-        int* te = texp + at * 32;
-        float mx = 0.f;
+        // `all`: the largest of the lane's magnitudes; `each`: one that all eight
+        // rows reach (in one lane at least, where they are alike)
+        float x[2][8], all = 0.f, each = INFINITY;
+        auto largest = [&](int i) { return mag(fabsf(x[0][i]), x[1][i]); };
 #pragma unroll
-        for (int i = 0; i < 8; i++) mx = mag(mag(mx, vx[i].get(0)), vx[i].get(1));
-        const int e = group_exponent(mx);
-        float x[2][8];
+        for (int i = 0; i < 8; i++) {
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) x[j][i] = vx[i].get(j);
+            all = mag(all, largest(i));
+            each = fminf(each, largest(i));
+        }
+        int code = PLAIN;
+        if (!__builtin_amdgcn_ballot_w64(each >= 0.25f) || __builtin_amdgcn_ballot_w64(!(all < 64.f))) {
+            // one factor by the largest, if every row comes near it
+            const uint32_t u = __builtin_amdgcn_readfirstlane(wave_max_u32(__float_as_uint(all)));
+            code = u == 0 ? NO_EXP : u >= 0x7f800000u ? BAD_EXP : (int)(u >> 23) - 127;
+            bool alike = !odd_value(code);
+            const float least = alike ? pow2(code - ALIKE) : 0.f;
+            if (!__builtin_amdgcn_ballot_w64(each >= least)) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[j][i] = vx[i].get(j);
-        if (scaled(e)) {
-            const float f = group_scale(e);
+                for (int i = 0; i < 8; i++) alike &= __builtin_amdgcn_ballot_w64(largest(i) >= least) != 0;
+            }
+            if (alike) {
+                const float f = code == NO_EXP ? 1.f : pow2(PLAIN - code);
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i >> 3][i & 7] *= f;
+                for (int i = 0; i < 16; i++) x[i >> 3][i & 7] *= f;
+                code = max(code, VALUE_MIN);  // (zeros: the least weight, not to hold others down)
+            } else {
+                const int lane1 = lane_here();
+                float mx[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx[i] = largest(i);
+                const int e = exponent_class(rows8_max(mx, lane1));  // of row lane / 8
+                const bool sc = scaled(e) && !odd_value(e);
+                code = __builtin_amdgcn_ballot_w64(odd_value(e)) ? ROWS_ODD : ROWS_SCALED;
+                const uint32_t f = __float_as_uint(sc ? pow2(PLAIN - e) : 1.f);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float fi = __uint_as_float(__builtin_amdgcn_readlane(f, 8 * i));
+                    x[0][i] *= fi;
+                    x[1][i] *= fi;
+                }
+                if (!(lane1 & 7))
+                    vfac[at * KT + 8 * wave + (lane1 >> 3)] = sc ? pow2(e - PLAIN) : e == NO_EXP ? pow2(VALUE_MIN) : 1.f;
+            }
         }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -861,7 +926,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             *(half8*)(buf + VH + o) = s.hi;
             if (LO) *(half8*)(buf + VL + o) = s.lo;
         }
-        te[16 * (wave >> 2) + 8 * (wave & 1) + 4 + (wave >> 1 & 1)] = e;
+        code_at[at * 32 + 16 * (wave >> 2) + 8 * (wave & 1) + 4 + (wave >> 1 & 1)] = code;
     };
 
     float16v acc[4];
@@ -870,7 +935,6 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    int ev = NO_EXP;  // the values' exponent so far
     bool odd = false;
 
     constexpr int RD = LO ? 2 : 1, MM = LO ? 3 : 2;  // fragments read and products of a step
@@ -879,7 +943,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     // the scores of the wave's block of the tile at v0, in buffer `at`
     auto scores = [&](int v0, int at) {
         const uint8_t* buf = sm + at * BUF;
-        const int4 ek = *(const int4*)(texp + at * 32 + 16 * kb + 8 * h);
+        const int4 ek = *(const int4*)(code_at + at * 32 + 16 * kb + 8 * h);
         const uint8_t* kp = buf + (kb * 16 + h) * KFRAG + n * 16;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.f;
@@ -904,10 +968,11 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         kbad = false;
         if (__builtin_amdgcn_ballot_w64((ek.x | ek.y | ek.z | ek.w) != ROWS_PLAIN)) {
             kbad = __builtin_amdgcn_ballot_w64(max(max(ek.x, ek.y), max(ek.z, ek.w)) == ROWS_ODD) != 0;
+            const float* kf = kfac + at * KT + 32 * kb + 4 * (lane_here() >> 5);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int e = i == 0 ? ek.x : i == 4 ? ek.y : i == 8 ? ek.z : ek.w;
-                const float4v f = *(const float4v*)(kfac + at * KT + 32 * kb + 2 * i + 4 * h);
+                const float4v f = *(const float4v*)(kf + 2 * i);
 #pragma unroll
                 for (int b = 0; b < 4; b++) s[i + b] *= e == ROWS_SCALED ? f[b] : 1.f;
             }
@@ -927,60 +992,83 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     };
     // their weights and the values' sum, from buffer `at`
     auto values = [&](int at) {
-        const int2 ew = *(const int2*)(texp + at * 32 + 16 * kb + 8 * h + 4);
-        int follow = 0;
-        if (kbad || __builtin_amdgcn_ballot_w64((ew.x != ev) | (ew.y != ev))) {
-            // other scales than so far: all zeros, a new largest one (the output so
-            // far follows), or too far from it for the weights' halves
-            int hi = max(ew.x, ew.y), lo = min(ew.x == NO_EXP ? BAD_EXP : ew.x, ew.y == NO_EXP ? BAD_EXP : ew.y);
-            hi = max(ev, max(__builtin_amdgcn_readlane(hi, 0), __builtin_amdgcn_readlane(hi, 32)));
-            lo = min(ev == NO_EXP ? BAD_EXP : ev, min(__builtin_amdgcn_readlane(lo, 0), __builtin_amdgcn_readlane(lo, 32)));
-            if (kbad || hi == BAD_EXP || (lo < BAD_EXP && hi - lo > FAR)) {
-                odd = true;
-                return;
-            }
-            follow = ev == NO_EXP ? 0 : ev - hi;
-            ev = hi;
+        const int2 cv = *(const int2*)(code_at + at * 32 + 16 * kb + 8 * h + 4);
+        const bool groups = __builtin_amdgcn_ballot_w64(max(cv.x, cv.y) >= ROWS_SCALED) == 0;
+        if (kbad || (!groups && __builtin_amdgcn_ballot_w64(max(cv.x, cv.y) == ROWS_ODD))) {
+            odd = true;
+            return;
         }
-        // m is the largest score up to 2^LAZY: the sums follow only when a score
-        // passes that
-        float mx = s[0];
+        // exponents of the two groups' factors, or of registers 4 a .. 4 a + 3's values
+        float e0 = (float)(cv.x - PLAIN), e1 = (float)(cv.y - PLAIN);
+        auto exponents = [&](int a) {
+            const float4v f = *(const float4v*)(vfac + at * KT + 32 * kb + 8 * (lane_here() >> 5) + 16 * (a >> 1) + 4 * (a & 1));
+            float4v e;
 #pragma unroll
-        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-        mx = lanes2_max(mx) * cq;
-        if (follow || __builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
-            const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1)), f = ldexpf(al, follow);
+            for (int b = 0; b < 4; b++) e[b] = (a < 2 ? cv.x : cv.y) == ROWS_SCALED ? (float)exponent_of(f[b]) : a < 2 ? e0 : e1;
+            return e;
+        };
+        // m is the largest score (and exponent) up to 2^LAZY: the sums follow only
+        // when one passes that
+        float mx;
+        if (groups) {
+            float a = s[0], b = s[8];
+#pragma unroll
+            for (int i = 1; i < 8; i++) a = fmaxf(a, s[i]), b = fmaxf(b, s[8 + i]);
+            mx = fmaxf(fmaf(a, cq, e0), fmaf(b, cq, e1));
+        } else {
+            mx = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+                const float4v e = exponents(a);
+#pragma unroll
+                for (int b = 0; b < 4; b++) mx = fmaxf(mx, fmaf(s[4 * a + b], cq, e[b]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        mx = lanes2_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
+            const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1));
             l *= al;
 #pragma unroll
-            for (int d = 0; d < 4; d++) acc[d] *= f;
+            for (int d = 0; d < 4; d++) acc[d] *= al;
             m = m1;
         }
         const float m0 = m == -INFINITY ? 0.f : m;
-        float f = cq, ref = m0 - SHIFT;
-        if (__builtin_amdgcn_ballot_w64(fabsf(m0) > FAR_SCORE)) {
+        float f = cq, ref = m0 - SHIFT, own = 1.f;
+        if (!groups || __builtin_amdgcn_ballot_w64(fabsf(m0) > FAR_SCORE)) {
             // Far from 0 a score is rounded as the maximum was before that is taken
             // off: the largest is then 0, and not what the product's rounding left.
+            // The weights without their values' factors are summed here.
+            float lu = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float p = s[i] * cq;
-                asm("" : "+v"(p));  // (no fma)
-                s[i] = p - m0;
+            for (int a = 0; a < 4; a++) {
+                const float4v e = exponents(a);
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    float p = s[4 * a + b] * cq;
+                    asm("" : "+v"(p));  // (no fma)
+                    p -= m0;
+                    lu += __builtin_amdgcn_exp2f(p);
+                    s[4 * a + b] = p + e[b];
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            l = fmaf(lu, (float)(1 << (int)SHIFT), l);
             f = 1.f;
             ref = -SHIFT;
+            e0 = e1 = own = 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            // the weights in units of the values' scale, their sum in its own
-            const int e = u ? ew.y : ew.x, de = e == NO_EXP ? 0 : e - ev;
-            const float ru = ref - (float)de;
+            // the weights in units of the group's factor, their sum in its own
+            const float e = u ? e1 : e0, ru = ref - e;
             float x[8], lu = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], f, -ru));
                 lu += x[i];
             }
-            l = fmaf(lu, ldexpf(1.0f, -de), l);
+            l = fmaf(lu, own * __builtin_amdgcn_exp2f(-e), l);
             const Split8 w = split8<true>(x);
             const uint8_t* vp = sm + at * BUF + VH + (kb * 4 + u * 2 + h) * VGROUP + (n >> 4) * 1024 + (n & 15) * 16;
 #pragma unroll
@@ -1038,33 +1126,31 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         }
     }
 
-    // The wave's state into LDS, in the values' own units (row r = 8 a + 4 h + b
-    // of block d is dim 32 d + 16 (a % 2) + 8 h + 2 b + a / 2), the weights by
-    // 2^-(SHIFT + LAZY) so that sums of large values stay finite.
+    // The wave's state into LDS (row r = 8 a + 4 h + b of block d is dim 32 d + 16
+    // (a % 2) + 8 h + 2 b + a / 2), the weights by 2^-(SHIFT + LAZY) so that sums of
+    // large values stay finite.
     __syncthreads();
     float* so = (float*)sm + wave * 32 * OROW;
     float2* ml = (float2*)((float*)sm + 8 * 32 * OROW) + wave * 32;  // (m, l)
     const int lane1 = this_lane(), n1 = lane1 & 31, h1 = lane1 >> 5;
     {
-        const float un = ldexpf(ev > NO_EXP ? pow2(ev - PLAIN) : 1.f, -(int)(SHIFT + LAZY));
+        const float un = pow2(-(int)(SHIFT + LAZY));
 #pragma unroll
         for (int d = 0; d < 4; d++)
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 *(float2*)(so + n1 * OROW + 32 * d + 16 * (i >> 2) + 8 * h1 + 2 * (i & 3)) =
                     make_float2(acc[d][i] * un, acc[d][8 + i] * un);
-        l = ldexpf(lanes2_sum(l), -(int)(SHIFT + LAZY));  // (m and l: the same in both lanes of a query)
+        l = lanes2_sum(l) * un;  // (m and l: the same in both lanes of a query)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (odd) {
-        // The blocks left out: the wave walks its blocks again, with the scales
-        // that the first walk went through (es), and takes those it left key by
-        // key, in f32; lane (n, h) has half the dims of its query.
+        // The blocks left out: the wave walks its blocks again and takes those it
+        // left key by key, in f32; lane (n, h) has half the dims of its query.
         const Query w = query();
         const Sight see = sight_of(a, ks, w.row);
         const float* q = a.q + (size_t)w.row * a.ldq + (size_t)w.head * HD + 64 * h1;
         float* o = so + n1 * OROW + 64 * h1;
-        int es = NO_EXP;
 #pragma unroll 1
         for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
             float mk = 0.f, mv = 0.f;  // the largest of key and value row n of the block
@@ -1077,22 +1163,8 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
                     mv = mag(mv, to_f32(vp[u]));
                 }
             }
-            const bool bad = odd_key(exponent_class(__float_as_uint(mk)));
-            uint32_t um = __float_as_uint(mv);  // of its group: keys 16 u + 4 h1 + {0 .. 3, 8 .. 11}
-            um = max(um, (uint32_t)__shfl_xor((int)um, 1));
-            um = max(um, (uint32_t)__shfl_xor((int)um, 2));
-            um = max(um, (uint32_t)__shfl_xor((int)um, 8));
-            int hi = exponent_class(um), lo = hi == NO_EXP ? BAD_EXP : hi;
-            hi = max(hi, __shfl_xor(hi, 4));
-            lo = min(lo, __shfl_xor(lo, 4));
-            hi = max(hi, __shfl_xor(hi, 16));
-            lo = min(lo, __shfl_xor(lo, 16));
-            hi = max(es, __builtin_amdgcn_readfirstlane(hi));
-            lo = min(es == NO_EXP ? BAD_EXP : es, __builtin_amdgcn_readfirstlane(lo));
-            if (!__builtin_amdgcn_ballot_w64(bad) && hi != BAD_EXP && !(lo < BAD_EXP && hi - lo > FAR)) {
-                es = hi;
-                continue;
-            }
+            const bool bad = odd_key(exponent_class(__float_as_uint(mk))) || odd_value(exponent_class(__float_as_uint(mv)));
+            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
 #pragma unroll 1
             for (int kn = 0; kn < 32; kn++) {
                 const int v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));

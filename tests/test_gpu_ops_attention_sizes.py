@@ -116,3 +116,65 @@ def test_large_keys_in_a_chunk(ops, ws, b, window, dtype, big):
     out = filled(ops, q.shape)
     ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, window=window)
     check(out.numpy(), *reference(q, k, v, visible(b, 0, window, 0)))
+
+
+# ---- values ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("first,rest", [(1, 1e6), (1, 1e8), (1, 1e30), (1e-8, 1), (1e-12, 1), (1e-8, 1e8), (1e8, 1)])
+@pytest.mark.parametrize("b", [200, 1100])
+def test_a_first_value_of_another_size(ops, ws, b, first, rest, dtype):
+    """Row 0 sees its own value alone, which may be far smaller than all others."""
+    T = ops.DevTensor
+    r = np.random.default_rng(24)
+    q, k, v = tensors(r, b, 0, 16, 8, dtype, extra=b)
+    v *= np.float32(rest)
+    v[:, 0] *= np.float32(first / rest)
+    v = rounded(v, dtype)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws)
+    check(out.numpy(), *reference(q, k, v, visible(b, 0, 0, 0)))
+
+
+@pytest.mark.parametrize("dtype,big", [("float32", 1e3), ("float32", 1e6), ("float32", 1e25), ("bfloat16", 1e6),
+                                       ("float16", 1e4), ("float32", 1e-6), ("float32", 1e-25)])
+@pytest.mark.parametrize("b,window", [(100, 1), (2000, 1), (2000, 3)])
+def test_neighbours_with_values_of_another_size(ops, ws, b, window, dtype, big):
+    """Every fourth row of a chunk has values `big` times the others'; the rows
+    around it see it through a short window, or not at all."""
+    T = ops.DevTensor
+    r = np.random.default_rng(25)
+    q, k, v = tensors(r, b, 0, 16, 8, dtype, extra=b)
+    v[:, 1::4] = rounded(np.clip(v[:, 1::4], -4, 4) * np.float32(big), dtype)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, window=window)
+    check(out.numpy(), *reference(q, k, v, visible(b, 0, window, 0)))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("b,ctx", [(5, 300), (64, 900), (700, 900)])
+def test_rows_of_zeros(ops, ws, b, ctx, dtype):
+    """Keys and values of zeros (a position that was never written) among
+    others, and rows that see nothing but zeros."""
+    T = ops.DevTensor
+    r = np.random.default_rng(26)
+    q, k, v = tensors(r, b, ctx, 16, 4, dtype, extra=b)
+    v[:, ::3] = 0
+    k[:, ::5] = 0
+    v[:, :40] = k[:, :40] = 0
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx, window=ctx // 2, sinks=20)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, ctx // 2, 20)))
+
+
+@pytest.mark.parametrize("std", [0.02, 1e-4, 300.0])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_values_and_keys_of_one_other_size(ops, ws, std, dtype):
+    T = ops.DevTensor
+    r = np.random.default_rng(27)
+    b, ctx = 300, 1000
+    q, k, v = tensors(r, b, ctx, 16, 4, dtype, extra=b)
+    k, v = (rounded(t * np.float32(std), dtype) for t in (k, v))
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx)
+    want, tol = reference(q, k, v, visible(b, ctx, 0, 0))
+    check(out.numpy(), want, tol)
