@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 
     float4v acc[8];
     float m = -INFINITY, l = 0.f;
-    bool odd = false;
+    int odd_lo = 0, odd_hi = -1;  // the first and last tile left out
 #pragma unroll
     for (int i = 0; i < 8; i++) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
 
@@ -470,7 +470,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
                 }
             }
         } else {
-            odd = true;
+            if (odd_hi < 0) odd_lo = v0;
+            odd_hi = v0;
         }
         if (v0 + 16 * NW < v_hi) load(v0 + 16 * NW);
     }
@@ -489,27 +490,32 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
             so[wave][n][VP == 2 ? 64 * (i >> 2) + 4 * r + (i & 3) : 8 * r + i] = acc[i][e] * un;
         }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (odd) {
+    if (odd_hi >= 0) {
         // the tiles left out, key by key; lane (n, kq) has 32 dims of its query
 #pragma unroll 1
-        for (int v0 = v_lo + 16 * wave; v0 < v_hi; v0 += 16 * NW) {
-            bool bad = false;
-            {
-                const T* vp = kv.value(ks.pos(min(v0 + n, ks.nv - 1)));
-#pragma unroll 1
-                for (int u = 0; u < 32; u++) bad |= !(fabsf(to_f32(vp[32 * kq + u])) < INFINITY);
+        for (int v0 = odd_lo; v0 <= odd_hi; v0 += 16 * NW) {
+            const T* row = kv.value(ks.pos(min(v0 + n, ks.nv - 1))) + 32 * kq;
+            float mv = 0.f;
+#pragma unroll
+            for (int u = 0; u < 32; u += 8) {
+                Raw<T, 8> r;
+                r.load(row, u);
+#pragma unroll
+                for (int i = 0; i < 8; i++) mv = mag(mv, r.get(i));
             }
-            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+            if (!__builtin_amdgcn_ballot_w64(!(mv < INFINITY))) continue;
 #pragma unroll 1
             for (int k = 0; k < 16; k++) {
                 const int v = v0 + k, pos = ks.pos(min(v, ks.nv - 1));
+                const bool vis = sees(a, ks, see, pos) & (v < v_hi);
+                if (!__builtin_amdgcn_ballot_w64(vis)) continue;
                 const T *kp = kv.key(pos), *vp = kv.value(pos);
                 float d = 0.f;
 #pragma unroll 4
                 for (int u = 0; u < 32; u++) d = fmaf(q[32 * kq + u], to_f32(kp[32 * kq + u]), d);
                 d = lanes4_sum(d) * c.qscale;
                 asm("" : "+v"(d));  // (rounded before the maximum comes off: no fma)
-                if (!(sees(a, ks, see, pos) & (v < v_hi))) continue;
+                if (!vis) continue;
                 float* o = &so[wave][n][32 * kq];
                 const float m1 = fmaxf(m, d), ref = m1 == -INFINITY ? 0.f : m1;
                 const float al = exp2f(m - ref), wt = exp2f(d - ref - LAZY);
@@ -619,7 +625,7 @@ struct Tile {
     // and the codes of a block's groups (8 of K, 4 of V in 64 bytes), the key and
     // value rows' factors
     static constexpr int USE = 2 * (BUF + 128 + 8 * KT);
-    static constexpr int LDS = USE > END_BYTES ? USE : END_BYTES;
+    static constexpr int LDS = (USE > END_BYTES ? USE : END_BYTES) + 64;  // (and two numbers a wave)
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
 
@@ -936,6 +942,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     bool odd = false;
+    int* odd_at = (int*)(sm + Tile<T>::LDS - 64) + 2 * wave;  // the first and last tile with a block left out
 
     constexpr int RD = LO ? 2 : 1, MM = LO ? 3 : 2;  // fragments read and products of a step
     float16v s;         // the block's scores, by 1 / cq
@@ -991,10 +998,17 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         }
     };
     // their weights and the values' sum, from buffer `at`
-    auto values = [&](int at) {
+    auto values = [&](int v0, int at) {
         const int2 cv = *(const int2*)(code_at + at * 32 + 16 * kb + 8 * h + 4);
         const bool groups = __builtin_amdgcn_ballot_w64(max(cv.x, cv.y) >= ROWS_SCALED) == 0;
-        if (kbad || (!groups && __builtin_amdgcn_ballot_w64(max(cv.x, cv.y) == ROWS_ODD))) {
+        int left = kbad || (!groups && __builtin_amdgcn_ballot_w64(max(cv.x, cv.y) == ROWS_ODD));
+        if (left) {
+            if (!odd) odd_at[0] = v0;
+            odd_at[1] = v0;
+        }
+        // (a branch of its own: one for both costs the loop its registers)
+        left = __builtin_amdgcn_readfirstlane(left);
+        if (left) {
             odd = true;
             return;
         }
@@ -1114,7 +1128,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         for (int v0 = v_lo, at = 0; v0 < v_hi; v0 += KT, at ^= 1) {
             __syncthreads();  // this tile is whole, the other buffer free
             scores(v0, at);
-            values(at);
+            values(v0, at);
             next(v0, at);
         }
     } else {
@@ -1122,7 +1136,7 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             __syncthreads();
             next(v0, at);
             scores(v0, at);
-            values(at);
+            values(v0, at);
         }
     }
 
@@ -1145,30 +1159,33 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (odd) {
-        // The blocks left out: the wave walks its blocks again and takes those it
-        // left key by key, in f32; lane (n, h) has half the dims of its query.
+        // The blocks left out: the wave walks its blocks again, from the first to
+        // the last of them, and takes those it left key by key, in f32; lane (n, h)
+        // has half the dims of its query.
         const Query w = query();
         const Sight see = sight_of(a, ks, w.row);
         const float* q = a.q + (size_t)w.row * a.ldq + (size_t)w.head * HD + 64 * h1;
         float* o = so + n1 * OROW + 64 * h1;
+        const int v1 = __builtin_amdgcn_readfirstlane(odd_at[1]);
 #pragma unroll 1
-        for (int v0 = v_lo; v0 < v_hi; v0 += KT) {
-            float mk = 0.f, mv = 0.f;  // the largest of key and value row n of the block
-            {
-                const int pos = ks.pos(min(v0 + 32 * kb + n1, ks.nv - 1));
-                const T *kp = kv.key(pos), *vp = kv.value(pos);
-#pragma unroll 1
-                for (int u = 0; u < HD; u++) {
-                    mk = mag(mk, to_f32(kp[u]));
-                    mv = mag(mv, to_f32(vp[u]));
-                }
+        for (int v0 = __builtin_amdgcn_readfirstlane(odd_at[0]); v0 <= v1; v0 += KT) {
+            const int at_n = ks.pos(min(v0 + 32 * kb + n1, ks.nv - 1));
+            const T* row = h1 ? kv.value(at_n) : kv.key(at_n);
+            float mx = 0.f;  // the largest of key or value row n of the block
+#pragma unroll 4
+            for (int u = 0; u < HD; u += 8) {
+                Raw<T, 8> r;
+                r.load(row, u);
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx = mag(mx, r.get(i));
             }
-            const bool bad = odd_key(exponent_class(__float_as_uint(mk))) || odd_value(exponent_class(__float_as_uint(mv)));
-            if (!__builtin_amdgcn_ballot_w64(bad)) continue;
+            const int e = exponent_class(__float_as_uint(mx));
+            if (!__builtin_amdgcn_ballot_w64(h1 ? odd_value(e) : odd_key(e))) continue;
 #pragma unroll 1
             for (int kn = 0; kn < 32; kn++) {
                 const int v = v0 + 32 * kb + kn, pos = ks.pos(min(v, ks.nv - 1));
                 const bool vis = sees(a, ks, see, pos) & (v < v_hi);
+                if (!__builtin_amdgcn_ballot_w64(vis)) continue;
                 const T *kp = kv.key(pos), *vp = kv.value(pos);
                 float d = 0.f;
 #pragma unroll 4

@@ -178,3 +178,24 @@ def test_values_and_keys_of_one_other_size(ops, ws, std, dtype):
     ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx)
     want, tol = reference(q, k, v, visible(b, ctx, 0, 0))
     check(out.numpy(), want, tol)
+
+
+# ---- rows one by one -------------------------------------------------------
+@pytest.mark.parametrize("places", [[0], [70], [0, -1], [3, 64, 1000, 2999], [63, 64, 65, 127, 128, 2000, -1]])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("b,ctx,nh,nkv", [(5, 3001, 16, 8), (64, 3001, 64, 1), (900, 2500, 16, 8)])
+def test_odd_rows_here_and_there(ops, ws, b, ctx, nh, nkv, dtype, places):
+    """Rows that are gone through one by one: values of 1e30 or 1e-30, keys of
+    1e-33, and an infinite value that the last row alone sees."""
+    T = ops.DevTensor
+    r = np.random.default_rng(31)
+    q, k, v = tensors(r, b, ctx, nh, nkv, dtype, extra=b)
+    for i, at in enumerate(places):
+        t, f = ((v, 1e-30), (k, 1e-33), (v, 1e30))[i % 3]
+        t[:, at] *= np.float32(f)
+    k, v = rounded(k, dtype), rounded(v, dtype)
+    want, tol = reference(q, k, v, visible(b, ctx, 0, 0))
+    v[:, -1] = np.inf
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx)
+    check(out.numpy()[:-1], want[:-1], tol[:-1])
