@@ -78,7 +78,12 @@ __device__ __forceinline__ float mag(float m, float x) { return __builtin_elemen
 __device__ __forceinline__ int exponent_of(float x) {
     return x == 0.f ? 0 : (int)(__float_as_uint(x) >> 23 & 255) - 127;
 }
-// 2^n for any n (what f32 cannot hold ends at its largest power)
+// The least exponent that a query row is scaled by (to 2^14: f32 holds the factor
+// and what undoes it), and the least factor of the scores: not 0, a score that is
+// not seen is -inf.
+constexpr int QUERY_MIN = -112;
+constexpr float LEAST = 1.4e-45f;
+// 2^n (what f32 cannot hold ends at its largest power)
 __device__ __forceinline__ float pow2(int n) { return ldexpf(1.0f, max(-300, min(n, 127))); }
 
 // A call as the kernels take it.  An item is a block of queries of a kv head
@@ -365,10 +370,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
         float mx = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i++) mx = fmaxf(mx, fabsf(x[i]));
-        eq = exponent_of(lanes4_max(mx)) - 14;
+        eq = max(exponent_of(lanes4_max(mx)), QUERY_MIN) - 14;
         f *= pow2(-eq);
     }
-    cq = fmaxf(fabsf(ldexpf(c.qscale, eq)), 1e-37f);  // (not 0: a score that is not seen is -inf)
+    cq = fmaxf(fabsf(ldexpf(c.qscale, eq)), LEAST);
     if constexpr (F32) {
 #pragma unroll
         for (int i = 0; i < 32; i++) qf[i] = x[i] * f;
@@ -827,9 +832,9 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
 #pragma unroll
             for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[j][i]));
         }
-        const int eq = exponent_of(lanes2_max(mx));  // (an infinite or NaN query ends as NaN by itself)
+        const int eq = max(exponent_of(lanes2_max(mx)), QUERY_MIN);  // (an infinite or NaN query ends as NaN by itself)
         const float sc = c.qscale < 0.f ? -pow2(14 - eq) : pow2(14 - eq);
-        cq = fmaxf(fabsf(ldexpf(c.qscale, eq - 14)), 1e-37f);  // (not 0: a score that is not seen is -inf)
+        cq = fmaxf(fabsf(ldexpf(c.qscale, eq - 14)), LEAST);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
 #pragma unroll

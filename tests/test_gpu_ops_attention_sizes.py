@@ -180,6 +180,60 @@ def test_values_and_keys_of_one_other_size(ops, ws, std, dtype):
     check(out.numpy(), want, tol)
 
 
+# ---- the ends of the range -------------------------------------------------
+@pytest.mark.parametrize("size", [1e-33, 1e-30, 1e30, 1e33])
+@pytest.mark.parametrize("scale", [0.0, 1e-6])
+@pytest.mark.parametrize("b,ctx", [(4, 300), (64, 300), (300, 400)])
+def test_far_keys(ops, ws, b, ctx, size, scale):
+    """Keys of 1e33 (1e-33) against queries of 1e-33 (1e33): ordinary scores, or
+    small ones with a scale of 1e-6."""
+    T = ops.DevTensor
+    r = np.random.default_rng(28)
+    q, k, v = tensors(r, b, ctx, 8, 2, "float32", extra=b)
+    q, k = q / np.float32(size), k * np.float32(size)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k), T.of(v), out, ws, pos0=ctx, scale=scale)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, 0, 0), scale or HD ** -0.5))
+
+
+@pytest.mark.parametrize("b,ctx", [(4, 300), (64, 300), (1000, 400)])
+def test_queries_of_1e_37(ops, ws, b, ctx):
+    """and a scale that makes ordinary scores of them"""
+    T = ops.DevTensor
+    r = np.random.default_rng(32)
+    q, k, v = tensors(r, b, ctx, 8, 2, "float32", extra=b)
+    q, k = q * np.float32(1e-37), k * np.float32(1e29)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k), T.of(v), out, ws, pos0=ctx, scale=1e7)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, 0, 0), np.float32(1e7)))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [1e-33, 1e-25, 1e25, 1e33])
+@pytest.mark.parametrize("b,ctx", [(4, 300), (64, 300), (300, 400)])
+def test_far_values(ops, ws, b, ctx, size, dtype):
+    T = ops.DevTensor
+    r = np.random.default_rng(29)
+    q, k, v = tensors(r, b, ctx, 8, 2, dtype, extra=b)
+    v = rounded(v * np.float32(size), dtype)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, 0, 0)))
+
+
+@pytest.mark.parametrize("b,ctx,nh,nkv", [(2, 300, 4, 2), (64, 300, 16, 4)])
+def test_queries_at_the_end_of_the_range(ops, ws, b, ctx, nh, nkv):
+    """Queries down to 1e-38 against f16 keys: every score is 0 within f32, the
+    output the mean of the values."""
+    T = ops.DevTensor
+    r = np.random.default_rng(30)
+    q, k, v = tensors(r, b, ctx, nh, nkv, "float16", extra=b)
+    q *= np.float32(1e-38)
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k, "float16"), T.of(v, "float16"), out, ws, pos0=ctx, scale=1e4)
+    check(out.numpy(), *reference(q, k, v, visible(b, ctx, 0, 0), 1e4))
+
+
 # ---- rows one by one -------------------------------------------------------
 @pytest.mark.parametrize("places", [[0], [70], [0, -1], [3, 64, 1000, 2999], [63, 64, 65, 127, 128, 2000, -1]])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
