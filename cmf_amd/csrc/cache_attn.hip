@@ -1280,8 +1280,7 @@ __global__ __launch_bounds__(64) void k_attn_join(AttnCall c) {
 // the most keys that a block of rows may have to read
 long long keys_bound(const cmf_attention_args& a, int rows) {
     const long long cached = a.d_pos0 ? std::min(a.len_bound, a.slots) : a.pos0;
-    long long n = cached + (a.d_mask ? a.b : std::min(a.b, rows));
-    if (!a.d_mask && !a.d_depth && !a.d_pos0) n = cached + a.b;
+    long long n = cached + a.b;  // (a chunk's last block sees all of its rows)
     if (a.window) n = std::min(n, (long long)a.sinks + a.window + (a.d_mask || a.d_depth ? a.b : rows));
     return std::max(1ll, n);
 }
