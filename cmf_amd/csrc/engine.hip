@@ -198,6 +198,7 @@ struct cmf_model_s {
     // first positions that stay visible (cmf_model_set_window)
     int window = 0, sinks = 0;
     void* op_ws = nullptr;  // scratch of the windowed and the tree attention
+    bool block_failed = false;  // an attention of run_block was refused (blocks_check)
     TreeBufs tree;  // cmf_verify_tree's buffers (from its first call on)
     bool has_tree = false;
     float* sc_logits = nullptr;  // cmf_score: a batch of logit rows and its results
@@ -438,9 +439,12 @@ cmf_attention_args attention_args(cmf_model_s* m, const LayerDev& l, const float
 
 // Attention of nb projected rows at positions *pb + padd + i through the
 // window: norms, rotation and append, then what the rows see.  max_len bounds
-// the positions stored with the rows.
+// the positions stored with the rows.  (CMF_WINDOW_ATTN_FAIL=1 refuses it, to
+// test that path.)
 int window_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* q, float* ao, int nb, const int* pb, int padd,
                      int max_len, hipStream_t s) {
+    static const bool refuse = getenv("CMF_WINDOW_ATTN_FAIL") && getenv("CMF_WINDOW_ATTN_FAIL")[0] == '1';
+    if (refuse) return fail("windowed attention refused (CMF_WINDOW_ATTN_FAIL)");
     const auto& c = m->c;
     cmf_qk_rope_args r = rope_args(m, l, qkv, q, nb);
     r.k = l.kc;
@@ -479,7 +483,7 @@ void run_block(cmf_model_s* m, LayerDev& l, float* h, int nb, const int* pb, int
     // waits for a producer launch
     const bool win = windowed(m, max_len);
     const bool wo_planes = !win && l.wo.dtype == DT_Q8ROW && (nh * hd) % 64 == 0;
-    if (win) (void)window_attention(m, l, m->qkv_out, m->qrot, m->ao, nb, pb, padd, max_len, s);
+    if (win && window_attention(m, l, m->qkv_out, m->qrot, m->ao, nb, pb, padd, max_len, s) != CMF_OK) m->block_failed = true;
     for (int b0 = 0; b0 < nb && !win; b0 += rows_per) {
         AttnArgs at{m->qkv_out + (size_t)b0 * QKV, QKV, l.q_norm, l.k_norm, m->rope, l.kc, l.vc, c.max_seq,
                     std::min(rows_per, nb - b0), nh, nkv, c.eps, pb, padd + b0, m->pm, m->pl, m->po, m->nch_cap,
@@ -755,14 +759,11 @@ void ensure_prefill_moe(cmf_model_s* m, int n) {
 // Causal attention of cnt chunk rows (positions *pb + i) in groups the
 // attention kernel serves (at most 32 queries per kv head); attend = 0 only
 // appends their K/V (the MTP warm).
-void prefill_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* ao, int cnt, const int* pb, int p0,
-                       bool attend, hipStream_t s) {
+int prefill_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* ao, int cnt, const int* pb, int p0,
+                      bool attend, hipStream_t s) {
     const auto& c = m->c;
     const int hd = c.head_dim, nh = c.n_heads, nkv = c.n_kv, QKV = (nh + 2 * nkv) * hd;
-    if (attend && windowed(m, p0 + cnt)) {
-        (void)window_attention(m, l, qkv, m->pf_q, ao, cnt, pb, 0, p0 + cnt, s);
-        return;
-    }
+    if (attend && windowed(m, p0 + cnt)) return window_attention(m, l, qkv, m->pf_q, ao, cnt, pb, 0, p0 + cnt, s);
     static const bool tiled = !(getenv("CMF_PREFILL_ATTN") && getenv("CMF_PREFILL_ATTN")[0] == '0');
     if (tiled && prefill_attention_fits(nh, nkv, hd)) {
         // the whole chunk at once: the tiled prefill attention (one launch
@@ -771,7 +772,7 @@ void prefill_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* ao,
                            c.eps, m->pf_q, attend ? ao : nullptr, m->pf_khl, m->pf_part, m->pf_mcell, m->pf_cells, m->pf_err, ++m->pf_tag,
                            !m->pf_xcd_off};
         launch_prefill_attention(pa, s);
-        return;
+        return CMF_OK;
     }
     const int rows_per = std::min(MAXB, std::max(1, 32 / (nh / nkv)));
     for (int b0 = 0; b0 < cnt; b0 += rows_per) {
@@ -781,6 +782,7 @@ void prefill_attention(cmf_model_s* m, LayerDev& l, const float* qkv, float* ao,
                     attend ? m->nch_cap : 0, attend ? ao + (size_t)b0 * nh * hd : nullptr, attend ? 1 : 0};
         launch_attention(at, p0 + b0 + nb, s);
     }
+    return CMF_OK;
 }
 
 // The routed-expert FFN over cnt > 16 prefill rows of h: the router on all
@@ -819,7 +821,7 @@ int prefill_block(cmf_model_s* m, LayerDev& l, float* h, int cnt, const int* pb,
     const int H = c.hidden, hd = c.head_dim, nh = c.n_heads, QKV = (nh + 2 * c.n_kv) * hd, I = c.inter;
     int rc = gemm(l.qkv, src_norm(h, H, l.in_norm, c.eps), cnt, m->pf_qkv, QKV, false, s);
     if (rc != CMF_OK) return rc;
-    prefill_attention(m, l, m->pf_qkv, m->pf_ao, cnt, pb, p0, true, s);
+    if ((rc = prefill_attention(m, l, m->pf_qkv, m->pf_ao, cnt, pb, p0, true, s)) != CMF_OK) return rc;
     XSrc ra{};
     ra.mode = XS_ROWS;
     ra.x = m->pf_ao;
@@ -1120,6 +1122,15 @@ static int xl_check(cmf_model m) {
     }
     return CMF_OK;
 }
+// After a call that ran run_block: an attention that was refused left earlier
+// rows in its place, in captured rounds too.
+static int blocks_check(cmf_model m) {
+    if (!m->block_failed) return CMF_OK;
+    m->block_failed = false;
+    m->decoding = false;
+    drop_graph(m);
+    return CMF_ERR;  // (with the refusal's message)
+}
 // The decode state and tip hidden before a call that may have to run again.
 struct XlSnap {
     DState st;
@@ -1231,7 +1242,7 @@ static int prefill_impl(cmf_model m, const int32_t* ids, int n, const ScoreOut* 
                 if (gemm(m->eh, src_cat(m, m->pf_toks, m->pf_h), pairs, m->pf_hm, H, false, s) ||
                     gemm(m->mtp.qkv, src_norm(m->pf_hm, H, m->mtp.in_norm, c.eps), pairs, m->pf_qkv, QKV, false, s))
                     return CMF_ERR;
-                prefill_attention(m, m->mtp, m->pf_qkv, nullptr, pairs, pb, p0, false, s);
+                if (prefill_attention(m, m->mtp, m->pf_qkv, nullptr, pairs, pb, p0, false, s) != CMF_OK) return CMF_ERR;
             }
         }
         if (p0 + cnt == n)
@@ -1498,6 +1509,7 @@ static int decode_rounds_impl(cmf_model m, int n, int spec, int k, cmf_gen_stats
     CMF_HIP(hipEventElapsedTime(&ms, e0, e1));
     (void)hipEventDestroy(e0);
     (void)hipEventDestroy(e1);
+    if (blocks_check(m) != CMF_OK) return CMF_ERR;
     const int xc = xl_check(m);
     if (xc != CMF_OK) return xc;
     m->next_pos_host = hs.next_pos;
@@ -1729,6 +1741,7 @@ static int forward_batch_impl(cmf_model m, const int32_t* tokens, int b, int pos
     hipLaunchKernelGGL(k_set_int, dim3(1), dim3(1), 0, s, pb, pos0 + b);
     CMF_HIP(hipStreamSynchronize(s));
     CMF_HIP(hipGetLastError());
+    if (blocks_check(m) != CMF_OK) return CMF_ERR;
     const int xc = xl_check(m);
     if (xc != CMF_OK) return xc;
     m->next_pos_host = pos0 + b;
@@ -1800,6 +1813,7 @@ static int verify_step_impl(cmf_model m, const int32_t* tokens, int b, int pos0,
     CMF_HIP(hipMemcpyAsync(&hs, m->st, sizeof(DState), hipMemcpyDeviceToHost, s));
     CMF_HIP(hipStreamSynchronize(s));
     CMF_HIP(hipGetLastError());
+    if (blocks_check(m) != CMF_OK) return CMF_ERR;
     const int xc = xl_check(m);
     if (xc != CMF_OK) return xc;
     m->next_pos_host = hs.next_pos;
