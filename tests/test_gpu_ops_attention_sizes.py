@@ -253,3 +253,43 @@ def test_odd_rows_here_and_there(ops, ws, b, ctx, nh, nkv, dtype, places):
     out = filled(ops, q.shape)
     ops.attention(T.of(q), T.of(k, dtype), T.of(v, dtype), out, ws, pos0=ctx)
     check(out.numpy()[:-1], want[:-1], tol[:-1])
+
+
+# ---- a first call that is captured ----------------------------------------
+FIRST = """
+import ctypes as C
+import numpy as np
+import cmf_amd
+from cmf_amd import ops
+cmf_amd.init(0)
+T = ops.DevTensor
+r = np.random.default_rng(1)
+n, nh, nkv = 300, 16, 4
+q, k, v = (T.of(r.standard_normal(s, dtype=np.float32)) for s in ((n, nh, 128), (nkv, n, 128), (nkv, n, 128)))
+out, eager, ws = T.of(np.zeros((n, nh, 128), np.float32)), T.empty((n, nh, 128)), T.empty(64 << 20, "uint8")
+hip = C.CDLL("libamdhip64.so.7")
+ok = lambda rc: rc and exit(f"HIP error {rc}")
+s, g, e = C.c_void_p(), C.c_void_p(), C.c_void_p()
+cmf_amd.check(cmf_amd.lib().cmf_sync())
+ok(hip.hipStreamCreateWithFlags(C.byref(s), 1))
+ok(hip.hipStreamBeginCapture(s, MODE))
+ops.attention(q, k, v, out, ws, stream=s.value)
+ok(hip.hipStreamEndCapture(s, C.byref(g)))
+ok(hip.hipGraphInstantiate(C.byref(e), g, None, None, C.c_size_t(0)))
+ops.attention(q, k, v, eager, ws)
+want = eager.numpy()
+for i in range(3):
+    out.buf.upload(np.full((n, nh, 128), 3, np.float32))
+    ok(hip.hipGraphLaunch(e, s))
+    ok(hip.hipStreamSynchronize(s))
+    assert np.array_equal(out.numpy(), want)
+print("done")
+"""
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+def test_a_first_call_may_be_captured(gpu, mode):
+    """In a process that has made no call before, and in every capture mode."""
+    r = subprocess.run([sys.executable, "-c", FIRST.replace("MODE", str(mode))], cwd=ROOT,
+                       env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stdout[-300:] + r.stderr[-1500:]
