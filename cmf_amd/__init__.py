@@ -150,6 +150,7 @@ SIGNATURES = {
     "cmf_last_error": (C.c_char_p, []),
     "cmf_init": (_I, [_I]),
     "cmf_device_count": (_I, []),
+    "cmf_device": (_I, []),
     "cmf_sync": (_I, []),
     "cmf_weight_upload": (_I, [_P, _S, _I, _I, _I, C.POINTER(_P)]),
     "cmf_weight_upload_q8": (_I, [_P, _P, _I, _I, C.POINTER(_P)]),

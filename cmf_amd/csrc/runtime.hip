@@ -366,6 +366,11 @@ int cmf_device_count(void) {
     return n;
 }
 
+int cmf_device(void) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return g_init ? g_dev : -1;
+}
+
 int cmf_init(int dev) {
     std::lock_guard<std::mutex> lk(g_mu);
     if (g_init) return CMF_OK;

@@ -6,13 +6,15 @@ probabilities.
 The functions take device tensors by their pointers: anything with data_ptr(),
 shape, stride() and dtype, as DevTensor below or torch tensors (a process that
 uses torch on the GPU imports it before this library is loaded: both bring a
-HIP runtime, and the first one serves both).  Head rows have 128 elements and
-are contiguous; activations are f32, caches and logits f32, f16 or bf16.
-Nothing is allocated, checked on the device or waited for; outputs are written
-in place.  stream: None for the calling thread's library stream
-(cmf_amd.lib().cmf_sync() waits for it), or a HIP stream handle (torch:
-stream.cuda_stream; 0 is the null stream).  Raises CmfError when the library
-refuses the arguments.
+HIP runtime, and the first one serves both).  They lie on the library's device
+(cmf_init's, else 0): a tensor whose get_device() says otherwise is refused.
+Head rows have 128 elements and are contiguous; activations are f32, caches and
+logits f32, f16 or bf16.  Nothing is allocated, checked on the device or waited
+for; outputs are written in place.  stream: None for the calling thread's
+library stream (cmf_amd.lib().cmf_sync() waits for it), or a HIP stream handle
+(torch: stream.cuda_stream; 0 is the null stream).  The library's stream waits
+for no other one: tensors that torch's work still reads or writes go with
+torch's stream.  Raises CmfError when the library refuses the arguments.
 """
 import ctypes as C
 import struct
@@ -57,6 +59,9 @@ class DevTensor:
         strides = [int(np.prod(shape[i + 1:], dtype=np.int64)) for i in range(len(shape))]
         n = int(np.prod(shape, dtype=np.int64))
         return cls(DevBuf(max(16, n * cls.SIZES[dtype])), shape, strides, dtype)
+
+    def get_device(self):
+        return _device_of_library()
 
     def data_ptr(self):
         return self.buf.p + self.offset * self.element_size()
@@ -117,8 +122,30 @@ def _dt(t):
         raise CmfError(f"dtype {t.dtype}: f32, f16 or bf16") from None
 
 
+_device = None  # the library's, once it has one
+
+
+def _device_of_library():
+    global _device
+    if _device is None:
+        d = lib().cmf_device()
+        if d < 0:
+            return 0  # (what the first call will take)
+        _device = d
+    return _device
+
+
 def _p(t):
-    return 0 if t is None else t.data_ptr()
+    if t is None:
+        return 0
+    try:
+        d = t.get_device()
+    except AttributeError:  # (a pointer and a layout, no more)
+        return t.data_ptr()
+    if d != _device and d != _device_of_library():
+        raise CmfError(f"a tensor {'of device %d' % d if d >= 0 else 'on the host'}: the library's device is "
+                       f"{_device_of_library()}")
+    return t.data_ptr()
 
 
 def _stream(s):
@@ -283,6 +310,7 @@ def kv_copy(dst_ptrs, src_ptrs, dst, src, *, n, pos0=0, idx=None, n_dev=None, po
     nbuf = dst_ptrs.shape[0]
     if src_ptrs.shape[0] != nbuf:
         raise CmfError("as many buffers on both sides")
+    _p(dst), _p(src)  # (on the library's device, as the other buffers)
     if idx is not None:
         _i32(idx, n, "idx")
     if n_dev is not None:

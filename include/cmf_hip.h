@@ -37,6 +37,8 @@ const char* cmf_last_error(void);
  * backend selection of gpu.rs:866-936.  Idempotent. */
 int cmf_init(int device);
 int cmf_device_count(void);
+/* The device that cmf_init selected, -1 before. */
+int cmf_device(void);
 /* Wait for all work on the calling thread's stream. */
 int cmf_sync(void);
 

@@ -1,0 +1,81 @@
+"""What cmf_amd.ops takes for a tensor, before any device is touched: layouts and
+devices by stand-ins that hold no memory."""
+import pytest
+
+import cmf_amd
+from cmf_amd import ops
+
+
+class Tensor:
+    """A contiguous tensor that says where it lies, at a pointer that is never
+    followed."""
+
+    def __init__(self, *shape, dtype="float32", device=0, strides=None):
+        self.shape, self.dtype, self.device = shape, dtype, device
+        st, n = [], 1
+        for s in reversed(shape):
+            st.insert(0, n)
+            n *= s
+        self.strides = tuple(strides or st)
+
+    def data_ptr(self):
+        return 4096
+
+    def stride(self):
+        return self.strides
+
+    def element_size(self):
+        return {"float32": 4, "uint8": 1}.get(self.dtype, 8)
+
+    def get_device(self):
+        return self.device
+
+
+def rope(where):
+    t = {n: Tensor(*s) for n, s in dict(qkv=(2, 8, 128), q=(2, 4, 128), k=(2, 16, 128), v=(2, 16, 128), q_norm=(128,),
+                                        k_norm=(128,), rope=(64, 64, 2)).items()}
+    t.update(depth=Tensor(2, dtype="int32"), pos0_dev=Tensor(1, dtype="int32"))
+    return ops.qk_rope, t, where
+
+
+def attention(where):
+    t = {n: Tensor(*s) for n, s in dict(q=(2, 4, 128), k=(2, 16, 128), v=(2, 16, 128), out=(2, 4, 128), k_new=(2, 2, 128),
+                                        v_new=(2, 2, 128)).items()}
+    t.update(ws=Tensor(64, dtype="uint8"), mask=Tensor(2, dtype="int64"), depth=Tensor(2, dtype="int32"),
+             pos0_dev=Tensor(1, dtype="int32"))
+    return ops.attention, t, where
+
+
+def copy(where):
+    t = dict(dst=Tensor(2, 16, 128), src=Tensor(2, 16, 128))
+    t.update({n: Tensor(3, dtype="int64") for n in ("dst_ptrs", "src_ptrs")})
+    t.update({n: Tensor(4, dtype="int32") for n in ("idx", "n_dev", "pos0_dev")}, n=4)
+    return ops.kv_copy, t, where
+
+
+def scores(where):
+    t = dict(logits=Tensor(3, 100), target=Tensor(3, dtype="int32"), logprob=Tensor(3), entropy=Tensor(3),
+             top_ids=Tensor(3, 5, dtype="int32"), top_lp=Tensor(3, 5), ws=Tensor(64, dtype="uint8"))
+    return ops.logprobs, t, where
+
+
+CALLS = [f(n) for f, names in (
+    (rope, "qkv q k v q_norm k_norm rope depth pos0_dev"), (attention, "q k v out k_new v_new ws mask depth pos0_dev"),
+    (copy, "dst src dst_ptrs src_ptrs idx n_dev pos0_dev"), (scores, "logits target logprob entropy top_ids top_lp ws"),
+) for n in names.split()]
+
+
+@pytest.mark.parametrize("device,word", [(-1, "on the host"), (1, "of device 1"), (7, "of device 7")])
+@pytest.mark.parametrize("call,tensors,name", CALLS, ids=[f"{c.__name__}-{n}" for c, _, n in CALLS])
+def test_tensors_of_another_device_are_refused(call, tensors, name, device, word):
+    args = dict(tensors, **{name: Tensor(*tensors[name].shape, dtype=tensors[name].dtype, device=device)})
+    with pytest.raises(cmf_amd.CmfError, match=word):
+        call(**args)
+
+
+def test_the_workspace_of_host_tensors_is_refused():
+    k = Tensor(2, 16, 128, device=-1)
+    with pytest.raises(cmf_amd.CmfError, match="on the host"):
+        ops.attention_workspace(Tensor(2, 4, 128), k, k, pos0=3)
+    with pytest.raises(cmf_amd.CmfError, match="on the host"):
+        ops.logprobs_workspace(Tensor(3, 100, device=-1))
