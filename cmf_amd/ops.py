@@ -187,9 +187,15 @@ def _f32(t, what):
         raise CmfError(f"{what} must be f32")
 
 
+def _vector(t, n):
+    """Whether t holds n elements in a row (one: without a dimension, too)."""
+    shape = t.shape
+    return n <= shape[0] and (t.stride()[0] == 1 or shape[0] == 1) if len(shape) == 1 else n <= 1 and not len(shape)
+
+
 def _i32(t, n, what):
-    if not (_name(t) == "int32" and t.stride()[-1] == 1 and t.shape[0] >= n):
-        raise CmfError(f"{what} must be int32, contiguous, of at least {n}")
+    if not (_name(t) == "int32" and _vector(t, n)):
+        raise CmfError(f"{what} must be int32, one-dimensional and contiguous, of at least {n}")
 
 
 def _cache(k, v, what):
@@ -255,7 +261,7 @@ def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, s
         nk, rows, nhst, nrst = _cache(k_new, v_new, "k_new / v_new")
         if nk != nkv or rows < b or k_new.dtype != k.dtype:
             raise CmfError("k_new / v_new must hold b rows of k's type")
-    if mask is not None and not (_name(mask) in ("int64", "uint64") and mask.shape[0] >= b and mask.stride()[0] == 1):
+    if mask is not None and not (_name(mask) in ("int64", "uint64") and _vector(mask, b)):
         raise CmfError("mask must be [b] of 64 bits")
     if depth is not None:
         _i32(depth, b, "depth")
@@ -329,7 +335,7 @@ def _logprobs_args(logits, target, logprob, entropy, top_ids, top_lp, top_k, ws,
     if target is not None:
         _i32(target, rows, "target")
     for t, w in ((logprob, "logprob"), (entropy, "entropy")):
-        if t is not None and not (_name(t) == "float32" and t.shape[0] >= rows and t.stride()[0] == 1):
+        if t is not None and not (_name(t) == "float32" and _vector(t, rows)):
             raise CmfError(f"{w} must be f32, [rows]")
     for t, w, d in ((top_ids, "top_ids", "int32"), (top_lp, "top_lp", "float32")):
         if t is not None and not (_name(t) == d and len(t.shape) == 2 and t.shape[0] >= rows and t.shape[1] == top_k and

@@ -79,3 +79,44 @@ def test_the_workspace_of_host_tensors_is_refused():
         ops.attention_workspace(Tensor(2, 4, 128), k, k, pos0=3)
     with pytest.raises(cmf_amd.CmfError, match="on the host"):
         ops.logprobs_workspace(Tensor(3, 100, device=-1))
+
+
+# (a call that passes the checks of its tensors ends at the library's own: no
+# depth without a mask, no target without a result)
+@pytest.mark.parametrize("ok,tensor", [
+    (True, Tensor(2, dtype="int32")), (True, Tensor(5, dtype="int32")), (False, Tensor(1, dtype="int32")),
+    (False, Tensor(2, dtype="int64")), (False, Tensor(2, dtype="int32", strides=(2,))), (False, Tensor(2, 3, dtype="int32")),
+    (False, Tensor(2, 1, dtype="int32")), (False, Tensor(dtype="int32"))])
+def test_vectors(ok, tensor):
+    t = attention("q")[1]
+    with pytest.raises(cmf_amd.CmfError, match="d_mask" if ok else "depth must be"):
+        ops.attention(t["q"], t["k"], t["v"], t["out"], t["ws"], depth=tensor)
+    t = scores("logits")[1]
+    with pytest.raises(cmf_amd.CmfError, match="together" if ok else "target must be"):
+        ops.logprobs(Tensor(2, 100), tensor, None, t["entropy"])
+
+
+@pytest.mark.parametrize("ok,tensor", [
+    (True, Tensor(dtype="int32")), (True, Tensor(1, dtype="int32")), (True, Tensor(1, dtype="int32", strides=(7,))),
+    (False, Tensor(0, dtype="int32")), (False, Tensor(dtype="float32")), (False, Tensor(1, 1, dtype="int32"))])
+def test_a_position_on_the_device(ok, tensor):
+    """one number, with a dimension or without"""
+    t = attention("q")[1]
+    with pytest.raises(cmf_amd.CmfError, match="len_bound past" if ok else "pos0_dev must be"):
+        ops.attention(t["q"], t["k"], t["v"], t["out"], t["ws"], pos0_dev=tensor, len_bound=16)
+
+
+@pytest.mark.parametrize("ok,tensor", [
+    (True, Tensor(2, dtype="int64")), (True, Tensor(9, dtype="uint64")), (False, Tensor(1, dtype="int64")),
+    (False, Tensor(2, 2, dtype="int64")), (False, Tensor(2, dtype="int64", strides=(2,))), (False, Tensor(2, dtype="int32"))])
+def test_masks(ok, tensor):
+    t = attention("q")[1]
+    with pytest.raises(cmf_amd.CmfError, match="needs d_depth" if ok else "mask must be"):
+        ops.attention(t["q"], t["k"], t["v"], t["out"], t["ws"], mask=tensor, window=3)
+
+
+@pytest.mark.parametrize("ok,tensor", [(True, Tensor(2)), (False, Tensor(1)), (False, Tensor(2, strides=(3,))),
+                                       (False, Tensor(2, 4)), (False, Tensor(2, dtype="float16"))])
+def test_results(ok, tensor):
+    with pytest.raises(cmf_amd.CmfError, match="together" if ok else "logprob must be"):
+        ops.logprobs(Tensor(2, 100), None, tensor)
