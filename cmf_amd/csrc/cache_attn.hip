@@ -1465,6 +1465,8 @@ int cmf_attention_dev(const cmf_attention_args* p) {
     if (!a.q || !a.out || ((!a.k || !a.v) && (a.slots > 0 || !a.k_new))) return fail("attention: null q, out, k or v");
     for (const void* x : {(const void*)a.q, (const void*)a.out, a.k, a.v, a.k_new, a.v_new, (const void*)a.ws})
         if (!aligned16(x)) return fail("attention: 16-byte aligned tensors");
+    // (a block of rows may write before another has read)
+    if (a.out == a.q && a.ldo != a.ldq) return fail("attention: out may be q with the same row stride (ldo = ldq)");
     OpScope sc;
     if (sc.enter(a.stream, "attention") != CMF_OK) return CMF_ERR;
     if (launch_cache_attention(a, sc.s) != CMF_OK) return CMF_ERR;

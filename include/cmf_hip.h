@@ -471,7 +471,7 @@ int cmf_qk_rope_dev(const cmf_qk_rope_args* a);
  * A row that sees nothing gets zeros.  What a row does not see may hold
  * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  At most 2^19
  * rows, 4096 query heads, 64 of them on a kv head, 2^30 positions, row strides
- * of 2^22 elements; more is refused.  out may be q.  ws: scratch of
+ * of 2^22 elements; more is refused.  out may be q (ldo = ldq).  ws: scratch of
  * at least cmf_attention_workspace bytes (at most 64 MiB) that no other call
  * uses meanwhile; captured graphs that may run at the same time need one
  * each. */

@@ -120,3 +120,10 @@ def test_masks(ok, tensor):
 def test_results(ok, tensor):
     with pytest.raises(cmf_amd.CmfError, match="together" if ok else "logprob must be"):
         ops.logprobs(Tensor(2, 100), None, tensor)
+
+
+def test_an_output_over_queries_of_another_stride_is_refused():
+    q = Tensor(2, 4, 128, strides=(1024, 128, 1))
+    k = Tensor(2, 16, 128)
+    with pytest.raises(cmf_amd.CmfError, match="ldo = ldq"):
+        ops.attention(q, k, k, Tensor(2, 4, 128), None)
