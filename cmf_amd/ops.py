@@ -222,14 +222,22 @@ def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=
     [nkv][slots][128], rope [positions][64][2] (cos, sin).  Row i at position
     pos0 + depth[i] (depth None: i; pos0_dev: an int32 tensor whose value is
     added); its key and value go to row pos0 + i, or row i with
-    at_pos=False."""
+    at_pos=False.  q None: keys and values only; k and v None: queries only."""
     b, hs, ldq = _rows(qkv, "qkv")
-    nkv, slots, hst, rst = _cache(k, v, "k / v")
-    bq, nh, ldo = _rows(q, "q")
-    if not (bq == b and hs == nh + 2 * nkv):
+    if (q is None and k is None) or (k is None) != (v is None):
+        raise CmfError("q, or k and v")
+    f32, bq, ldo, slots, hst, rst = qkv.dtype, b, 0, 0, 0, 0
+    if k is not None:
+        nkv, slots, hst, rst = _cache(k, v, "k / v")
+    if q is not None:
+        bq, nh, ldo = _rows(q, "q")
+    if q is None:
+        nh = hs - 2 * nkv
+    elif k is None:
+        nkv = (hs - nh) // 2
+    if not (bq == b and hs == nh + 2 * nkv and nh > 0 and nkv > 0):
         raise CmfError("qkv must hold nh + 2 nkv heads of every row of q")
-    f32 = qkv.dtype
-    if _name(qkv) != "float32" or q.dtype != f32 or rope.dtype != f32:
+    if _name(qkv) != "float32" or (q is not None and q.dtype != f32) or rope.dtype != f32:
         raise CmfError("qkv, q and rope must be f32")
     for t in (q_norm, k_norm):
         if t is not None and not (t.dtype == f32 and t.shape == (128,) and t.stride()[0] == 1):
@@ -242,7 +250,7 @@ def qk_rope(qkv, q, k, v, q_norm, k_norm, rope, *, pos0=0, pos0_dev=None, depth=
     if pos0_dev is not None:
         _i32(pos0_dev, 1, "pos0_dev")
     check(_qk_rope((_p(qkv), _p(q), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(rope), _p(pos0_dev), _p(depth), eps, hst, rst,
-                    b, nh, nkv, ldq, ldo, _dt(k), positions, pos0, slots, 1 if at_pos else 0, _stream(stream))))
+                    b, nh, nkv, ldq, ldo, 0 if k is None else _dt(k), positions, pos0, slots, 1 if at_pos else 0, _stream(stream))))
 
 
 def _attention_args(q, k, v, out, ws, pos0, k_new, v_new, mask, depth, window, sinks, scale, pos0_dev, len_bound, stream):

@@ -127,3 +127,16 @@ def test_an_output_over_queries_of_another_stride_is_refused():
     k = Tensor(2, 16, 128)
     with pytest.raises(cmf_amd.CmfError, match="ldo = ldq"):
         ops.attention(q, k, k, Tensor(2, 4, 128), None)
+
+
+@pytest.mark.parametrize("q,k,v,word", [
+    (None, None, None, "q, or k and v"), (Tensor(2, 4, 128), Tensor(2, 16, 128), None, "q, or k and v"),
+    (Tensor(2, 4, 128), None, Tensor(2, 16, 128), "q, or k and v"), (Tensor(2, 5, 128), None, None, "qkv must hold"),
+    (Tensor(2, 8, 128), None, None, "qkv must hold"), (Tensor(3, 4, 128), None, None, "qkv must hold"),
+    (None, Tensor(4, 16, 128), Tensor(4, 16, 128), "qkv must hold"), (Tensor(2, 4, 128, dtype="float16"), None, None, "f32"),
+    # (these are in order up to the library's own check of the positions)
+    (Tensor(2, 4, 128), None, None, "positions"), (None, Tensor(2, 100, 128), Tensor(2, 100, 128), "positions"),
+    (Tensor(2, 6, 128), Tensor(1, 100, 128), Tensor(1, 100, 128), "positions")])
+def test_queries_or_keys_alone(q, k, v, word):
+    with pytest.raises(cmf_amd.CmfError, match=word):
+        ops.qk_rope(Tensor(2, 8, 128), q, k, v, None, None, Tensor(64, 64, 2), pos0=63)
