@@ -74,6 +74,8 @@ class DevTensor:
 
     def __getitem__(self, key):
         key = key if isinstance(key, tuple) else (key,)
+        if len(key) > len(self.shape):
+            raise IndexError(f"{len(key)} indices for {len(self.shape)} dimensions")
         shape, strides, off = [], [], self.offset
         for i, (n, st) in enumerate(zip(self.shape, self._strides)):
             k = key[i] if i < len(key) else slice(None)
@@ -83,6 +85,8 @@ class DevTensor:
                 shape.append(max(0, -(-(hi - lo) // step)))
                 strides.append(st * step)
             else:
+                if not -n <= k < n:
+                    raise IndexError(f"index {k} of {n}")
                 off += (k % n) * st
         return DevTensor(self.buf, shape, strides, self.dtype, off)
 

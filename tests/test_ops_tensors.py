@@ -140,3 +140,13 @@ def test_an_output_over_queries_of_another_stride_is_refused():
 def test_queries_or_keys_alone(q, k, v, word):
     with pytest.raises(cmf_amd.CmfError, match=word):
         ops.qk_rope(Tensor(2, 8, 128), q, k, v, None, None, Tensor(64, 64, 2), pos0=63)
+
+
+def test_views_of_a_device_tensor():
+    t = ops.DevTensor(None, (3, 5, 128), (640, 128, 1), "float32")
+    assert t[2].offset == t[-1].offset == 1280 and t[2].shape == (5, 128)
+    v = t[1:, ::2, 4]
+    assert v.shape == (2, 3) and v.stride() == (640, 256) and v.offset == 644
+    for key in (3, -4, (0, 5), (0, 0, 128), (0, 0, 0, 0)):
+        with pytest.raises(IndexError):
+            t[key]
