@@ -10,13 +10,16 @@
 namespace cmf {
 
 int OpScope::enter(void* stream, const char* who) {
-    if (ensure_init() != CMF_OK) return CMF_ERR;
     int cur = -1;
-    CMF_HIP(hipGetDevice(&cur));
-    if (cur != device()) {
-        CMF_HIP(hipSetDevice(device()));
-        back = cur;
+    if (hipGetDevice(&cur) != hipSuccess) {
+        (void)hipGetLastError();
+        cur = -1;
     }
+    // (a thread's first call makes the library's device current itself)
+    const int rc = ensure_init();
+    if (cur >= 0 && cur != device()) back = cur;
+    if (rc != CMF_OK) return CMF_ERR;
+    if (back >= 0) CMF_HIP(hipSetDevice(device()));
     if (!stream) {
         s = cmf::stream();
     } else if (stream == CMF_STREAM_NULL) {
