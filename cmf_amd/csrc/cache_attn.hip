@@ -605,9 +605,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 // one after the other (scores 1550, weights and values 2300, splitting 1850,
 // loads 1280, the barrier), and by 26000 cycles a workgroup to read and split
 // the queries and to join and write the outputs.  4100 rows of 16 heads on 8
-// behind 4000 through a window of 1024, f32: 176 us, 196 TFLOP/s of the formula
-// (588 of products); 64 rows of 32 heads on 8 over 65536 bf16 keys: 185 us, 371
-// TFLOP/s (743 of products).
+// behind 4000 through a window of 1024, f32: 177 us with the join, 195 TFLOP/s of
+// the formula (585 of products), MFMAs busy 33 % of the CUs' cycles; 64 rows of 32
+// heads on 8 over 65536 bf16 keys: 183 to 192 us from box to box, 359 TFLOP/s at
+// least (717 of products), MFMAs 34 %.  Keys and values of standard deviation
+// 0.02, whose rows need factors: 202 and 234 us.
 // grid whole + nsplit (items - whole), block 512, LDS Tile<T>::LDS: the items
 // (those in one piece, then the splits of the others) in eight runs, one to an
 // XCD (workgroups go round them), whose L2 then serves neighbouring blocks the

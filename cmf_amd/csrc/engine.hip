@@ -1892,9 +1892,11 @@ __global__ __launch_bounds__(64) void k_tree_accept(const float* __restrict__ lo
     }
 }
 
-// The path's hidden rows in order, row j = path[min(j, a)], and the tokens
-// after them (0 past the path): the (hidden, next token) pairs of the MTP
-// cache; the last one is the tip.  grid (rows), block 256.
+// The path's hidden rows in order, row j = path[min(j, a)]: with the tokens
+// after them the (hidden, next token) pairs of the MTP cache (those past the
+// path, with an earlier tree's tokens, lie behind the committed position and are
+// written again before they are read); the last one is the tip.  grid (rows),
+// block 256.
 __global__ __launch_bounds__(256) void k_tree_path(const float* __restrict__ h, int H, const TreeRes* __restrict__ r,
                                                    float* __restrict__ out, float* __restrict__ tip) {
     const int j = blockIdx.x, a = r->a;

@@ -386,7 +386,8 @@ int cmf_score(cmf_model m, const int32_t* ids, int n, float* logprobs, float* en
  * position p sees (p - window, p] and the first sinks positions; window 0: the
  * whole cache.  For the calls after it, whatever the cache holds; keys keep
  * their positions' rotation.  Up to window + sinks positions nothing changes;
- * past them a token costs the window's bytes, not the context's. */
+ * past them the attention reads the window's bytes, not the context's, and the
+ * blocks run as six launches: it pays for contexts of several windows. */
 int cmf_model_set_window(cmf_model m, int window, int sinks);
 /* sparse_distribution_into (sampler.rs:440-514) of one logits row [vocab]
  * (host) on the device sampler: ids ascending and their probabilities
@@ -469,7 +470,9 @@ int cmf_qk_rope_dev(const cmf_qk_rope_args* a);
  *   the new rows j by bit j of d_mask[i] (b <= 64: cmf_tree_masks), or without
  *   d_mask the rows j <= i under the same window (positions pos0 + j).
  * A row that sees nothing gets zeros.  What a row does not see may hold
- * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  At most 2^19
+ * anything, infinities and NaN too.  scale 0: 1 / sqrt(128).  Scores, weights
+ * and sums are f32; the factors of a product may be taken as two f16 halves (22
+ * bits, relative to a row's largest element).  At most 2^19
  * rows, 4096 query heads, 64 of them on a kv head, 2^30 positions, row strides
  * of 2^22 elements; more is refused.  out may be q (ldo = ldq).  ws: scratch of
  * at least cmf_attention_workspace bytes (at most 64 MiB) that no other call
