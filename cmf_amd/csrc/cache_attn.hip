@@ -619,6 +619,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnCall c) {
 constexpr int KT = 64, TQ = 128;     // keys of a tile, queries of a workgroup
 constexpr float SHIFT = 6.f, LAZY = 8.f;  // weights are 2^(s - m + SHIFT) <= 2^(SHIFT + LAZY)
 constexpr float FAR_SCORE = 4096.f;  // (log2 units: a product's rounding moves a weight by 2^-12 of itself here)
+constexpr float UNIT_MIN = -60.f;    // (below the exponents of all values that the tiles take)
 constexpr int KFRAG = 528;           // 32 keys x 8 dims (512 B), padded against bank conflicts
 constexpr int K_BYTES = 32 * KFRAG;  // one half (hi or lo) of the keys
 constexpr int VGROUP = 2048;         // 8 keys x 128 dims: [dim % 2][dim / 2][8 keys]
@@ -632,7 +633,7 @@ struct Tile {
     // and the codes of a block's groups (8 of K, 4 of V in 64 bytes), the key and
     // value rows' factors
     static constexpr int USE = 2 * (BUF + 128 + 8 * KT);
-    static constexpr int LDS = (USE > END_BYTES ? USE : END_BYTES) + 64;  // (and two numbers a wave)
+    static constexpr int LDS = (USE > END_BYTES ? USE : END_BYTES) + 64 + 2048;  // (and two numbers a wave, one a lane)
 };
 static_assert(Tile<float>::LDS <= 160 * 1024, "LDS of a CU");
 
@@ -950,6 +951,11 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     float m = -INFINITY, l = 0.f;
     bool odd = false;
     int* odd_at = (int*)(sm + Tile<T>::LDS - 64) + 2 * wave;  // the first and last tile with a block left out
+    // Scores far from 0 have no bits for the values' exponents: from the first such
+    // block on, m is of the scores alone and acc is in units of 2^unit, a lane's.
+    bool far = false;
+    float* unit = (float*)(sm + Tile<T>::LDS - 64 - 2048) + 64 * wave;
+    unit[lane] = 0.f;
 
     constexpr int RD = LO ? 2 : 1, MM = LO ? 3 : 2;  // fragments read and products of a step
     float16v s;         // the block's scores, by 1 / cq
@@ -1047,19 +1053,33 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
             }
         }
         mx = lanes2_max(mx);
+        far |= __builtin_amdgcn_ballot_w64((fabsf(mx) > FAR_SCORE) & (mx > -INFINITY)) != 0;
+        if (far) {
+            mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+            mx = lanes2_max(mx) * cq;
+        }
         if (__builtin_amdgcn_ballot_w64(mx > m + LAZY)) {
-            const float m1 = fmaxf(m, mx), al = exp2f(m - (m1 == -INFINITY ? 0.f : m1));
+            const float m1 = fmaxf(m, mx), down = m - (m1 == -INFINITY ? 0.f : m1), al = exp2f(down);
+            float f = al;
+            if (far) {  // (the unit goes up with m: what acc holds keeps its bits)
+                float* at = unit + lane_here();
+                const float u0 = *at, u1 = fmaxf(u0 + down, UNIT_MIN);
+                f = exp2f(u0 - u1 + down);
+                *at = u1;
+            }
             l *= al;
 #pragma unroll
-            for (int d = 0; d < 4; d++) acc[d] *= al;
+            for (int d = 0; d < 4; d++) acc[d] *= f;
             m = m1;
         }
         const float m0 = m == -INFINITY ? 0.f : m;
         float f = cq, ref = m0 - SHIFT, own = 1.f;
-        if (!groups || __builtin_amdgcn_ballot_w64(fabsf(m0) > FAR_SCORE)) {
-            // Far from 0 a score is rounded as the maximum was before that is taken
-            // off: the largest is then 0, and not what the product's rounding left.
-            // The weights without their values' factors are summed here.
+        if (!groups || far) {
+            // A score is rounded as the maximum was before that is taken off: the
+            // largest is then 0, and not what the product's rounding left.  The
+            // weights without their values' factors are summed here.
             float lu = 0.f;
 #pragma unroll
             for (int a = 0; a < 4; a++) {
@@ -1075,6 +1095,22 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
                 __builtin_amdgcn_sched_barrier(0);
             }
             l = fmaf(lu, (float)(1 << (int)SHIFT), l);
+            if (far) {
+                float* at = unit + lane_here();
+                float u0 = *at, most = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; i++) most = fmaxf(most, s[i]);
+                most = lanes2_max(most) - u0;
+                if (__builtin_amdgcn_ballot_w64(most > LAZY)) {
+                    const float up = most > LAZY ? ceilf(most) : 0.f, f1 = exp2f(-up);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) acc[d] *= f1;
+                    u0 += up;
+                    *at = u0;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] -= u0;
+            }
             f = 1.f;
             ref = -SHIFT;
             e0 = e1 = own = 0.f;
@@ -1155,13 +1191,13 @@ __global__ __launch_bounds__(512, 2) void k_attn_tiles(AttnCall c) {
     float2* ml = (float2*)((float*)sm + 8 * 32 * OROW) + wave * 32;  // (m, l)
     const int lane1 = this_lane(), n1 = lane1 & 31, h1 = lane1 >> 5;
     {
-        const float un = pow2(-(int)(SHIFT + LAZY));
+        const float un = pow2(-(int)(SHIFT + LAZY)), uo = un * exp2f(unit[lane1]);
 #pragma unroll
         for (int d = 0; d < 4; d++)
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 *(float2*)(so + n1 * OROW + 32 * d + 16 * (i >> 2) + 8 * h1 + 2 * (i & 3)) =
-                    make_float2(acc[d][i] * un, acc[d][8 + i] * un);
+                    make_float2(acc[d][i] * uo, acc[d][8 + i] * uo);
         l = lanes2_sum(l) * un;  // (m and l: the same in both lanes of a query)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }

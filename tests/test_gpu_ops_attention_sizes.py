@@ -47,6 +47,33 @@ def test_large_scores(ops, ws, b, ctx, nh, nkv, dtype, power):
     check(out.numpy(), want, tol)
 
 
+@pytest.mark.parametrize("power", [6, 12, 14, 15, 16, 20, 30])
+@pytest.mark.parametrize("sizes", [(0.01,), (1e-9,), (300.0,), (1e-3, 1.0, 4e3, 0.0), (1e-12, 1e12)])
+@pytest.mark.parametrize("b,ctx,nh,nkv", [(5, 300, 4, 2), (64, 1000, 64, 1), (900, 300, 4, 2)])
+def test_large_scores_of_values_of_other_sizes(ops, ws, b, ctx, nh, nkv, sizes, power):
+    """The same with values of another size, row by row: the mean of the values
+    of a row's largest scores, rounded by the largest of these."""
+    T = ops.DevTensor
+    r = np.random.default_rng(b + power)
+    q, k, v = tensors(r, b, ctx, nh, nkv, "float32", extra=b)
+    for t in (q, k):
+        t[...] = np.where(t < 0, -1, 1)
+        t[..., 6:] = 0
+        t *= np.float32(2.0 ** power)
+    v *= np.float32(sizes)[np.arange(ctx + b) * 7 % len(sizes)][None, :, None]
+    out = filled(ops, q.shape)
+    ops.attention(T.of(q), T.of(k), T.of(v), out, ws, pos0=ctx, scale=0.125)
+    got, hpk = out.numpy(), nh // nkv
+    for h in range(nh):
+        s = np.einsum("id,jd->ij", q[:, h], k[h // hpk])
+        s[~visible(b, ctx, 0, 0)] = -np.inf
+        top = s == s.max(1, keepdims=True)
+        val = v[h // hpk].astype(np.float64)
+        want = top @ val / top.sum(1, keepdims=True)
+        most = (top * np.abs(val).max(1)).max(1, keepdims=True)
+        check(got[:, h], want, most * U * (8 * np.sqrt(ctx + b) + 16))
+
+
 @pytest.mark.parametrize("power", [12, 20, 30])
 @pytest.mark.parametrize("b,ctx,nh,nkv,dtype", [(5, 300, 16, 8, "float32"), (9, 300, 16, 8, "bfloat16"),
                                                 (700, 900, 16, 4, "float32"), (700, 900, 16, 4, "bfloat16")])
